@@ -122,4 +122,62 @@ XGB_DLL int XGBBTrainHost(const float* X, bst_ulong rows, bst_ulong cols, const 
                           void* nodes, bst_ulong node_capacity, uint32_t* tree_sizes,
                           float* margins);
 
+/* Device operators for a model on top of leaf indices: embedding lookup with
+ * scaling, its gradient, and layer norm. No counterpart in the reference.
+ * Every buffer is the caller's device memory, dtype codes are those of
+ * XGBufferDescriptor (1 f32, 3 f16, 4 bf16, 7 i32, 8 i64), strides count
+ * elements, and the values of a matrix row are contiguous. Work is enqueued on
+ * `stream` (a cudaStream_t of `device`; -1: the calling thread's device) and
+ * not waited for; nothing is allocated, so the calls may be captured. Arguments
+ * are checked before anything is enqueued. Outputs must not overlap inputs.
+ * Workspaces (256-byte aligned, of the size that their query gives) may be
+ * reused once the call's work on the stream is done. Sums are float32 in an
+ * order that depends on the sizes alone: equal inputs give equal bits.
+ * Limits: 1 <= dim <= 2^20, 1 <= vocab < 2^31, tokens and rows < 2^31. */
+/* out[r] = scale * sum over t of token_scale[r][t] * table[tokens[r][t]]:
+ * tokens [rows][per_row] (per_row 1: a lookup), table [vocab][dim], out
+ * [rows][dim] of the table's type or one of the two f32. token_scale is f32
+ * with any strides (0: broadcast), or NULL for ones. A token below 0 is
+ * missing: it adds nothing, and its scale is not used. A token of vocab or
+ * more is not read: the row's result is NaN. */
+XGB_DLL int XGBBEmbedding(int device, const void* tokens, int token_type, bst_ulong rows, bst_ulong per_row,
+                          int64_t token_stride_row, int64_t token_stride_col, const void* table, int table_type,
+                          bst_ulong vocab, bst_ulong dim, int64_t table_stride, float scale,
+                          const float* token_scale, int64_t scale_stride_row, int64_t scale_stride_col, void* out,
+                          int out_type, int64_t out_stride, void* stream);
+/* The table's gradient, out[v] = scale * sum over tokens[r][t] == v of
+ * token_scale[r][t] * grad[r], added to what out holds when accumulate is not
+ * 0; out [vocab][dim] of grad's type or one of the two f32. Tokens below 0 and
+ * of vocab or more add nothing. */
+XGB_DLL int XGBBEmbeddingBackwardWorkspace(bst_ulong rows, bst_ulong per_row, bst_ulong vocab, bst_ulong dim,
+                                           size_t* bytes);
+XGB_DLL int XGBBEmbeddingBackward(int device, const void* grad, int grad_type, int64_t grad_stride,
+                                  const void* tokens, int token_type, bst_ulong rows, bst_ulong per_row,
+                                  int64_t token_stride_row, int64_t token_stride_col, bst_ulong vocab,
+                                  bst_ulong dim, float scale, const float* token_scale, int64_t scale_stride_row,
+                                  int64_t scale_stride_col, void* out, int out_type, int64_t out_stride,
+                                  int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+/* The scales' gradient, out[r][t] = scale * <grad[r], table[tokens[r][t]]>,
+ * contiguous: 0 for a missing token, NaN for one of vocab or more. */
+XGB_DLL int XGBBEmbeddingScaleBackward(int device, const void* grad, int grad_type, int64_t grad_stride,
+                                       const void* tokens, int token_type, bst_ulong rows, bst_ulong per_row,
+                                       int64_t token_stride_row, int64_t token_stride_col, const void* table,
+                                       int table_type, bst_ulong vocab, bst_ulong dim, int64_t table_stride,
+                                       float scale, float* out, void* stream);
+/* y = (x - mean) * rstd * weight + bias for every row of x [rows][dim], with
+ * rstd = 1 / sqrt(variance + eps). weight and bias (f32 or x's type, each may
+ * be NULL) are contiguous, mean and rstd [rows] f32 (each may be NULL). */
+XGB_DLL int XGBBLayerNorm(int device, const void* x, int type, bst_ulong rows, bst_ulong dim, int64_t x_stride,
+                          const void* weight, const void* bias, int param_type, float eps, void* y,
+                          int64_t y_stride, float* mean, float* rstd, void* stream);
+/* The gradients of x, weight and bias (dweight, dbias: [dim] of param_type,
+ * each may be NULL) from y's, with the mean and rstd that XGBBLayerNorm wrote.
+ * The workspace is needed for dweight and dbias only. */
+XGB_DLL int XGBBLayerNormBackwardWorkspace(bst_ulong rows, bst_ulong dim, size_t* bytes);
+XGB_DLL int XGBBLayerNormBackward(int device, const void* grad, int64_t grad_stride, const void* x, int type,
+                                  bst_ulong rows, bst_ulong dim, int64_t x_stride, const float* mean,
+                                  const float* rstd, const void* weight, int param_type, void* dx,
+                                  int64_t dx_stride, void* dweight, void* dbias, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 #endif /* XGB_B200_EXTENSIONS_H_ */

@@ -1,0 +1,108 @@
+// Loads, stores and small helpers shared by the operators of nn.h.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "common.h"
+#include "nn.h"
+
+namespace xgbb::nn {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N consecutive values moved as one access of up to 16 bytes each. The
+// address has to be a multiple of min(16, N * sizeof(T)).
+template <class T, int N>
+struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
+  T v[N];
+  __device__ __forceinline__ float f(int i) const { return to_f32(v[i]); }
+};
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> load(const T* p) {
+  return *reinterpret_cast<const Pack<T, N>*>(p);
+}
+template <class T, int N>
+__device__ __forceinline__ void store(T* p, const float (&f)[N]) {
+  Pack<T, N> o;
+#pragma unroll
+  for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(f[i]);
+  *reinterpret_cast<Pack<T, N>*>(p) = o;
+}
+
+// Division of 32-bit numbers by an invariant divisor: with s = ceil(log2 d)
+// and m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(n, m) + n) >> s, the
+// sum in 33 bits (Granlund and Montgomery, "Division by invariant integers
+// using multiplication", 1994).
+struct FastDiv {
+  uint32_t d, m, s;
+  FastDiv() : d(1), m(1), s(0) {}
+  explicit FastDiv(uint32_t divisor) : d(divisor), s(0) {
+    while (s < 32 && (1ull << s) < divisor) ++s;
+    m = uint32_t((((1ull << s) - divisor) << 32) / divisor + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return uint32_t((uint64_t(__umulhi(n, m)) + n) >> s);
+  }
+};
+
+__device__ __forceinline__ int64_t load_token(const void* data, bool wide, int64_t at) {
+  return wide ? static_cast<const int64_t*>(data)[at] : int64_t(static_cast<const int32_t*>(data)[at]);
+}
+
+// Whether every row starts at a multiple of n values' bytes, or of 16.
+inline bool row_aligned(const void* p, int64_t stride, uint64_t rows, size_t size, uint64_t n) {
+  const size_t b = n * size < 16 ? n * size : 16;
+  return reinterpret_cast<uintptr_t>(p) % b == 0 && (rows <= 1 || (stride * int64_t(size)) % int64_t(b) == 0);
+}
+
+inline unsigned blocks_for(uint64_t work, uint64_t per_block) {
+  return unsigned((work + per_block - 1) / per_block);
+}
+
+// Calls f with a null pointer of the type that a dtype code stands for.
+template <class F>
+void with_type(int type, F&& f) {
+  if (type == kF32) f(static_cast<float*>(nullptr));
+  else if (type == kF16) f(static_cast<__half*>(nullptr));
+  else f(static_cast<__nv_bfloat16*>(nullptr));
+}
+// The same for a pair (a, b): equal, or one of them float.
+inline bool pairs_up(int a, int b) { return a == b || a == kF32 || b == kF32; }
+template <class F>
+void with_types(int a, int b, F&& f) {
+  with_type(a, [&](auto* pa) {
+    if (a == b) f(pa, pa);
+    else if constexpr (std::is_same_v<decltype(pa), float*>) with_type(b, [&](auto* pb) { f(pa, pb); });
+    else f(pa, static_cast<float*>(nullptr));
+  });
+}
+
+// Calls f with the widest VE that the two matrices' rows allow: 16 bytes of
+// T, two 16-bit values, or one value.
+template <class T, class F>
+void with_width(const Mat& a, uint64_t a_rows, const Mat& b, uint64_t b_rows, uint64_t dim, F&& f) {
+  const auto fits = [&](uint64_t n) {
+    return dim % n == 0 && row_aligned(a.data, a.stride, a_rows, type_size(a.type), n) &&
+           row_aligned(b.data, b.stride, b_rows, type_size(b.type), n);
+  };
+  constexpr int kWide = 16 / sizeof(T);
+  if (fits(kWide)) f(std::integral_constant<int, kWide>());
+  else if (kWide > 4 && fits(2)) f(std::integral_constant<int, kWide == 4 ? 1 : 2>());
+  else f(std::integral_constant<int, 1>());
+}
+
+}  // namespace xgbb::nn
