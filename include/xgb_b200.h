@@ -124,60 +124,117 @@ XGB_DLL int XGBBTrainHost(const float* X, bst_ulong rows, bst_ulong cols, const 
 
 /* Device operators for a model on top of leaf indices: embedding lookup with
  * scaling, its gradient, and layer norm. No counterpart in the reference.
- * Every buffer is the caller's device memory, dtype codes are those of
- * XGBufferDescriptor (1 f32, 3 f16, 4 bf16, 7 i32, 8 i64), strides count
+ * Arguments come in one structure a call, which is read before the call
+ * returns. Every buffer is the caller's device memory, dtype codes are those
+ * of XGBufferDescriptor (1 f32, 3 f16, 4 bf16, 7 i32, 8 i64), strides count
  * elements, and the values of a matrix row are contiguous. Work is enqueued on
  * `stream` (a cudaStream_t of `device`; -1: the calling thread's device) and
  * not waited for; nothing is allocated, so the calls may be captured. Arguments
  * are checked before anything is enqueued. Outputs must not overlap inputs.
  * Workspaces (256-byte aligned, of the size that their query gives) may be
  * reused once the call's work on the stream is done. Sums are float32 in an
- * order that depends on the sizes alone: equal inputs give equal bits.
- * Limits: 1 <= dim <= 2^20, 1 <= vocab < 2^31, tokens and rows < 2^31. */
+ * order that depends on the sizes and alignment alone: equal inputs give equal
+ * bits. Limits: 1 <= dim <= 2^20, 1 <= vocab < 2^31, tokens and rows < 2^31. */
+
+/* tokens [rows][per_row] (per_row 1: a lookup); token_scale f32 with any
+ * strides (0: broadcast), or NULL for ones. A token below 0 is missing: it
+ * adds nothing, and its scale is not used. */
+typedef struct {
+  const void* tokens;
+  const float* token_scale;
+  bst_ulong rows, per_row;
+  int64_t stride_row, stride_col;
+  int64_t scale_stride_row, scale_stride_col;
+  int32_t type;
+  float scale;
+} XGBBTokens;
+
 /* out[r] = scale * sum over t of token_scale[r][t] * table[tokens[r][t]]:
- * tokens [rows][per_row] (per_row 1: a lookup), table [vocab][dim], out
- * [rows][dim] of the table's type or one of the two f32. token_scale is f32
- * with any strides (0: broadcast), or NULL for ones. A token below 0 is
- * missing: it adds nothing, and its scale is not used. A token of vocab or
- * more is not read: the row's result is NaN. */
-XGB_DLL int XGBBEmbedding(int device, const void* tokens, int token_type, bst_ulong rows, bst_ulong per_row,
-                          int64_t token_stride_row, int64_t token_stride_col, const void* table, int table_type,
-                          bst_ulong vocab, bst_ulong dim, int64_t table_stride, float scale,
-                          const float* token_scale, int64_t scale_stride_row, int64_t scale_stride_col, void* out,
-                          int out_type, int64_t out_stride, void* stream);
+ * table [vocab][dim], out [rows][dim] of the table's type or one of the two
+ * f32. A token of vocab or more is not read: the row's result is NaN. */
+typedef struct {
+  XGBBTokens tokens;
+  const void* table;
+  void* out;
+  void* stream;
+  bst_ulong vocab, dim;
+  int64_t table_stride, out_stride;
+  int32_t table_type, out_type, device;
+} XGBBEmbeddingArgs;
+XGB_DLL int XGBBEmbedding(const XGBBEmbeddingArgs* args);
+
 /* The table's gradient, out[v] = scale * sum over tokens[r][t] == v of
  * token_scale[r][t] * grad[r], added to what out holds when accumulate is not
  * 0; out [vocab][dim] of grad's type or one of the two f32. Tokens below 0 and
  * of vocab or more add nothing. */
+typedef struct {
+  XGBBTokens tokens;
+  const void* grad;
+  void* out;
+  void* workspace;
+  void* stream;
+  size_t workspace_bytes;
+  bst_ulong vocab, dim;
+  int64_t grad_stride, out_stride;
+  int32_t grad_type, out_type, accumulate, device;
+} XGBBEmbeddingBackwardArgs;
 XGB_DLL int XGBBEmbeddingBackwardWorkspace(bst_ulong rows, bst_ulong per_row, bst_ulong vocab, bst_ulong dim,
                                            size_t* bytes);
-XGB_DLL int XGBBEmbeddingBackward(int device, const void* grad, int grad_type, int64_t grad_stride,
-                                  const void* tokens, int token_type, bst_ulong rows, bst_ulong per_row,
-                                  int64_t token_stride_row, int64_t token_stride_col, bst_ulong vocab,
-                                  bst_ulong dim, float scale, const float* token_scale, int64_t scale_stride_row,
-                                  int64_t scale_stride_col, void* out, int out_type, int64_t out_stride,
-                                  int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+XGB_DLL int XGBBEmbeddingBackward(const XGBBEmbeddingBackwardArgs* args);
+
 /* The scales' gradient, out[r][t] = scale * <grad[r], table[tokens[r][t]]>,
- * contiguous: 0 for a missing token, NaN for one of vocab or more. */
-XGB_DLL int XGBBEmbeddingScaleBackward(int device, const void* grad, int grad_type, int64_t grad_stride,
-                                       const void* tokens, int token_type, bst_ulong rows, bst_ulong per_row,
-                                       int64_t token_stride_row, int64_t token_stride_col, const void* table,
-                                       int table_type, bst_ulong vocab, bst_ulong dim, int64_t table_stride,
-                                       float scale, float* out, void* stream);
+ * contiguous: 0 for a missing token, NaN for one of vocab or more.
+ * tokens.token_scale is not used. */
+typedef struct {
+  XGBBTokens tokens;
+  const void* grad;
+  const void* table;
+  float* out;
+  void* stream;
+  bst_ulong vocab, dim;
+  int64_t grad_stride, table_stride;
+  int32_t grad_type, table_type, device;
+} XGBBEmbeddingScaleBackwardArgs;
+XGB_DLL int XGBBEmbeddingScaleBackward(const XGBBEmbeddingScaleBackwardArgs* args);
+
 /* y = (x - mean) * rstd * weight + bias for every row of x [rows][dim], with
  * rstd = 1 / sqrt(variance + eps). weight and bias (f32 or x's type, each may
  * be NULL) are contiguous, mean and rstd [rows] f32 (each may be NULL). */
-XGB_DLL int XGBBLayerNorm(int device, const void* x, int type, bst_ulong rows, bst_ulong dim, int64_t x_stride,
-                          const void* weight, const void* bias, int param_type, float eps, void* y,
-                          int64_t y_stride, float* mean, float* rstd, void* stream);
+typedef struct {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  void* y;
+  float* mean;
+  float* rstd;
+  void* stream;
+  bst_ulong rows, dim;
+  int64_t x_stride, y_stride;
+  int32_t type, param_type, device;
+  float eps;
+} XGBBLayerNormArgs;
+XGB_DLL int XGBBLayerNorm(const XGBBLayerNormArgs* args);
+
 /* The gradients of x, weight and bias (dweight, dbias: [dim] of param_type,
  * each may be NULL) from y's, with the mean and rstd that XGBBLayerNorm wrote.
  * The workspace is needed for dweight and dbias only. */
+typedef struct {
+  const void* grad;
+  const void* x;
+  const float* mean;
+  const float* rstd;
+  const void* weight;
+  void* dx;
+  void* dweight;
+  void* dbias;
+  void* workspace;
+  void* stream;
+  size_t workspace_bytes;
+  bst_ulong rows, dim;
+  int64_t grad_stride, x_stride, dx_stride;
+  int32_t type, param_type, device;
+} XGBBLayerNormBackwardArgs;
 XGB_DLL int XGBBLayerNormBackwardWorkspace(bst_ulong rows, bst_ulong dim, size_t* bytes);
-XGB_DLL int XGBBLayerNormBackward(int device, const void* grad, int64_t grad_stride, const void* x, int type,
-                                  bst_ulong rows, bst_ulong dim, int64_t x_stride, const float* mean,
-                                  const float* rstd, const void* weight, int param_type, void* dx,
-                                  int64_t dx_stride, void* dweight, void* dbias, void* workspace,
-                                  size_t workspace_bytes, void* stream);
+XGB_DLL int XGBBLayerNormBackward(const XGBBLayerNormBackwardArgs* args);
 
 #endif /* XGB_B200_EXTENSIONS_H_ */

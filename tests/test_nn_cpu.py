@@ -2,6 +2,9 @@
 kernels to, against differences; and what the library and the Python layer
 refuse before any device is touched."""
 import ctypes
+import os
+import struct
+import subprocess
 
 import numpy as np
 import pytest
@@ -117,19 +120,44 @@ def test_wrong_arguments_are_refused(at):
 
 
 def test_library_refuses_before_it_touches_a_device():
-    # Types that do not pair up, an index type that is none, a workspace that is too small or not aligned.
+    # Types that do not pair up, an index type that is none, a workspace that is missing, not aligned or too small.
+    need = nn.embedding_backward_workspace(3, 1, 4, 2)
+
     def backward(**kw):
-        a = dict(grad_type=1, token_type=7, out_type=1, workspace=4096, size=1 << 30)
+        a = dict(grad_type=1, token_type=7, out_type=1, workspace=4096, size=need)
         a.update(kw)
-        ret = _LIB.XGBBEmbeddingBackward(-1, 4096, a["grad_type"], 2, 8192, a["token_type"], 3, 1, 1, 0, 4, 2, 1.0,
-                                         None, 0, 0, 16384, a["out_type"], 2, 0, a["workspace"], a["size"], None)
+        ret = _LIB.XGBBEmbeddingBackward(nn._pack_embedding_backward(
+            8192, 0, 3, 1, 1, 0, 0, 0, a["token_type"], 1.0, 4096, 16384, a["workspace"], 0, a["size"], 4, 2, 2, 2,
+            a["grad_type"], a["out_type"], 0, -1))
         return ret, _LIB.XGBGetLastError().decode()
 
     for kw, needle in ((dict(grad_type=3, out_type=4), "grad's type"), (dict(token_type=1), "int32"),
-                       (dict(grad_type=2), "float32"), (dict(workspace=None), "null"),
-                       (dict(workspace=4097), "aligned")):
+                       (dict(grad_type=2), "float32"), (dict(workspace=0), "null"),
+                       (dict(workspace=4097), "aligned"), (dict(size=need - 1), "smaller")):
         ret, message = backward(**kw)
         assert ret == -1 and needle in message, (kw, message)
+    for name in ("Embedding", "EmbeddingBackward", "EmbeddingScaleBackward", "LayerNorm", "LayerNormBackward"):
+        assert getattr(_LIB, "XGBB" + name)(None) == -1
+
+
+def test_argument_structures_are_packed_as_the_header_lays_them_out(tmp_path):
+    """The sizes and a few offsets of the packed arguments, against the C compiler's."""
+    source = tmp_path / "sizes.c"
+    source.write_text('''#include <stdio.h>
+#include "xgb_b200.h"
+int main(void) {
+  printf("%zu %zu %zu %zu %zu %zu", sizeof(XGBBTokens), sizeof(XGBBEmbeddingArgs), sizeof(XGBBEmbeddingBackwardArgs),
+         sizeof(XGBBEmbeddingScaleBackwardArgs), sizeof(XGBBLayerNormArgs), sizeof(XGBBLayerNormBackwardArgs));
+  return 0;
+}''')
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    program = str(tmp_path / "sizes")
+    subprocess.run(["gcc", "-I", include, str(source), "-o", program], check=True)
+    got = [int(v) for v in subprocess.run([program], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [struct.calcsize("@" + nn._TOKENS), struct.calcsize("@" + nn._TOKENS + "PPPQQqqiii4x"),
+                   len(nn._pack_embedding_backward(*[0] * 9, 1.0, *[0] * 13)),
+                   len(nn._pack_embedding_scale_backward(*[0] * 9, 1.0, *[0] * 11)),
+                   len(nn._pack_layer_norm(*[0] * 14, 1.0)), len(nn._pack_layer_norm_backward(*[0] * 19))]
 
 
 def test_workspace_sizes_are_refused_like_the_calls():

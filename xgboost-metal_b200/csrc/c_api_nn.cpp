@@ -63,32 +63,43 @@ void require_tokens(const nn::Tokens& k, uint64_t vocab, uint64_t dim) {
   if (k.rows * k.per_row) require_pointer(k.data, nn::type_size(k.type), "tokens");
 }
 
-void require_scales(const nn::Scales& s) {
-  if (s.data) require_pointer(s.data, 4, "token_scale");
+nn::Tokens tokens_of(const XGBBTokens& t, uint64_t vocab, uint64_t dim) {
+  const nn::Tokens k{t.tokens, t.type, t.rows, t.per_row, t.stride_row, t.stride_col};
+  require_tokens(k, vocab, dim);
+  require(std::isfinite(t.scale), "scale must be finite");
+  return k;
 }
 
-void require_finite(float v, const char* message) { require(std::isfinite(v), message); }
+nn::Scales scales_of(const XGBBTokens& t) {
+  if (t.token_scale) require_pointer(t.token_scale, 4, "token_scale");
+  return {t.token_scale, t.scale_stride_row, t.scale_stride_col};
+}
+
+void require_rows(uint64_t rows, uint64_t dim) {
+  require_dim(dim);
+  require(rows <= kMaxTokens, "there may be at most 2147483647 rows");
+}
+
+void require_params(int type, int param_type) {
+  require(is_float(param_type), "weight and bias must be float32 (1), float16 (3) or bfloat16 (4)");
+  require(param_type == type || param_type == nn::kF32, "weight and bias must have x's type or be float32");
+}
 
 }  // namespace
 
-XGB_DLL int XGBBEmbedding(int device, const void* tokens, int token_type, bst_ulong rows, bst_ulong per_row,
-                          int64_t token_stride_row, int64_t token_stride_col, const void* table, int table_type,
-                          bst_ulong vocab, bst_ulong dim, int64_t table_stride, float scale,
-                          const float* token_scale, int64_t scale_stride_row, int64_t scale_stride_col, void* out,
-                          int out_type, int64_t out_stride, void* stream) {
+XGB_DLL int XGBBEmbedding(const XGBBEmbeddingArgs* args) {
   return guarded([&] {
-    const nn::Tokens k{tokens, token_type, rows, per_row, token_stride_row, token_stride_col};
-    const nn::Mat w{table, table_type, table_stride}, y{out, out_type, out_stride};
-    const nn::Scales s{token_scale, scale_stride_row, scale_stride_col};
-    require_tokens(k, vocab, dim);
-    require_mat(w, vocab, dim, false, "table");
-    require_mat(y, rows, dim, true, "out");
-    require_types(table_type, out_type, "out must have the table's type, or one of them must be float32");
-    require_scales(s);
-    require_finite(scale, "scale must be finite");
-    require(!rows || out != table, "out must not be the table");
-    const OnDevice on(device);
-    nn::embedding(k, w, vocab, dim, scale, s, y, static_cast<cudaStream_t>(stream));
+    require(args != nullptr, "args is a null pointer");
+    const XGBBEmbeddingArgs& a = *args;
+    const nn::Tokens k = tokens_of(a.tokens, a.vocab, a.dim);
+    const nn::Scales s = scales_of(a.tokens);
+    const nn::Mat w{a.table, a.table_type, a.table_stride}, y{a.out, a.out_type, a.out_stride};
+    require_mat(w, a.vocab, a.dim, false, "table");
+    require_mat(y, k.rows, a.dim, true, "out");
+    require_types(a.table_type, a.out_type, "out must have the table's type, or one of them must be float32");
+    require(!k.rows || a.out != a.table, "out must not be the table");
+    const OnDevice on(a.device);
+    nn::embedding(k, w, a.vocab, a.dim, a.tokens.scale, s, y, static_cast<cudaStream_t>(a.stream));
   });
 }
 
@@ -102,107 +113,97 @@ XGB_DLL int XGBBEmbeddingBackwardWorkspace(bst_ulong rows, bst_ulong per_row, bs
   });
 }
 
-XGB_DLL int XGBBEmbeddingBackward(int device, const void* grad, int grad_type, int64_t grad_stride,
-                                  const void* tokens, int token_type, bst_ulong rows, bst_ulong per_row,
-                                  int64_t token_stride_row, int64_t token_stride_col, bst_ulong vocab,
-                                  bst_ulong dim, float scale, const float* token_scale, int64_t scale_stride_row,
-                                  int64_t scale_stride_col, void* out, int out_type, int64_t out_stride,
-                                  int accumulate, void* workspace, size_t workspace_bytes, void* stream) {
+XGB_DLL int XGBBEmbeddingBackward(const XGBBEmbeddingBackwardArgs* args) {
   return guarded([&] {
-    const nn::Tokens k{tokens, token_type, rows, per_row, token_stride_row, token_stride_col};
-    const nn::Mat g{grad, grad_type, grad_stride}, y{out, out_type, out_stride};
-    const nn::Scales s{token_scale, scale_stride_row, scale_stride_col};
-    require_tokens(k, vocab, dim);
-    require_mat(g, rows, dim, false, "grad");
-    require_mat(y, vocab, dim, true, "out");
-    require_types(grad_type, out_type, "out must have grad's type, or one of them must be float32");
-    require_scales(s);
-    require_finite(scale, "scale must be finite");
-    require(!rows || out != grad, "out must not be grad");
-    if (nn::embedding_backward_workspace(k, vocab, dim)) require_pointer(workspace, 256, "workspace");
-    const OnDevice on(device);
-    nn::embedding_backward(g, k, vocab, dim, scale, s, y, accumulate != 0, workspace, workspace_bytes,
-                           static_cast<cudaStream_t>(stream));
+    require(args != nullptr, "args is a null pointer");
+    const XGBBEmbeddingBackwardArgs& a = *args;
+    const nn::Tokens k = tokens_of(a.tokens, a.vocab, a.dim);
+    const nn::Scales s = scales_of(a.tokens);
+    const nn::Mat g{a.grad, a.grad_type, a.grad_stride}, y{a.out, a.out_type, a.out_stride};
+    require_mat(g, k.rows, a.dim, false, "grad");
+    require_mat(y, a.vocab, a.dim, true, "out");
+    require_types(a.grad_type, a.out_type, "out must have grad's type, or one of them must be float32");
+    require(!k.rows || a.out != a.grad, "out must not be grad");
+    if (const size_t need = nn::embedding_backward_workspace(k, a.vocab, a.dim)) {
+      require_pointer(a.workspace, 256, "workspace");
+      require(a.workspace_bytes >= need, "the workspace is smaller than its query says");
+    }
+    const OnDevice on(a.device);
+    nn::embedding_backward(g, k, a.vocab, a.dim, a.tokens.scale, s, y, a.accumulate != 0, a.workspace,
+                           static_cast<cudaStream_t>(a.stream));
   });
 }
 
-XGB_DLL int XGBBEmbeddingScaleBackward(int device, const void* grad, int grad_type, int64_t grad_stride,
-                                       const void* tokens, int token_type, bst_ulong rows, bst_ulong per_row,
-                                       int64_t token_stride_row, int64_t token_stride_col, const void* table,
-                                       int table_type, bst_ulong vocab, bst_ulong dim, int64_t table_stride,
-                                       float scale, float* out, void* stream) {
+XGB_DLL int XGBBEmbeddingScaleBackward(const XGBBEmbeddingScaleBackwardArgs* args) {
   return guarded([&] {
-    const nn::Tokens k{tokens, token_type, rows, per_row, token_stride_row, token_stride_col};
-    const nn::Mat g{grad, grad_type, grad_stride}, w{table, table_type, table_stride};
-    require_tokens(k, vocab, dim);
-    require_mat(g, rows, dim, false, "grad");
-    require_mat(w, vocab, dim, false, "table");
-    require_types(table_type, grad_type, "grad must have the table's type, or one of them must be float32");
-    require_finite(scale, "scale must be finite");
-    if (rows * per_row) require_pointer(out, 4, "out");
-    const OnDevice on(device);
-    nn::embedding_scale_backward(g, k, w, vocab, dim, scale, out, static_cast<cudaStream_t>(stream));
+    require(args != nullptr, "args is a null pointer");
+    const XGBBEmbeddingScaleBackwardArgs& a = *args;
+    const nn::Tokens k = tokens_of(a.tokens, a.vocab, a.dim);
+    const nn::Mat g{a.grad, a.grad_type, a.grad_stride}, w{a.table, a.table_type, a.table_stride};
+    require_mat(g, k.rows, a.dim, false, "grad");
+    require_mat(w, a.vocab, a.dim, false, "table");
+    require_types(a.table_type, a.grad_type, "grad must have the table's type, or one of them must be float32");
+    if (k.rows * k.per_row) require_pointer(a.out, 4, "out");
+    const OnDevice on(a.device);
+    nn::embedding_scale_backward(g, k, w, a.vocab, a.dim, a.tokens.scale, a.out,
+                                 static_cast<cudaStream_t>(a.stream));
   });
 }
 
-XGB_DLL int XGBBLayerNorm(int device, const void* x, int type, bst_ulong rows, bst_ulong dim, int64_t x_stride,
-                          const void* weight, const void* bias, int param_type, float eps, void* y,
-                          int64_t y_stride, float* mean, float* rstd, void* stream) {
+XGB_DLL int XGBBLayerNorm(const XGBBLayerNormArgs* args) {
   return guarded([&] {
-    const nn::Mat in{x, type, x_stride}, out{y, type, y_stride};
-    require_dim(dim);
-    require(rows <= kMaxTokens, "there may be at most 2147483647 rows");
-    require_mat(in, rows, dim, false, "x");
-    require_mat(out, rows, dim, true, "y");
-    require(is_float(param_type), "weight and bias must be float32 (1), float16 (3) or bfloat16 (4)");
-    require(param_type == type || param_type == nn::kF32, "weight and bias must have x's type or be float32");
-    if (weight) require_pointer(weight, nn::type_size(param_type), "weight");
-    if (bias) require_pointer(bias, nn::type_size(param_type), "bias");
-    if (mean) require_pointer(mean, 4, "mean");
-    if (rstd) require_pointer(rstd, 4, "rstd");
-    require(std::isfinite(eps) && eps >= 0.0f, "eps must be finite and not negative");
-    require(!rows || x != y, "y must not be x");
-    const OnDevice on(device);
-    nn::layer_norm(in, rows, dim, weight, bias, param_type, eps, out, mean, rstd,
-                   static_cast<cudaStream_t>(stream));
+    require(args != nullptr, "args is a null pointer");
+    const XGBBLayerNormArgs& a = *args;
+    const nn::Mat in{a.x, a.type, a.x_stride}, out{a.y, a.type, a.y_stride};
+    require_rows(a.rows, a.dim);
+    require_mat(in, a.rows, a.dim, false, "x");
+    require_mat(out, a.rows, a.dim, true, "y");
+    require_params(a.type, a.param_type);
+    if (a.weight) require_pointer(a.weight, nn::type_size(a.param_type), "weight");
+    if (a.bias) require_pointer(a.bias, nn::type_size(a.param_type), "bias");
+    if (a.mean) require_pointer(a.mean, 4, "mean");
+    if (a.rstd) require_pointer(a.rstd, 4, "rstd");
+    require(std::isfinite(a.eps) && a.eps >= 0.0f, "eps must be finite and not negative");
+    require(!a.rows || a.x != a.y, "y must not be x");
+    const OnDevice on(a.device);
+    nn::layer_norm(in, a.rows, a.dim, a.weight, a.bias, a.param_type, a.eps, out, a.mean, a.rstd,
+                   static_cast<cudaStream_t>(a.stream));
   });
 }
 
 XGB_DLL int XGBBLayerNormBackwardWorkspace(bst_ulong rows, bst_ulong dim, size_t* bytes) {
   return guarded([&] {
     require(bytes != nullptr, "bytes is a null pointer");
-    require_dim(dim);
-    require(rows <= kMaxTokens, "there may be at most 2147483647 rows");
+    require_rows(rows, dim);
     *bytes = nn::layer_norm_backward_workspace(rows, dim);
   });
 }
 
-XGB_DLL int XGBBLayerNormBackward(int device, const void* grad, int64_t grad_stride, const void* x, int type,
-                                  bst_ulong rows, bst_ulong dim, int64_t x_stride, const float* mean,
-                                  const float* rstd, const void* weight, int param_type, void* dx,
-                                  int64_t dx_stride, void* dweight, void* dbias, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
+XGB_DLL int XGBBLayerNormBackward(const XGBBLayerNormBackwardArgs* args) {
   return guarded([&] {
-    const nn::Mat g{grad, type, grad_stride}, in{x, type, x_stride}, out{dx, type, dx_stride};
-    require_dim(dim);
-    require(rows <= kMaxTokens, "there may be at most 2147483647 rows");
-    require_mat(g, rows, dim, false, "grad");
-    require_mat(in, rows, dim, false, "x");
-    require_mat(out, rows, dim, true, "dx");
-    require(is_float(param_type), "weight must be float32 (1), float16 (3) or bfloat16 (4)");
-    require(param_type == type || param_type == nn::kF32, "weight must have x's type or be float32");
-    if (rows) {
-      require_pointer(mean, 4, "mean");
-      require_pointer(rstd, 4, "rstd");
+    require(args != nullptr, "args is a null pointer");
+    const XGBBLayerNormBackwardArgs& a = *args;
+    const nn::Mat g{a.grad, a.type, a.grad_stride}, in{a.x, a.type, a.x_stride}, out{a.dx, a.type, a.dx_stride};
+    require_rows(a.rows, a.dim);
+    require_mat(g, a.rows, a.dim, false, "grad");
+    require_mat(in, a.rows, a.dim, false, "x");
+    require_mat(out, a.rows, a.dim, true, "dx");
+    require_params(a.type, a.param_type);
+    if (a.rows) {
+      require_pointer(a.mean, 4, "mean");
+      require_pointer(a.rstd, 4, "rstd");
     }
-    if (weight) require_pointer(weight, nn::type_size(param_type), "weight");
-    if (dweight) require_pointer(dweight, nn::type_size(param_type), "dweight");
-    if (dbias) require_pointer(dbias, nn::type_size(param_type), "dbias");
-    require(!rows || (dx != grad && dx != x), "dx must be neither grad nor x");
-    if ((dweight || dbias) && nn::layer_norm_backward_workspace(rows, dim))
-      require_pointer(workspace, 256, "workspace");
-    const OnDevice on(device);
-    nn::layer_norm_backward(g, in, mean, rstd, rows, dim, weight, param_type, out, dweight, dbias, workspace,
-                            workspace_bytes, static_cast<cudaStream_t>(stream));
+    if (a.weight) require_pointer(a.weight, nn::type_size(a.param_type), "weight");
+    if (a.dweight) require_pointer(a.dweight, nn::type_size(a.param_type), "dweight");
+    if (a.dbias) require_pointer(a.dbias, nn::type_size(a.param_type), "dbias");
+    require(!a.rows || (a.dx != a.grad && a.dx != a.x), "dx must be neither grad nor x");
+    const size_t need = a.dweight || a.dbias ? nn::layer_norm_backward_workspace(a.rows, a.dim) : 0;
+    if (need) {
+      require_pointer(a.workspace, 256, "workspace");
+      require(a.workspace_bytes >= need, "the workspace is smaller than its query says");
+    }
+    const OnDevice on(a.device);
+    nn::layer_norm_backward(g, in, a.mean, a.rstd, a.rows, a.dim, a.weight, a.param_type, out, a.dweight, a.dbias,
+                            a.workspace, static_cast<cudaStream_t>(a.stream));
   });
 }

@@ -353,11 +353,10 @@ size_t embedding_backward_workspace(const Tokens& k, uint64_t, uint64_t dim) {
 }
 
 void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64_t dim, float scale,
-                        const Scales& s, const Mat& out, bool accumulate, void* workspace, size_t bytes,
+                        const Scales& s, const Mat& out, bool accumulate, void* workspace,
                         cudaStream_t stream) {
   const uint32_t n = uint32_t(k.rows * k.per_row);
   const Layout at(n, dim);
-  require(bytes >= at.bytes, "the workspace is smaller than its query says");
   char* w = static_cast<char*>(workspace);
   const auto u32 = [&](size_t offset) { return reinterpret_cast<uint32_t*>(w + offset); };
   int from = 0;

@@ -6,6 +6,7 @@
 // All arithmetic is float32; the variance is the mean square of the centred
 // values, never a difference of two large sums. Results are rounded once.
 #include <algorithm>
+#include <initializer_list>
 
 #include "nn_device.cuh"
 
@@ -14,8 +15,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// The sum of one value a thread over the block, in every thread. `part` holds
-// one float a warp.
+// Sums N values a thread over the block, in every thread. `part` is not the
+// one that the call before used, so one barrier does: whoever still reads that
+// one has not passed this one.
 template <int N>
 __device__ __forceinline__ void block_sum(float (&v)[N], float (*part)[N]) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -23,7 +25,6 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float (*part)[N]) {
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int m = 16; m; m >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], m);
-  __syncthreads();
   if (lane == 0)
 #pragma unroll
     for (int i = 0; i < N; ++i) part[warp][i] = v[i];
@@ -36,125 +37,391 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float (*part)[N]) {
   }
 }
 
-// A block a row, any length: three passes over the row.
-template <class T, class P, int VE>
-__global__ void __launch_bounds__(kThreads)
-    norm_kernel(const T* __restrict__ x, int64_t x_stride, uint64_t rows, uint32_t dim, const P* __restrict__ w,
-                const P* __restrict__ b, float eps, T* __restrict__ y, int64_t y_stride, float* __restrict__ mean,
-                float* __restrict__ rstd) {
-  __shared__ float part[32][1];
-  for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* xr = x + int64_t(row) * x_stride;
-    float sum[1] = {0.0f};
-    for (uint32_t c = threadIdx.x * VE; c < dim; c += kThreads * VE) {
-      const auto v = load<T, VE>(xr + c);
+// Sums N values a thread over groups of G lanes, or over the block.
+template <bool WARP, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], uint32_t G, float (*part)[N]) {
+  if constexpr (WARP) {
 #pragma unroll
-      for (int e = 0; e < VE; ++e) sum[0] += v.f(e);
-    }
-    block_sum<1>(sum, part);
-    const float m = sum[0] / float(dim);
-    float square[1] = {0.0f};
-    for (uint32_t c = threadIdx.x * VE; c < dim; c += kThreads * VE) {
-      const auto v = load<T, VE>(xr + c);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) square[0] = fmaf(v.f(e) - m, v.f(e) - m, square[0]);
-    }
-    block_sum<1>(square, part);
-    const float q = 1.0f / sqrtf(square[0] / float(dim) + eps);
-    if (threadIdx.x == 0) {
-      if (mean) mean[row] = m;
-      if (rstd) rstd[row] = q;
-    }
-    for (uint32_t c = threadIdx.x * VE; c < dim; c += kThreads * VE) {
-      const auto v = load<T, VE>(xr + c);
-      float r[VE];
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        r[e] = (v.f(e) - m) * q;
-        if (w) r[e] *= to_f32(w[c + e]);
-        if (b) r[e] += to_f32(b[c + e]);
-      }
-      store<T, VE>(y + int64_t(row) * y_stride + c, r);
-    }
+    for (int i = 0; i < N; ++i)
+      for (uint32_t m = G >> 1; m; m >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], m);
+  } else {
+    block_sum<N>(v, part);
   }
 }
 
-// dx, a block a row, any length.
-template <class T, class P, int VE>
-__global__ void __launch_bounds__(kThreads)
-    norm_dx_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x, int64_t x_stride,
-                   const float* __restrict__ mean, const float* __restrict__ rstd, uint64_t rows, uint32_t dim,
-                   const P* __restrict__ w, T* __restrict__ dx, int64_t dx_stride) {
-  __shared__ float part[32][2];
-  for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* xr = x + int64_t(row) * x_stride;
-    const T* gr = grad + int64_t(row) * grad_stride;
-    const float m = mean[row], q = rstd[row];
-    float sum[2] = {0.0f, 0.0f};
-    for (uint32_t c = threadIdx.x * VE; c < dim; c += kThreads * VE) {
-      const auto v = load<T, VE>(xr + c);
-      const auto d = load<T, VE>(gr + c);
+// Forward. A row stays in registers between its load and its store: CH pieces
+// of VE values a thread, in their own type. WARP: 2^lg lanes hold a row, else
+// the block does.
+template <class T, class P, int VE, int CH, bool WARP>
+__global__ void __launch_bounds__(WARP ? kThreads : 1024)
+    norm_kernel(const T* __restrict__ x, int64_t x_stride, uint64_t rows, uint32_t dim, const P* __restrict__ w,
+                const P* __restrict__ b, float eps, T* __restrict__ y, int64_t y_stride, float* __restrict__ mean,
+                float* __restrict__ rstd, int lg) {
+  __shared__ float part[2][32][1];
+  const uint32_t G = WARP ? 1u << lg : blockDim.x;
+  const uint32_t at = WARP ? threadIdx.x & (G - 1) : threadIdx.x;
+  const uint64_t row = WARP ? uint64_t(blockIdx.x) * (kThreads >> lg) + (threadIdx.x >> lg) : blockIdx.x;
+  const bool here = row < rows;
+  const T* xr = x + int64_t(row) * x_stride;
+  Pack<T, VE> v[CH];
+  float sum[1] = {0.0f};
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float g = w ? d.f(e) * to_f32(w[c + e]) : d.f(e);
-        sum[0] += g;
-        sum[1] = fmaf(g, (v.f(e) - m) * q, sum[1]);
+  for (int i = 0; i < CH; ++i) {
+    const uint32_t c = (at + i * G) * VE;
+    if (here && c < dim) v[i] = load<T, VE>(xr + c);
+  }
+#pragma unroll
+  for (int i = 0; i < CH; ++i)
+    if (here && (at + i * G) * VE < dim)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) sum[0] += v[i].f(e);
+  row_sum<WARP, 1>(sum, G, part[0]);
+  const float m = sum[0] / float(dim);
+  float square[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < CH; ++i)
+    if (here && (at + i * G) * VE < dim)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) square[0] = fmaf(v[i].f(e) - m, v[i].f(e) - m, square[0]);
+  row_sum<WARP, 1>(square, G, part[1]);
+  const float q = 1.0f / sqrtf(square[0] / float(dim) + eps);
+  if (!here) return;
+  if (at == 0) {
+    if (mean) mean[row] = m;
+    if (rstd) rstd[row] = q;
+  }
+  T* yr = y + int64_t(row) * y_stride;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const uint32_t c = (at + i * G) * VE;
+    if (c >= dim) continue;
+    float r[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) r[e] = (v[i].f(e) - m) * q;
+    if (w) {
+      const auto f = load<P, VE>(w + c);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) r[e] *= f.f(e);
+    }
+    if (b) {
+      const auto f = load<P, VE>(b + c);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) r[e] += f.f(e);
+    }
+    store<T, VE>(yr + c, r);
+  }
+}
+
+// Forward for rows that registers do not hold: three passes, a block a row.
+template <class T, class P, int VE>
+__global__ void __launch_bounds__(1024)
+    norm_long_kernel(const T* __restrict__ x, int64_t x_stride, uint64_t rows, uint32_t dim,
+                     const P* __restrict__ w, const P* __restrict__ b, float eps, T* __restrict__ y,
+                     int64_t y_stride, float* __restrict__ mean, float* __restrict__ rstd) {
+  __shared__ float part[2][32][1];
+  const uint64_t row = blockIdx.x;
+  const T* xr = x + int64_t(row) * x_stride;
+  float sum[1] = {0.0f};
+  for (uint32_t c = threadIdx.x * VE; c < dim; c += blockDim.x * VE) {
+    const auto v = load<T, VE>(xr + c);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) sum[0] += v.f(e);
+  }
+  block_sum<1>(sum, part[0]);
+  const float m = sum[0] / float(dim);
+  float square[1] = {0.0f};
+  for (uint32_t c = threadIdx.x * VE; c < dim; c += blockDim.x * VE) {
+    const auto v = load<T, VE>(xr + c);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) square[0] = fmaf(v.f(e) - m, v.f(e) - m, square[0]);
+  }
+  block_sum<1>(square, part[1]);
+  const float q = 1.0f / sqrtf(square[0] / float(dim) + eps);
+  if (threadIdx.x == 0) {
+    if (mean) mean[row] = m;
+    if (rstd) rstd[row] = q;
+  }
+  for (uint32_t c = threadIdx.x * VE; c < dim; c += blockDim.x * VE) {
+    const auto v = load<T, VE>(xr + c);
+    float r[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      r[e] = (v.f(e) - m) * q;
+      if (w) r[e] *= to_f32(w[c + e]);
+      if (b) r[e] += to_f32(b[c + e]);
+    }
+    store<T, VE>(y + int64_t(row) * y_stride + c, r);
+  }
+}
+
+// Backward. A thread owns CH pieces of VE columns, 8 values in all, of every
+// row that its group takes: the rows' dx from registers, and the columns' sums
+// of dy h and dy kept in registers from the first row to the last. The next
+// row's values are under way while this one's are summed (packed 16-bit values,
+// whose registers leave room). WARP: 2^lg lanes hold a row, else the block does.
+// parts[block][2][dim] gets the block's sums.
+template <class T, class P, int VE, int CH, bool WARP>
+__global__ void __launch_bounds__(WARP ? kThreads : 1024, WARP ? 4 : 1)
+    norm_grad_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x, int64_t x_stride,
+                     const float* __restrict__ mean, const float* __restrict__ rstd, uint64_t rows, uint32_t dim,
+                     const P* __restrict__ w, T* __restrict__ dx, int64_t dx_stride, float* __restrict__ parts,
+                     int lg) {
+  constexpr bool kAhead = sizeof(T) == 2 && VE == 8;
+  constexpr int E = CH * VE;
+  __shared__ float part[2][32][2];
+  const uint32_t G = WARP ? 1u << lg : blockDim.x;
+  const uint32_t at = WARP ? threadIdx.x & (G - 1) : threadIdx.x;
+  const uint32_t groups = WARP ? kThreads >> lg : 1;
+  const uint64_t step = uint64_t(gridDim.x) * groups;
+  const float inverse = 1.0f / float(dim);
+  float wv[E], dw[E] = {}, db[E] = {};
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const uint32_t c = (at + i * G) * VE;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) wv[i * VE + e] = w && c + e < dim ? to_f32(w[c + e]) : 1.0f;
+  }
+  Pack<T, VE> nv[CH], nd[CH];
+  float nm = 0.0f, nq = 0.0f;
+  const auto fetch = [&](uint64_t row) {
+    if (row >= rows) return;
+    nm = mean[row];
+    nq = rstd[row];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const uint32_t c = (at + i * G) * VE;
+      if (c < dim) {
+        nv[i] = load<T, VE>(x + int64_t(row) * x_stride + c);
+        nd[i] = load<T, VE>(grad + int64_t(row) * grad_stride + c);
       }
     }
-    block_sum<2>(sum, part);
-    const float a = sum[0] / float(dim), bb = sum[1] / float(dim);
-    for (uint32_t c = threadIdx.x * VE; c < dim; c += kThreads * VE) {
-      const auto v = load<T, VE>(xr + c);
-      const auto d = load<T, VE>(gr + c);
+  };
+  uint64_t row = uint64_t(blockIdx.x) * groups + (WARP ? threadIdx.x >> lg : 0);
+  const uint64_t turns = (rows - min(rows, uint64_t(blockIdx.x) * groups) + step - 1) / step;
+  if (kAhead) fetch(row);
+  for (uint64_t turn = 0; turn < turns; ++turn, row += step) {
+    if (!kAhead) fetch(row);
+    Pack<T, VE> v[CH], d[CH];
+    const float m = nm, q = nq;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) v[i] = nv[i], d[i] = nd[i];
+    if (kAhead) fetch(row + step);
+    const bool here = row < rows;
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (here && (at + i * G) * VE < dim)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const int j = i * VE + e;
+          const float h = (v[i].f(e) - m) * q, g = d[i].f(e) * wv[j];
+          sum[0] += g;
+          sum[1] = fmaf(g, h, sum[1]);
+          dw[j] = fmaf(d[i].f(e), h, dw[j]);
+          db[j] += d[i].f(e);
+        }
+    row_sum<WARP, 2>(sum, G, part[turn & 1]);
+    const float a = sum[0] * inverse, bb = sum[1] * inverse;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const uint32_t c = (at + i * G) * VE;
+      if (!here || c >= dim) continue;
       float r[VE];
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float g = w ? d.f(e) * to_f32(w[c + e]) : d.f(e);
-        r[e] = q * (g - a - (v.f(e) - m) * q * bb);
+        const float h = (v[i].f(e) - m) * q, g = d[i].f(e) * wv[i * VE + e];
+        r[e] = q * (g - a - h * bb);
       }
       store<T, VE>(dx + int64_t(row) * dx_stride + c, r);
     }
   }
+  if (!parts) return;
+  float* out = parts + uint64_t(blockIdx.x) * 2 * dim;
+  if constexpr (WARP) {
+    // The groups' sums: over the warp's lanes, then over the warps in order.
+    extern __shared__ float sums[];  // [warps][2][G * E]
+    for (uint32_t m = G; m < 32; m <<= 1)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        dw[j] += __shfl_xor_sync(0xffffffffu, dw[j], m);
+        db[j] += __shfl_xor_sync(0xffffffffu, db[j], m);
+      }
+    const uint32_t width = G * E, warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) < G)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const uint32_t c = (at + (j / VE) * G) * VE + j % VE;
+        sums[(warp * 2) * width + c] = dw[j];
+        sums[(warp * 2 + 1) * width + c] = db[j];
+      }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < 2 * width; i += kThreads) {
+      const uint32_t which = i / width, c = i % width;
+      float s = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kThreads / 32; ++q) s += sums[q * 2 * width + i];
+      if (c < dim) out[which * dim + c] = s;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const uint32_t c = (at + i * G) * VE;
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (c + e < dim) {
+          out[c + e] = dw[i * VE + e];
+          out[dim + c + e] = db[i * VE + e];
+        }
+    }
+  }
 }
 
-constexpr uint32_t kMaxParts = 296;
+// dx for rows that registers do not hold: two passes, a block a row.
+template <class T, class P, int VE>
+__global__ void __launch_bounds__(1024)
+    norm_grad_long_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x,
+                          int64_t x_stride, const float* __restrict__ mean, const float* __restrict__ rstd,
+                          uint32_t dim, const P* __restrict__ w, T* __restrict__ dx, int64_t dx_stride) {
+  __shared__ float part[32][2];
+  const uint64_t row = blockIdx.x;
+  const T* xr = x + int64_t(row) * x_stride;
+  const T* gr = grad + int64_t(row) * grad_stride;
+  const float m = mean[row], q = rstd[row];
+  float sum[2] = {0.0f, 0.0f};
+  for (uint32_t c = threadIdx.x * VE; c < dim; c += blockDim.x * VE) {
+    const auto v = load<T, VE>(xr + c);
+    const auto d = load<T, VE>(gr + c);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float g = w ? d.f(e) * to_f32(w[c + e]) : d.f(e);
+      sum[0] += g;
+      sum[1] = fmaf(g, (v.f(e) - m) * q, sum[1]);
+    }
+  }
+  block_sum<2>(sum, part);
+  const float a = sum[0] / float(dim), bb = sum[1] / float(dim);
+  for (uint32_t c = threadIdx.x * VE; c < dim; c += blockDim.x * VE) {
+    const auto v = load<T, VE>(xr + c);
+    const auto d = load<T, VE>(gr + c);
+    float r[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float g = w ? d.f(e) * to_f32(w[c + e]) : d.f(e);
+      r[e] = q * (g - a - (v.f(e) - m) * q * bb);
+    }
+    store<T, VE>(dx + int64_t(row) * dx_stride + c, r);
+  }
+}
 
-uint32_t part_count(uint64_t rows) { return uint32_t(std::min<uint64_t>(kMaxParts, (rows + 15) / 16)); }
-
-// Block (x, y) sums the column tile y over the rows x, x + gridDim.x, ... into
-// parts[x][2][dim]: the weight's gradient, then the bias's.
-template <class T>
+// The column sums that go with norm_grad_long_kernel: block (x, y) sums the
+// column tile y over a span of rows.
+template <class T, int VE>
 __global__ void __launch_bounds__(kThreads)
     norm_columns_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x, int64_t x_stride,
                         const float* __restrict__ mean, const float* __restrict__ rstd, uint64_t rows, uint32_t dim,
                         float* __restrict__ parts) {
-  const uint32_t c = blockIdx.y * kThreads + threadIdx.x;
+  constexpr int U = 4;
+  const uint32_t c = (blockIdx.y * kThreads + threadIdx.x) * VE;
   if (c >= dim) return;
-  float dw = 0.0f, db = 0.0f;
-  for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const float d = to_f32(grad[int64_t(row) * grad_stride + c]);
-    dw = fmaf(d, (to_f32(x[int64_t(row) * x_stride + c]) - mean[row]) * rstd[row], dw);
-    db += d;
+  float dw[VE] = {}, db[VE] = {};
+  for (uint64_t row = blockIdx.x; row < rows; row += uint64_t(gridDim.x) * U) {
+    Pack<T, VE> v[U], d[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t r = row + uint64_t(u) * gridDim.x;
+      if (r < rows) {
+        v[u] = load<T, VE>(x + int64_t(r) * x_stride + c);
+        d[u] = load<T, VE>(grad + int64_t(r) * grad_stride + c);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t r = row + uint64_t(u) * gridDim.x;
+      if (r >= rows) break;
+      const float m = mean[r], q = rstd[r];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        dw[e] = fmaf(d[u].f(e), (v[u].f(e) - m) * q, dw[e]);
+        db[e] += d[u].f(e);
+      }
+    }
   }
-  parts[(uint64_t(blockIdx.x) * 2) * dim + c] = dw;
-  parts[(uint64_t(blockIdx.x) * 2 + 1) * dim + c] = db;
+  float* out = parts + uint64_t(blockIdx.x) * 2 * dim + c;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    out[e] = dw[e];
+    out[dim + e] = db[e];
+  }
 }
 
-// The parts' sums, in their order.
+// The parts' sums: 32 columns a block (of dw's and db's 2 dim), each warp
+// every eighth part, then the warps in order.
 template <class P>
 __global__ void __launch_bounds__(kThreads)
     norm_parts_kernel(const float* __restrict__ parts, uint32_t count, uint32_t dim, P* __restrict__ dw,
                       P* __restrict__ db) {
-  const uint32_t c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= dim) return;
-  float a = 0.0f, b = 0.0f;
-  for (uint32_t p = 0; p < count; ++p) {
-    a += parts[uint64_t(p) * 2 * dim + c];
-    b += parts[(uint64_t(p) * 2 + 1) * dim + c];
-  }
-  if (dw) dw[c] = from_f32<P>(a);
-  if (db) db[c] = from_f32<P>(b);
+  constexpr int kWarps = kThreads / 32, U = 8;
+  __shared__ float sums[kWarps][32];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (c < 2 * dim)
+    for (uint32_t p = warp; p < count; p += kWarps * U) {
+      float v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = p + u * kWarps < count ? parts[uint64_t(p + u * kWarps) * 2 * dim + c] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) s += v[u];
+    }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp || c >= 2 * dim) return;
+#pragma unroll
+  for (int q = 1; q < kWarps; ++q) s += sums[q][lane];
+  P* to = c < dim ? dw : db;
+  if (to) to[c < dim ? c : c - dim] = from_f32<P>(s);
 }
+
+bool param_aligned(const void* p, size_t size, uint64_t n) {
+  return reinterpret_cast<uintptr_t>(p) % std::min<size_t>(16, n * size) == 0;
+}
+
+// Calls f with the widest VE that every matrix and vector allows.
+template <class T, class F>
+void with_norm_width(std::initializer_list<Mat> mats, std::initializer_list<const void*> vectors, int param_type,
+                     uint64_t rows, uint64_t dim, F&& f) {
+  const auto fits = [&](uint64_t n) {
+    bool ok = dim % n == 0;
+    for (const Mat& m : mats) ok = ok && row_aligned(m.data, m.stride, rows, type_size(m.type), n);
+    for (const void* p : vectors) ok = ok && param_aligned(p, type_size(param_type), n);
+    return ok;
+  };
+  constexpr int kWide = 16 / sizeof(T);
+  if (fits(kWide)) f(std::integral_constant<int, kWide>());
+  else if (kWide > 4 && fits(2)) f(std::integral_constant<int, kWide == 4 ? 1 : 2>());
+  else f(std::integral_constant<int, 1>());
+}
+
+// How norm_grad_kernel takes rows of `dim` values: lanes or threads a row,
+// blocks, and rows that its registers hold.
+struct GradPlan {
+  bool fits, warp;
+  int lg = 0;
+  uint32_t threads = 0, blocks = 0;
+  GradPlan(uint64_t rows, uint64_t dim) : fits(dim <= 8192), warp(dim <= 256) {
+    if (!fits) {
+      blocks = uint32_t(std::min<uint64_t>(296, (rows + 15) / 16));
+      return;
+    }
+    if (warp) {
+      while ((8ull << lg) < dim) ++lg;
+      threads = kThreads;
+      blocks = uint32_t(std::min<uint64_t>(148 * 4, (rows + (kThreads >> lg) - 1) / (kThreads >> lg)));
+      return;
+    }
+    threads = uint32_t((dim + 255) / 256 * 32);
+    blocks = uint32_t(std::min<uint64_t>(148 * (1024 / threads), rows));
+  }
+};
 
 }  // namespace
 
@@ -164,50 +431,84 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
   with_types(x.type, param_type, [&](auto* pt, auto* pp) {
     using T = std::remove_pointer_t<decltype(pt)>;
     using P = std::remove_pointer_t<decltype(pp)>;
-    with_width<T>(x, rows, y, rows, dim, [&](auto width) {
-      norm_kernel<T, P, decltype(width)::value>
-          <<<unsigned(std::min<uint64_t>(rows, 1u << 30)), kThreads, 0, stream>>>(
-              static_cast<const T*>(x.data), x.stride, rows, uint32_t(dim), static_cast<const P*>(weight),
-              static_cast<const P*>(bias), eps, static_cast<T*>(const_cast<void*>(y.data)), y.stride, mean, rstd);
+    const T* in = static_cast<const T*>(x.data);
+    T* out = static_cast<T*>(const_cast<void*>(y.data));
+    const P *w = static_cast<const P*>(weight), *b = static_cast<const P*>(bias);
+    with_norm_width<T>({x, y}, {weight, bias}, param_type, rows, dim, [&](auto width) {
+      constexpr int VE = decltype(width)::value;
+      constexpr int kMost = std::min(32 / VE, 16);  // pieces of a thread
+      const uint64_t pieces = (dim + VE - 1) / VE;
+      const auto go = [&](auto count, auto in_warp, unsigned blocks, unsigned threads, int lg) {
+        norm_kernel<T, P, VE, decltype(count)::value, decltype(in_warp)::value><<<blocks, threads, 0, stream>>>(
+            in, x.stride, rows, uint32_t(dim), w, b, eps, out, y.stride, mean, rstd, lg);
+      };
+      const auto pick = [&](uint64_t need, auto in_warp, unsigned blocks, unsigned threads, int lg) {
+        if (need <= 1) go(std::integral_constant<int, 1>(), in_warp, blocks, threads, lg);
+        else if (need <= 2) go(std::integral_constant<int, 2>(), in_warp, blocks, threads, lg);
+        else if (need <= 4) go(std::integral_constant<int, 4>(), in_warp, blocks, threads, lg);
+        else if constexpr (kMost >= 8) {
+          if (need <= 8 || kMost == 8) go(std::integral_constant<int, 8>(), in_warp, blocks, threads, lg);
+          else go(std::integral_constant<int, kMost>(), in_warp, blocks, threads, lg);
+        }
+      };
+      if (pieces <= 32 * kMost && rows >= 148) {
+        int lg = 0;
+        while (lg < 5 && (1ull << lg) < pieces) ++lg;
+        pick((pieces + (1u << lg) - 1) >> lg, std::true_type(), blocks_for(rows, kThreads >> lg), kThreads, lg);
+        return;
+      }
+      if (pieces > 1024 * kMost) {
+        norm_long_kernel<T, P, VE><<<unsigned(rows), 1024, 0, stream>>>(in, x.stride, rows, uint32_t(dim), w, b,
+                                                                      eps, out, y.stride, mean, rstd);
+        return;
+      }
+      // Many rows: as few threads a row as hold it. Few: as many as it has pieces.
+      const uint64_t each = rows >= 148 ? std::min<uint64_t>(kMost, 4) : 1;
+      const uint64_t threads = std::min<uint64_t>(1024, ((pieces + each - 1) / each + 31) / 32 * 32);
+      pick((pieces + threads - 1) / threads, std::false_type(), unsigned(rows), unsigned(threads), 0);
     });
   });
   XGBB_CUDA(cudaGetLastError());
 }
 
-size_t layer_norm_backward_workspace(uint64_t rows, uint64_t dim) { return size_t(part_count(rows)) * 2 * dim * 4; }
+size_t layer_norm_backward_workspace(uint64_t rows, uint64_t dim) {
+  return size_t(GradPlan(rows, dim).blocks) * 2 * dim * 4;
+}
 
 void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const float* rstd, uint64_t rows,
                          uint64_t dim, const void* weight, int param_type, const Mat& dx, void* dweight,
-                         void* dbias, void* workspace, size_t bytes, cudaStream_t stream) {
-  require(!(dweight || dbias) || bytes >= layer_norm_backward_workspace(rows, dim),
-          "the workspace is smaller than its query says");
+                         void* dbias, void* workspace, cudaStream_t stream) {
+  const bool params = dweight || dbias;
+  const GradPlan plan(rows, dim);
+  float* parts = params ? static_cast<float*>(workspace) : nullptr;
   with_types(x.type, param_type, [&](auto* pt, auto* pp) {
     using T = std::remove_pointer_t<decltype(pt)>;
     using P = std::remove_pointer_t<decltype(pp)>;
     const T* g = static_cast<const T*>(grad.data);
     const T* v = static_cast<const T*>(x.data);
-    if (rows) {
-      // The widths that x and dx allow, and grad too.
-      with_width<T>(x, rows, dx, rows, dim, [&](auto wide) {
-        constexpr int VE = decltype(wide)::value;
-        const auto go = [&](auto width) {
-          norm_dx_kernel<T, P, decltype(width)::value>
-              <<<unsigned(std::min<uint64_t>(rows, 1u << 30)), kThreads, 0, stream>>>(
-                  g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), static_cast<const P*>(weight),
-                  static_cast<T*>(const_cast<void*>(dx.data)), dx.stride);
-        };
-        if (row_aligned(grad.data, grad.stride, rows, sizeof(T), VE)) go(std::integral_constant<int, VE>());
-        else go(std::integral_constant<int, 1>());
+    const P* w = static_cast<const P*>(weight);
+    T* out = static_cast<T*>(const_cast<void*>(dx.data));
+    if (rows)
+      with_norm_width<T>({grad, x, dx}, {}, param_type, rows, dim, [&](auto width) {
+        constexpr int VE = decltype(width)::value;
+        if (plan.fits && plan.warp) {
+          norm_grad_kernel<T, P, VE, 8 / VE, true>
+              <<<plan.blocks, plan.threads, (kThreads / 32) * 2 * (8u << plan.lg) * 4, stream>>>(
+                  g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts, plan.lg);
+        } else if (plan.fits) {
+          norm_grad_kernel<T, P, VE, 8 / VE, false><<<plan.blocks, plan.threads, 0, stream>>>(
+              g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts, 0);
+        } else {
+          norm_grad_long_kernel<T, P, VE><<<unsigned(rows), 1024, 0, stream>>>(
+              g, grad.stride, v, x.stride, mean, rstd, uint32_t(dim), w, out, dx.stride);
+          if (params)
+            norm_columns_kernel<T, VE><<<dim3(plan.blocks, blocks_for(dim, kThreads * VE)), kThreads, 0, stream>>>(
+                g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), parts);
+        }
       });
-    }
-    if (!dweight && !dbias) return;
-    float* parts = static_cast<float*>(workspace);
-    const uint32_t count = part_count(rows);
-    if (count)
-      norm_columns_kernel<T><<<dim3(count, blocks_for(dim, kThreads)), kThreads, 0, stream>>>(
-          g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), parts);
-    norm_parts_kernel<P><<<blocks_for(dim, kThreads), kThreads, 0, stream>>>(
-        parts, count, uint32_t(dim), static_cast<P*>(dweight), static_cast<P*>(dbias));
+    if (params)
+      norm_parts_kernel<P><<<blocks_for(2 * dim, 32), kThreads, 0, stream>>>(
+          parts, plan.blocks, uint32_t(dim), static_cast<P*>(dweight), static_cast<P*>(dbias));
   });
   XGBB_CUDA(cudaGetLastError());
 }

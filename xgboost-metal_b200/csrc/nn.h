@@ -42,7 +42,7 @@ void embedding(const Tokens& k, const Mat& table, uint64_t vocab, uint64_t dim, 
 // out[v] (+)= scale * sum over tokens[r][t] == v of scales[r][t] * grad[r].
 size_t embedding_backward_workspace(const Tokens& k, uint64_t vocab, uint64_t dim);
 void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64_t dim, float scale,
-                        const Scales& s, const Mat& out, bool accumulate, void* workspace, size_t bytes,
+                        const Scales& s, const Mat& out, bool accumulate, void* workspace,
                         cudaStream_t stream);
 // out[r][t] = scale * <grad[r], table[tokens[r][t]]>, contiguous.
 void embedding_scale_backward(const Mat& grad, const Tokens& k, const Mat& table, uint64_t vocab, uint64_t dim,
@@ -56,6 +56,6 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
 size_t layer_norm_backward_workspace(uint64_t rows, uint64_t dim);
 void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const float* rstd, uint64_t rows,
                          uint64_t dim, const void* weight, int param_type, const Mat& dx, void* dweight,
-                         void* dbias, void* workspace, size_t bytes, cudaStream_t stream);
+                         void* dbias, void* workspace, cudaStream_t stream);
 
 }  // namespace xgbb::nn

@@ -22,6 +22,7 @@ inputs give equal bits. These functions have no counterpart in the reference.
 import contextlib
 import ctypes
 import json
+import struct
 import sys
 
 import numpy as np
@@ -32,66 +33,75 @@ __all__ = ["embedding", "embedding_backward", "embedding_backward_workspace", "e
            "layer_norm", "layer_norm_backward", "layer_norm_backward_workspace", "leaf_tokens"]
 
 _F32, _F16, _BF16, _I32, _I64 = 1, 3, 4, 7, 8
-_P, _I, _U, _S, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_int64, ctypes.c_float
-_TOKENS = [_P, _I, _U, _U, _S, _S]
+_FLOATS, _INTS = (_F32, _F16, _BF16), (_I32, _I64)
 
-_LIB.XGBBEmbedding.argtypes = [_I] + _TOKENS + [_P, _I, _U, _U, _S, _F, _P, _S, _S, _P, _I, _S, _P]
-_LIB.XGBBEmbeddingBackwardWorkspace.argtypes = [_U, _U, _U, _U, _P]
-_LIB.XGBBEmbeddingBackward.argtypes = ([_I, _P, _I, _S] + _TOKENS +
-                                       [_U, _U, _F, _P, _S, _S, _P, _I, _S, _I, _P, ctypes.c_size_t, _P])
-_LIB.XGBBEmbeddingScaleBackward.argtypes = [_I, _P, _I, _S] + _TOKENS + [_P, _I, _U, _U, _S, _F, _P, _P]
-_LIB.XGBBLayerNorm.argtypes = [_I, _P, _I, _U, _U, _S, _P, _P, _I, _F, _P, _S, _P, _P, _P]
-_LIB.XGBBLayerNormBackwardWorkspace.argtypes = [_U, _U, _P]
-_LIB.XGBBLayerNormBackward.argtypes = [_I, _P, _S, _P, _I, _U, _U, _S, _P, _P, _P, _I, _P, _S, _P, _P, _P,
-                                       ctypes.c_size_t, _P]
+# The argument structures of include/xgb_b200.h.
+_TOKENS = "PPQQqqqqif"
+_pack_embedding = struct.Struct("@" + _TOKENS + "PPPQQqqiii4x").pack
+_pack_embedding_backward = struct.Struct("@" + _TOKENS + "PPPPNQQqqiiii").pack
+_pack_embedding_scale_backward = struct.Struct("@" + _TOKENS + "PPPPQQqqiii4x").pack
+_pack_layer_norm = struct.Struct("@PPPPPPPQQqqiiif").pack
+_pack_layer_norm_backward = struct.Struct("@PPPPPPPPPPNQQqqqiii4x").pack
+
+for _name in ("XGBBEmbedding", "XGBBEmbeddingBackward", "XGBBEmbeddingScaleBackward", "XGBBLayerNorm",
+              "XGBBLayerNormBackward"):
+    getattr(_LIB, _name).argtypes = [ctypes.c_char_p]
+_SIZES = [ctypes.c_uint64] * 4
+_LIB.XGBBEmbeddingBackwardWorkspace.argtypes = _SIZES + [ctypes.c_void_p]
+_LIB.XGBBLayerNormBackwardWorkspace.argtypes = _SIZES[:2] + [ctypes.c_void_p]
 
 _TYPESTR = {"<f4": _F32, "<f2": _F16, "<i4": _I32, "<i8": _I64}
-_torch_codes = {}
+_codes, _dtypes = {}, {}  # torch's dtypes by code and back, filled when the first tensor comes
+_raw_stream = None
 
 
-def _torch():
-    return sys.modules["torch"]
+def _know_torch():
+    global _raw_stream
+    t = sys.modules["torch"]
+    _codes.update({t.float32: _F32, t.float16: _F16, t.bfloat16: _BF16, t.int32: _I32, t.int64: _I64})
+    _dtypes.update({c: d for d, c in _codes.items()})
+    _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or \
+        (lambda device: t.cuda.current_stream(device).cuda_stream)
 
 
-def _torch_code(dtype):
-    if not _torch_codes:
-        t = _torch()
-        _torch_codes.update({t.float32: _F32, t.float16: _F16, t.bfloat16: _BF16, t.int32: _I32, t.int64: _I64})
-    return _torch_codes.get(dtype, 0)
+def _call(function, args):
+    if function(args) != 0:
+        _check_call(-1)
 
 
-class _View:
-    """What a call needs of an array: pointer, shape, strides (in elements),
-    dtype code, device ordinal (-1: the current one) and the tensor, if it is
-    one."""
-    __slots__ = ("ptr", "shape", "strides", "code", "device", "tensor")
+def _view(a, what):
+    """What a call needs of an array: (pointer, shape, strides in elements,
+    dtype code, device ordinal or -1 for the current one, the tensor or None)."""
+    try:
+        ptr = a.data_ptr()
+    except AttributeError:
+        return _interface_view(a, what)
+    if not a.is_cuda:
+        raise XGBoostError("%s must be in device memory" % what)
+    if not _codes:
+        _know_torch()
+    return ptr, a.shape, a.stride(), _codes.get(a.dtype, 0), a.get_device(), a
 
-    def __init__(self, a, what):
-        if hasattr(a, "data_ptr"):
-            if not a.is_cuda:
-                raise XGBoostError("%s must be in device memory" % what)
-            self.ptr, self.shape, self.strides = a.data_ptr(), a.shape, a.stride()
-            self.code, self.device, self.tensor = _torch_code(a.dtype), a.get_device(), a
-            return
-        inf = getattr(a, "__cuda_array_interface__", None)
-        if inf is None:
-            raise XGBoostError("%s must be a device array: a CUDA tensor, or an object with a "
-                               "__cuda_array_interface__" % what)
-        self.ptr, self.shape, self.code = int(inf["data"][0] or 0), tuple(inf["shape"]), _TYPESTR.get(inf["typestr"], 0)
-        self.device, self.tensor = -1, None
-        if inf.get("mask") is not None:
-            raise XGBoostError("%s must not be masked" % what)
-        size = int(inf["typestr"][2:])
-        if inf.get("strides") is None:
-            strides, step = [], 1
-            for n in reversed(self.shape):
-                strides.append(step)
-                step *= n
-            self.strides = tuple(reversed(strides))
-        else:
-            if any(s % size for s in inf["strides"]):
-                raise XGBoostError("%s has strides that are no multiples of its item size" % what)
-            self.strides = tuple(s // size for s in inf["strides"])
+
+def _interface_view(a, what):
+    inf = getattr(a, "__cuda_array_interface__", None)
+    if inf is None:
+        raise XGBoostError("%s must be a device array: a CUDA tensor, or an object with a "
+                           "__cuda_array_interface__" % what)
+    if inf.get("mask") is not None:
+        raise XGBoostError("%s must not be masked" % what)
+    shape, size = tuple(inf["shape"]), int(inf["typestr"][2:])
+    if inf.get("strides") is None:
+        strides, step = [], 1
+        for n in reversed(shape):
+            strides.append(step)
+            step *= n
+        strides = tuple(reversed(strides))
+    else:
+        if any(s % size for s in inf["strides"]):
+            raise XGBoostError("%s has strides that are no multiples of its item size" % what)
+        strides = tuple(s // size for s in inf["strides"])
+    return int(inf["data"][0] or 0), shape, strides, _TYPESTR.get(inf["typestr"], 0), -1, None
 
 
 def _flat(shape, strides, what):
@@ -110,24 +120,25 @@ def _flat(shape, strides, what):
 
 def _matrix(v, what):
     """(rows, columns, row stride) of an array of rows with contiguous values."""
-    if not v.shape:
-        raise XGBoostError("%s must have at least one dimension" % what)
-    if v.code not in (_F32, _F16, _BF16):
+    shape, strides = v[1], v[2]
+    if v[3] not in _FLOATS:
         raise XGBoostError("%s must be float32, float16 or bfloat16" % what)
-    n = v.shape[-1]
-    if n > 1 and v.strides[-1] != 1:
+    if not shape:
+        raise XGBoostError("%s must have at least one dimension" % what)
+    n = shape[-1]
+    if n > 1 and strides[-1] != 1:
         raise XGBoostError("%s must have contiguous values in its last dimension" % what)
-    if len(v.shape) == 2:
-        return v.shape[0], n, v.strides[0]
-    rows, stride = _flat(v.shape[:-1], v.strides[:-1], what)
+    if len(shape) == 2:
+        return shape[0], n, strides[0]
+    rows, stride = _flat(shape[:-1], strides[:-1], what)
     return rows, n, stride
 
 
 def _token_grid(v, bag):
     """(rows, per_row, row stride, column stride, leading shape) of tokens."""
-    if v.code not in (_I32, _I64):
+    shape, strides = v[1], v[2]
+    if v[3] not in _INTS:
         raise XGBoostError("tokens must be int32 or int64")
-    shape, strides = v.shape, v.strides
     if not bag:
         if len(shape) == 1:
             return shape[0], 1, strides[0], 0, shape
@@ -136,62 +147,70 @@ def _token_grid(v, bag):
     if not shape:
         raise XGBoostError("a bag of tokens must have at least one dimension")
     if len(shape) == 2:
-        return shape[0], shape[1], strides[0], strides[1], shape[:-1]
+        return shape[0], shape[1], strides[0], strides[1], shape[:1]
     rows, stride = _flat(shape[:-1], strides[:-1], "tokens")
     return rows, shape[-1], stride, strides[-1], shape[:-1]
 
 
-def _token_scale(scale, tokens, bag):
-    """The view and strides of token_scale, broadcast to the tokens' shape."""
+def _scale_grid(scale, tokens, bag):
+    """(pointer, row stride, column stride, device) of token_scale, broadcast to
+    the tokens' shape."""
     if scale is None:
-        return None, 0, 0
+        return 0, 0, 0, -1
     if hasattr(scale, "expand"):
         try:
-            scale = scale.expand(tokens.shape)
+            scale = scale.expand(tokens[1])
         except RuntimeError as e:
             raise XGBoostError("token_scale does not broadcast to the tokens' shape: %s" % e) from None
-    v = _View(scale, "token_scale")
-    if tuple(v.shape) != tuple(tokens.shape):
+    ptr, shape, strides, code, device, _ = _view(scale, "token_scale")
+    if tuple(shape) != tuple(tokens[1]):
         raise XGBoostError("token_scale must have the tokens' shape")
-    if v.code != _F32:
+    if code != _F32:
         raise XGBoostError("token_scale must be float32")
     if not bag:
-        return v, _flat(v.shape, v.strides, "token_scale")[1], 0
-    return v, _flat(v.shape[:-1], v.strides[:-1], "token_scale")[1], v.strides[-1]
+        return ptr, _flat(shape, strides, "token_scale")[1], 0, device
+    return ptr, _flat(shape[:-1], strides[:-1], "token_scale")[1], strides[-1], device
 
 
-def _device(*views):
+def _one_device(*devices):
     device = -1
-    for v in views:
-        if v is not None and v.device >= 0:
-            if device >= 0 and v.device != device:
+    for d in devices:
+        if d >= 0 and d != device:
+            if device >= 0:
                 raise XGBoostError("the arrays are on different devices")
-            device = v.device
+            device = d
     return device
 
 
-def _handle(stream, device, tensor):
-    """The stream's handle."""
-    if stream is None:
-        return _torch().cuda.current_stream(device).cuda_stream if tensor is not None else 0
+def _stream_handle(stream):
     for name in ("cuda_stream", "ptr"):
         if hasattr(stream, name):
             return int(getattr(stream, name))
     return int(stream)
 
 
+def _handle(stream, device, v):
+    """The handle of the stream to use: torch's current one for tensors."""
+    if v[5] is not None:
+        return _raw_stream(device)
+    return 0 if stream is None else _stream_handle(stream)
+
+
 @contextlib.contextmanager
 def _on(stream, tensors):
     """Makes a given stream torch's current one, so that results and workspaces
     come from its own memory, and tells torch that the inputs are used on it."""
-    tensors = [t for t in tensors if hasattr(t, "record_stream")]
-    if not tensors:
+    torch = sys.modules["torch"]
+    tensors = [t for t in tensors if hasattr(t, "record_stream") and t.is_cuda]
+    if not tensors:  # refused by the call
         yield
         return
-    torch, device = _torch(), tensors[0].device
-    handle = _handle(stream, device, None)
-    s = stream if isinstance(stream, torch.cuda.Stream) else \
-        torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    device = tensors[0].device
+    if isinstance(stream, torch.cuda.Stream):
+        s = stream
+    else:
+        handle = _stream_handle(stream)
+        s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
     with torch.cuda.stream(s):
         for t in tensors:
             t.record_stream(s)
@@ -199,66 +218,82 @@ def _on(stream, tensors):
 
 
 def _dtype_code(dtype):
-    if isinstance(dtype, (str, np.dtype, type)):
+    if dtype in _codes:
+        return _codes[dtype]
+    try:
         return _TYPESTR.get(np.dtype(dtype).str, 0)
-    return _torch_code(dtype)
+    except TypeError:
+        return 0
 
 
 def _result(out, shape, code, like, what):
-    """The array that a result goes to, and its view: `out`, checked, or a new
-    one of like's kind."""
+    """(array, pointer, dtype code, row stride, device) of a result: `out`,
+    checked, or a new one of like's kind. Any float type does where code is 0."""
     if out is None:
-        if like.tensor is None:
+        tensor = like[5]
+        if tensor is None:
             raise XGBoostError("%s must be given where the inputs are no tensors" % what)
-        dtype = like.tensor.dtype if code == like.code else \
-            next((d for d, c in _torch_codes.items() if c == code), None)
-        if dtype is None:
+        if code not in _FLOATS:
             raise XGBoostError("%s must be float32, float16 or bfloat16" % what)
-        out = like.tensor.new_empty(shape, dtype=dtype)
-        return out, _View(out, what)
-    v = _View(out, what)
-    if tuple(v.shape) != tuple(shape):
+        out = tensor.new_empty(shape) if code == like[3] else tensor.new_empty(shape, dtype=_dtypes[code])
+        return out, out.data_ptr(), code, shape[-1] if shape else 1, like[4]
+    v = _view(out, what)
+    if tuple(v[1]) != tuple(shape):
         raise XGBoostError("%s must have the shape %s" % (what, tuple(shape)))
-    if code and v.code != code:
+    if code and v[3] != code:
         raise XGBoostError("%s has another type than it must have" % what)
-    return out, v
+    return out, v[0], v[3], _matrix(v, what)[2] if shape else 1, v[4]
 
 
-def _vector(v, n, codes, what):
-    if v is None:
-        return
-    if tuple(v.shape) != (n,) or (n > 1 and v.strides[0] != 1):
-        raise XGBoostError("%s must be %d contiguous values" % (what, n))
-    if v.code not in codes:
+def _flat_result(out, shape, code, like, what):
+    """_result for contiguous values."""
+    got = _result(out, shape, code, like, what)
+    if out is not None:
+        v = _view(out, what)
+        n, stride = _flat(v[1], v[2], what)
+        if n > 1 and stride != 1:
+            raise XGBoostError("%s must be contiguous" % what)
+    return got
+
+
+def _vector(a, dim, code, what):
+    """(pointer, dtype code, device) of weight or bias."""
+    ptr, shape, strides, own, device, _ = _view(a, what)
+    if tuple(shape) != (dim,) or (dim > 1 and strides[0] != 1):
+        raise XGBoostError("%s must be %d contiguous values" % (what, dim))
+    if own != code and own != _F32:
         raise XGBoostError("%s must be float32 or have x's type" % what)
+    return ptr, own, device
 
 
-def _stats(v, lead, rows, what):
-    if tuple(v.shape) != tuple(lead) or (rows > 1 and _flat(v.shape, v.strides, what)[1] != 1):
+def _row_values(a, lead, what):
+    """(pointer, device) of mean or rstd."""
+    ptr, shape, strides, code, device, _ = _view(a, what)
+    if tuple(shape) != tuple(lead):
         raise XGBoostError("%s must be contiguous, one value a row" % what)
-    if v.code != _F32:
+    n, stride = _flat(shape, strides, what)
+    if n > 1 and stride != 1:
+        raise XGBoostError("%s must be contiguous, one value a row" % what)
+    if code != _F32:
         raise XGBoostError("%s must be float32" % what)
+    return ptr, device
 
 
-def _workspace(workspace, size, like):
+def _space(workspace, size, like):
+    """(workspace, pointer) of `size` bytes."""
     if not size:
-        return None
+        return None, 0
     if workspace is None:
-        if like.tensor is None:
+        if like[5] is None:
             raise XGBoostError("workspace must be given where the inputs are no tensors")
-        workspace = like.tensor.new_empty(size, dtype=_torch().uint8)
-        return workspace
-    v = _View(workspace, "workspace")
-    items = int(np.prod(v.shape, dtype=np.int64))
-    width = v.tensor.element_size() if v.tensor is not None else \
-        int(workspace.__cuda_array_interface__["typestr"][2:])
-    if items * width < size or (items > 1 and _flat(v.shape, v.strides, "workspace")[1] != 1):
+        workspace = like[5].new_empty(size, dtype=sys.modules["torch"].uint8)
+        return workspace, workspace.data_ptr()
+    v = _view(workspace, "workspace")
+    n, stride = _flat(v[1], v[2], "workspace")
+    width = v[5].element_size() if v[5] is not None else int(workspace.__cuda_array_interface__["typestr"][2:])
+    if n * width < size or (n > 1 and stride != 1):
         raise XGBoostError("workspace must be %d contiguous bytes" % size)
-    return workspace
-
-
-def _pointer(array):
-    return None if array is None else _View(array, "workspace").ptr
+    return workspace, v[0]
 
 
 def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None, out_dtype=None, stream=None):
@@ -275,19 +310,19 @@ def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None
         with _on(stream, (tokens, table, token_scale, out)):
             return embedding(tokens, table, scale=scale, token_scale=token_scale, bag=bag, out=out,
                              out_dtype=out_dtype)
-    k, w = _View(tokens, "tokens"), _View(table, "table")
-    if len(w.shape) != 2:
-        raise XGBoostError("table must have two dimensions")
+    k, w = _view(tokens, "tokens"), _view(table, "table")
     rows, per_row, stride_row, stride_col, lead = _token_grid(k, bag)
     vocab, dim, table_stride = _matrix(w, "table")
-    s, s_row, s_col = _token_scale(token_scale, k, bag)
-    code = w.code if out_dtype is None else _dtype_code(out_dtype)
-    out, y = _result(out, (*lead, dim), 0 if out is not None and out_dtype is None else code, w, "out")
-    y_rows, _, y_stride = _matrix(y, "out")
-    device = _device(k, w, s, y)
-    _check_call(_LIB.XGBBEmbedding(device, k.ptr, k.code, rows, per_row, stride_row, stride_col, w.ptr, w.code, vocab,
-                                   dim, table_stride, scale, s and s.ptr, s_row, s_col, y.ptr, y.code, y_stride,
-                                   _handle(stream, device, w.tensor)))
+    if len(w[1]) != 2:
+        raise XGBoostError("table must have two dimensions")
+    s, s_row, s_col, s_device = _scale_grid(token_scale, k, bag)
+    code = w[3] if out_dtype is None else _dtype_code(out_dtype)
+    out, y, code, y_stride, y_device = _result(out, (*lead, dim), 0 if out is not None and out_dtype is None else code,
+                                               w, "out")
+    device = _one_device(w[4], k[4], s_device, y_device)
+    _call(_LIB.XGBBEmbedding, _pack_embedding(
+        k[0], s, rows, per_row, stride_row, stride_col, s_row, s_col, k[3], scale, w[0], y,
+        _handle(stream, device, w), vocab, dim, table_stride, y_stride, w[3], code, device))
     return out
 
 
@@ -309,24 +344,23 @@ def embedding_backward(grad, tokens, vocab, *, scale=1.0, token_scale=None, bag=
         with _on(stream, (grad, tokens, token_scale, out, workspace)):
             return embedding_backward(grad, tokens, vocab, scale=scale, token_scale=token_scale, bag=bag, out=out,
                                       out_dtype=out_dtype, accumulate=accumulate, workspace=workspace)
-    g, k = _View(grad, "grad"), _View(tokens, "tokens")
+    g, k = _view(grad, "grad"), _view(tokens, "tokens")
     rows, per_row, stride_row, stride_col, lead = _token_grid(k, bag)
-    g_rows, dim, g_stride = _matrix(g, "grad")
-    if tuple(g.shape[:-1]) != tuple(lead):
+    _, dim, g_stride = _matrix(g, "grad")
+    if g[1][:-1] != lead:
         raise XGBoostError("grad must have the shape of the lookup's result")
     if accumulate and out is None:
         raise XGBoostError("accumulate needs out")
-    s, s_row, s_col = _token_scale(token_scale, k, bag)
-    code = g.code if out_dtype is None else _dtype_code(out_dtype)
-    out, y = _result(out, (vocab, dim), 0 if out is not None and out_dtype is None else code, g, "out")
-    _, _, y_stride = _matrix(y, "out")
-    device = _device(g, k, s, y)
+    s, s_row, s_col, s_device = _scale_grid(token_scale, k, bag)
     size = embedding_backward_workspace(rows, per_row, vocab, dim)
-    workspace = _workspace(workspace, size, g)
-    _check_call(_LIB.XGBBEmbeddingBackward(device, g.ptr, g.code, g_stride, k.ptr, k.code, rows, per_row, stride_row,
-                                           stride_col, vocab, dim, scale, s and s.ptr, s_row, s_col, y.ptr, y.code,
-                                           y_stride, bool(accumulate), _pointer(workspace), size,
-                                           _handle(stream, device, g.tensor)))
+    code = g[3] if out_dtype is None else _dtype_code(out_dtype)
+    out, y, code, y_stride, y_device = _result(out, (vocab, dim), 0 if out is not None and out_dtype is None else code,
+                                               g, "out")
+    device = _one_device(g[4], k[4], s_device, y_device)
+    workspace, space = _space(workspace, size, g)
+    _call(_LIB.XGBBEmbeddingBackward, _pack_embedding_backward(
+        k[0], s, rows, per_row, stride_row, stride_col, s_row, s_col, k[3], scale, g[0], y, space,
+        _handle(stream, device, g), size, vocab, dim, g_stride, y_stride, g[3], code, bool(accumulate), device))
     return out
 
 
@@ -338,21 +372,19 @@ def embedding_scale_backward(grad, tokens, table, *, scale=1.0, bag=False, out=N
     if stream is not None and hasattr(grad, "data_ptr"):
         with _on(stream, (grad, tokens, table, out)):
             return embedding_scale_backward(grad, tokens, table, scale=scale, bag=bag, out=out)
-    g, k, w = _View(grad, "grad"), _View(tokens, "tokens"), _View(table, "table")
-    if len(w.shape) != 2:
-        raise XGBoostError("table must have two dimensions")
+    g, k, w = _view(grad, "grad"), _view(tokens, "tokens"), _view(table, "table")
     rows, per_row, stride_row, stride_col, lead = _token_grid(k, bag)
     vocab, dim, table_stride = _matrix(w, "table")
-    g_rows, g_dim, g_stride = _matrix(g, "grad")
-    if tuple(g.shape[:-1]) != tuple(lead) or g_dim != dim:
+    if len(w[1]) != 2:
+        raise XGBoostError("table must have two dimensions")
+    _, g_dim, g_stride = _matrix(g, "grad")
+    if g[1][:-1] != lead or g_dim != dim:
         raise XGBoostError("grad must have the shape of the lookup's result")
-    out, y = _result(out, tuple(k.shape), _F32, g, "out")
-    if rows * per_row > 1 and _flat(y.shape, y.strides, "out")[1] != 1:
-        raise XGBoostError("out must be contiguous")
-    device = _device(g, k, w, y)
-    _check_call(_LIB.XGBBEmbeddingScaleBackward(device, g.ptr, g.code, g_stride, k.ptr, k.code, rows, per_row,
-                                                stride_row, stride_col, w.ptr, w.code, vocab, dim, table_stride,
-                                                scale, y.ptr, _handle(stream, device, g.tensor)))
+    out, y, _, _, y_device = _flat_result(out, tuple(k[1]), _F32, g, "out")
+    device = _one_device(g[4], k[4], w[4], y_device)
+    _call(_LIB.XGBBEmbeddingScaleBackward, _pack_embedding_scale_backward(
+        k[0], 0, rows, per_row, stride_row, stride_col, 0, 0, k[3], scale, g[0], w[0], y,
+        _handle(stream, device, g), vocab, dim, g_stride, table_stride, g[3], w[3], device))
     return out
 
 
@@ -364,25 +396,24 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
     if stream is not None and hasattr(x, "data_ptr"):
         with _on(stream, (x, weight, bias, out, mean, rstd)):
             return layer_norm(x, weight, bias, eps=eps, out=out, mean=mean, rstd=rstd)
-    v = _View(x, "x")
+    v = _view(x, "x")
     rows, dim, stride = _matrix(v, "x")
-    w = None if weight is None else _View(weight, "weight")
-    b = None if bias is None else _View(bias, "bias")
-    _vector(w, dim, (v.code, _F32), "weight")
-    _vector(b, dim, (v.code, _F32), "bias")
-    if w is not None and b is not None and w.code != b.code:
+    w, w_code, w_device = (0, 0, -1) if weight is None else _vector(weight, dim, v[3], "weight")
+    b, b_code, b_device = (0, 0, -1) if bias is None else _vector(bias, dim, v[3], "bias")
+    if w_code and b_code and w_code != b_code:
         raise XGBoostError("weight and bias must have the same type")
-    param = w.code if w is not None else b.code if b is not None else _F32
-    lead = v.shape[:-1]
-    out, y = _result(out, v.shape, v.code, v, "out")
-    mean, m = _result(mean, lead, _F32, v, "mean")
-    rstd, q = _result(rstd, lead, _F32, v, "rstd")
-    _stats(m, lead, rows, "mean")
-    _stats(q, lead, rows, "rstd")
-    _, _, y_stride = _matrix(y, "out")
-    device = _device(v, w, b, y, m, q)
-    _check_call(_LIB.XGBBLayerNorm(device, v.ptr, v.code, rows, dim, stride, w and w.ptr, b and b.ptr, param, eps,
-                                   y.ptr, y_stride, m.ptr, q.ptr, _handle(stream, device, v.tensor)))
+    lead = v[1][:-1]
+    out, y, _, y_stride, y_device = _result(out, v[1], v[3], v, "out")
+    if mean is None and rstd is None and v[5] is not None:
+        mean, rstd = v[5].new_empty((2, *lead), dtype=_dtypes[_F32]).unbind()
+        m, q, m_device, q_device = mean.data_ptr(), rstd.data_ptr(), v[4], v[4]
+    else:
+        mean, m, _, _, m_device = _flat_result(mean, lead, _F32, v, "mean")
+        rstd, q, _, _, q_device = _flat_result(rstd, lead, _F32, v, "rstd")
+    device = _one_device(v[4], w_device, b_device, y_device, m_device, q_device)
+    _call(_LIB.XGBBLayerNorm, _pack_layer_norm(
+        v[0], w, b, y, m, q, _handle(stream, device, v), rows, dim, stride, y_stride, v[3],
+        w_code or b_code or _F32, device, eps))
     return out, mean, rstd
 
 
@@ -403,36 +434,30 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
         with _on(stream, (grad, x, mean, rstd, weight, out, dweight, dbias, workspace)):
             return layer_norm_backward(grad, x, mean, rstd, weight, bias_grad=bias_grad, out=out, dweight=dweight,
                                        dbias=dbias, workspace=workspace)
-    g, v = _View(grad, "grad"), _View(x, "x")
+    g, v = _view(grad, "grad"), _view(x, "x")
     rows, dim, stride = _matrix(v, "x")
     _, _, g_stride = _matrix(g, "grad")
-    if tuple(g.shape) != tuple(v.shape) or g.code != v.code:
+    if g[1] != v[1] or g[3] != v[3]:
         raise XGBoostError("grad must have x's shape and type")
-    m, q = _View(mean, "mean"), _View(rstd, "rstd")
-    lead = v.shape[:-1]
-    _stats(m, lead, rows, "mean")
-    _stats(q, lead, rows, "rstd")
-    w = None if weight is None else _View(weight, "weight")
-    _vector(w, dim, (v.code, _F32), "weight")
-    out, dx = _result(out, v.shape, v.code, v, "out")
-    _, _, dx_stride = _matrix(dx, "out")
-    dw = db = None
-    size = 0
-    if w is not None:
-        dweight, dw = _result(dweight, (dim,), w.code, w, "dweight")
-        _vector(dw, dim, (w.code,), "dweight")
+    lead = v[1][:-1]
+    m, m_device = _row_values(mean, lead, "mean")
+    q, q_device = _row_values(rstd, lead, "rstd")
+    out, dx, _, dx_stride, dx_device = _result(out, v[1], v[3], v, "out")
+    w = dw = db = space = size = 0
+    w_code, w_device, dw_device, db_device = _F32, -1, -1, -1
+    if weight is not None:
+        w, w_code, w_device = _vector(weight, dim, v[3], "weight")
+        dweight, dw, _, _, dw_device = _flat_result(dweight, (dim,), w_code, v, "dweight")
         if bias_grad:
-            dbias, db = _result(dbias, (dim,), w.code, w, "dbias")
-            _vector(db, dim, (w.code,), "dbias")
+            dbias, db, _, _, db_device = _flat_result(dbias, (dim,), w_code, v, "dbias")
         size = layer_norm_backward_workspace(rows, dim)
-        workspace = _workspace(workspace, size, v)
+        workspace, space = _space(workspace, size, v)
     elif dweight is not None or dbias is not None:
         raise XGBoostError("dweight and dbias need weight")
-    device = _device(g, v, m, q, w, dx, dw, db)
-    _check_call(_LIB.XGBBLayerNormBackward(device, g.ptr, g_stride, v.ptr, v.code, rows, dim, stride, m.ptr, q.ptr,
-                                           w and w.ptr, w.code if w is not None else _F32, dx.ptr, dx_stride,
-                                           dw and dw.ptr, db and db.ptr, _pointer(workspace) if size else None, size,
-                                           _handle(stream, device, v.tensor)))
+    device = _one_device(v[4], g[4], m_device, q_device, w_device, dx_device, dw_device, db_device)
+    _call(_LIB.XGBBLayerNormBackward, _pack_layer_norm_backward(
+        g[0], v[0], m, q, w, dx, dw, db, space, _handle(stream, device, v), size, rows, dim, g_stride, stride,
+        dx_stride, v[3], w_code, device))
     return out, dweight, dbias
 
 
