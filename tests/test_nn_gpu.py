@@ -210,13 +210,22 @@ def test_layer_norm_and_its_gradient(shape, types):
                            torch.full((rows, pad), 7.0, device=DEV))
 
 
-@pytest.mark.parametrize("rows,dim", [(5000, 64), (3001, 200), (1203, 1024), (2500, 3), (700, 2048), (601, 777)])
-def test_weight_gradient_over_many_rows(rows, dim):
+# Rows enough that blocks take many each, of 64 lanes' values or fewer, of whole and of partly filled blocks.
+@pytest.mark.parametrize("rows,dim,a,p", [
+    (5000, 64, F32, F32), (3001, 200, F32, F32), (1203, 1024, F32, F32), (2500, 3, F32, F32), (700, 2048, F32, F32),
+    (601, 777, F32, F32), (9001, 512, BF16, F32), (5003, 1000, F16, F16), (2501, 2048, BF16, BF16),
+    (2500, 1996, F32, F32), (2401, 4096, F32, F32), (2400, 3080, F16, F32), (2399, 4096, BF16, F32),
+    (2403, 8192, BF16, F32), (2402, 8000, F32, F32), (2370, 16384, BF16, BF16), (2369, 16000, F16, F32),
+    (300, 9001, F32, F32)])
+def test_many_rows(rows, dim, a, p):
     g = _gen(7, rows, dim)
-    x, grad, w = _matrix(g, rows, dim, F32), _matrix(g, rows, dim, F32), _matrix(g, 1, dim, F32)[0]
-    _, mean, rstd = nn.layer_norm(x, w)
+    x = (torch.randn(rows, dim, generator=g) * 2 + 30 * torch.randn(rows, 1, generator=g)).to(a).to(DEV)
+    grad, w, b = _matrix(g, rows, dim, a), _matrix(g, 1, dim, p)[0], _matrix(g, 1, dim, p)[0]
+    y, mean, rstd = nn.layer_norm(x, w, b)
+    for got, want, what in zip((y, mean, rstd), R.norm(x, w, b), ("y", "mean", "rstd")):
+        R.close(got, want, what)
     dx, dw, db = nn.layer_norm_backward(grad, x, mean, rstd, w)
-    wants = R.norm_grad(grad, x, mean, rstd, w)
+    wants = R.norm_grad(grad, x, mean, rstd, w, p)
     for got, want, what in zip((dx, dw, db), wants, ("dx", "dweight", "dbias")):
         R.close(got, want, what)
 

@@ -15,6 +15,14 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// 1 / sqrt(v): the device's approximation and one step of Newton's method.
+// 0, infinity and NaN pass through the approximation.
+__device__ __forceinline__ float inverse_sqrt(float v) {
+  const float r = rsqrtf(v);
+  const float e = fmaf(-v * r, r, 1.0f);  // NaN for v = 0 and infinity
+  return fabsf(e) < 1.0f ? fmaf(0.5f * r, e, r) : r;
+}
+
 // Sums N values a thread over the block, in every thread. `part` is not the
 // one that the call before used, so one barrier does: whoever still reads that
 // one has not passed this one.
@@ -84,7 +92,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024)
 #pragma unroll
       for (int e = 0; e < VE; ++e) square[0] = fmaf(v[i].f(e) - m, v[i].f(e) - m, square[0]);
   row_sum<WARP, 1>(square, G, part[1]);
-  const float q = 1.0f / sqrtf(square[0] / float(dim) + eps);
+  const float q = inverse_sqrt(square[0] / float(dim) + eps);
   if (!here) return;
   if (at == 0) {
     if (mean) mean[row] = m;
@@ -112,6 +120,162 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024)
   }
 }
 
+// Sums N values a lane over the warp, N a power of two: each shuffle halves how
+// many a lane holds, and lane j ends with the sum of value j / (32 / N).
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N], uint32_t lane) {
+  uint32_t k = 16;
+#pragma unroll
+  for (int n = N / 2; n >= 1; n >>= 1, k >>= 1) {
+    const bool upper = lane & k;
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      v[i] = (upper ? v[i + n] : v[i]) + __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + n], k);
+  }
+  float s = v[0];
+#pragma unroll
+  for (int j = 16 / N; j; j >>= 1) s += __shfl_xor_sync(0xffffffffu, s, j);
+  return s;
+}
+
+// Forward for many rows of 16-byte pieces, a block R rows at a time, whose sums
+// share their shuffles and their barrier. Blocks stay, CH pieces a thread, and
+// the next R rows are under way into shared memory, where each thread reads
+// back only what it copied itself; weight and bias come from the L1 cache once
+// for all R rows. A warp takes its own values' mean and squares about it, and
+// one barrier joins the warps: with n_w values, sum s_w and squares M_w of
+// warp w,
+//   mean = sum s_w / n,  variance n = sum M_w + n_w (s_w / n_w - mean)^2,
+// all of whose terms are positive. FULL: every thread holds CH pieces.
+template <class T, class P, int CH, int R, int MOST, bool FULL>
+__global__ void __launch_bounds__(MOST)
+    norm_ring_kernel(const T* __restrict__ x, int64_t x_stride, uint32_t rows, uint32_t dim,
+                     const P* __restrict__ w, const P* __restrict__ b, float eps, T* __restrict__ y,
+                     int64_t y_stride, float* __restrict__ mean, float* __restrict__ rstd) {
+  constexpr int VE = 16 / sizeof(T), H = VE / 2, L = 32 / R, W = MOST / 32 / L;
+  extern __shared__ uint4 ring[];  // [2][R][CH][threads]
+  __shared__ __align__(16) float2 part[2][R][MOST / 32];
+  const uint32_t G = blockDim.x, at = threadIdx.x, lane = at & 31, warp = at >> 5;
+  const float inverse = 1.0f / float(dim);
+  const auto has = [&](int i) { return FULL || (at + i * G) * VE < dim; };
+  const auto count = [&](uint32_t q) {  // values that warp q holds
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const uint32_t first = (q * 32 + i * G) * VE;
+      n += first < dim ? min(dim - first, 32u * VE) : 0u;
+    }
+    return q * 32 < G ? float(n) : 0.0f;
+  };
+  for (uint32_t i = at; i < 2 * R * (MOST / 32); i += G) (&part[0][0][0])[i] = both(0.0f);
+  __syncthreads();
+  const float warp_n = count(warp), warp_inverse = warp_n > 0.0f ? 1.0f / warp_n : 0.0f;
+  // After the barrier L lanes join the warps of a row, W warps each.
+  const uint32_t mine = lane / L, first = (lane & (L - 1)) * W;
+  const uint32_t row_bytes = CH * G * 16, stage_bytes = R * row_bytes;
+  char* const own = reinterpret_cast<char*>(ring + at);
+  const auto fetch = [&](uint32_t row, char* to) {
+    const T* from = x + int64_t(row) * x_stride + at * VE;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (row + r < rows)
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+          if (has(i)) copy_async16(to + r * row_bytes + i * G * 16, from + r * x_stride + i * G * VE);
+    copy_commit();
+  };
+  const uint32_t step = gridDim.x * R;
+  fetch(blockIdx.x * R, own);
+  fetch(blockIdx.x * R + step, own + stage_bytes);
+  uint32_t turn = 0;
+  for (uint32_t row = blockIdx.x * R; row < rows; row += step, turn ^= 1) {
+    char* const stage = own + turn * stage_bytes;
+    copy_wait<1>();
+    float2 v[R][CH][H];
+    float s[R], near[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float2 sum = both(0.0f);
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        if (has(i)) {
+          unpack16<T>(*reinterpret_cast<const uint4*>(stage + r * row_bytes + i * G * 16), v[r][i]);
+#pragma unroll
+          for (int e = 0; e < H; ++e) sum = add2(sum, v[r][i][e]);
+        }
+      s[r] = sum.x + sum.y;
+    }
+    fetch(row + 2 * step, stage);  // the thread has read its values out
+    const float sum = warp_sums<R>(s, lane);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      near[r] = __shfl_sync(0xffffffffu, sum, r * L) * warp_inverse;
+      float2 square = both(0.0f);
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        if (has(i))
+#pragma unroll
+          for (int e = 0; e < H; ++e) {
+            v[r][i][e] = add2(v[r][i][e], both(-near[r]));
+            square = fma2(v[r][i][e], v[r][i][e], square);
+          }
+      s[r] = square.x + square.y;
+    }
+    const float square = warp_sums<R>(s, lane);
+    if ((lane & (L - 1)) == 0) part[turn][mine][warp] = make_float2(sum, square);
+    __syncthreads();
+    float2 other[W];
+    float m = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      other[j] = part[turn][mine][first + j];
+      m += other[j].x;
+    }
+#pragma unroll
+    for (int k = L / 2; k; k >>= 1) m += __shfl_xor_sync(0xffffffffu, m, k);
+    m *= inverse;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float n = FULL ? warp_n : count(first + j);
+      const float off = n > 0.0f && (!FULL || (first + j) * 32 < G) ? __fdividef(other[j].x, n) - m : 0.0f;
+      q += fmaf(n * off, off, other[j].y);
+    }
+#pragma unroll
+    for (int k = L / 2; k; k >>= 1) q += __shfl_xor_sync(0xffffffffu, q, k);
+    q = inverse_sqrt(q * inverse + eps);
+    if (warp == 0 && (lane & (L - 1)) == 0 && row + mine < rows) {
+      if (mean) mean[row + mine] = m;
+      if (rstd) rstd[row + mine] = q;
+    }
+    // (x - mean) q, from the value about the warp's mean.
+    float2 scale[R], rest[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float qr = __shfl_sync(0xffffffffu, q, r * L), mr = __shfl_sync(0xffffffffu, m, r * L);
+      scale[r] = both(qr);
+      rest[r] = both((near[r] - mr) * qr);
+    }
+    T* to = y + int64_t(row) * y_stride + at * VE;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (has(i)) {
+        float2 wv[H], bv[H];
+        if (w) load_pairs<P, H>(w + (at + i * G) * VE, wv);
+        if (b) load_pairs<P, H>(b + (at + i * G) * VE, bv);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+          for (int e = 0; e < H; ++e) {
+            v[r][i][e] = fma2(v[r][i][e], scale[r], rest[r]);
+            if (w) v[r][i][e] = b ? fma2(v[r][i][e], wv[e], bv[e]) : mul2(v[r][i][e], wv[e]);
+            else if (b) v[r][i][e] = add2(v[r][i][e], bv[e]);
+          }
+          if (row + r < rows) *reinterpret_cast<uint4*>(to + r * y_stride + i * G * VE) = pack16<T>(v[r][i]);
+        }
+      }
+  }
+}
+
 // Forward for rows that registers do not hold: three passes, a block a row.
 template <class T, class P, int VE>
 __global__ void __launch_bounds__(1024)
@@ -136,7 +300,7 @@ __global__ void __launch_bounds__(1024)
     for (int e = 0; e < VE; ++e) square[0] = fmaf(v.f(e) - m, v.f(e) - m, square[0]);
   }
   block_sum<1>(square, part[1]);
-  const float q = 1.0f / sqrtf(square[0] / float(dim) + eps);
+  const float q = inverse_sqrt(square[0] / float(dim) + eps);
   if (threadIdx.x == 0) {
     if (mean) mean[row] = m;
     if (rstd) rstd[row] = q;
@@ -276,6 +440,252 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024, WARP ? 4 : 1)
   }
 }
 
+// The same for many rows of 16-byte pieces, a block a row at a time, with the
+// next S - 1 rows under way into shared memory.
+template <class T, class P, int S, bool FULL>
+__global__ void __launch_bounds__(1024)
+    norm_grad_ring_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x,
+                          int64_t x_stride, const float* __restrict__ mean, const float* __restrict__ rstd,
+                          uint64_t rows, uint32_t dim, const P* __restrict__ w, T* __restrict__ dx,
+                          int64_t dx_stride, float* __restrict__ parts) {
+  constexpr int VE = 16 / sizeof(T), CH = 8 / VE, H = VE / 2;
+  extern __shared__ uint4 ring[];  // [S][2][CH][threads]
+  __shared__ float part[2][2][32];
+  const uint32_t G = blockDim.x, at = threadIdx.x, lane = at & 31, warp = at >> 5, warps = G >> 5;
+  const float inverse = 1.0f / float(dim);
+  float2 wv[CH][H], dw[CH][H] = {}, db[CH][H] = {};
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const uint32_t c = (at + i * G) * VE;
+#pragma unroll
+    for (int e = 0; e < H; ++e)
+      wv[i][e] = w && c < dim ? make_float2(to_f32(w[c + 2 * e]), to_f32(w[c + 2 * e + 1])) : both(1.0f);
+  }
+  const auto has = [&](int i) { return FULL || (at + i * G) * VE < dim; };
+  const uint32_t half = CH * G * 16, stage_bytes = 2 * half;
+  char* const own = reinterpret_cast<char*>(ring + at);
+  const auto fetch = [&](const T* xs, const T* gs, bool there, char* to) {
+    if (there)
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        if (has(i)) {
+          copy_async16(to + i * G * 16, xs + i * G * VE);
+          copy_async16(to + half + i * G * 16, gs + i * G * VE);
+        }
+    copy_commit();
+  };
+  const uint32_t step = gridDim.x;
+  const int64_t x_step = int64_t(step) * x_stride, g_step = int64_t(step) * grad_stride;
+  const int64_t dx_step = int64_t(step) * dx_stride;
+  const T* xr = x + int64_t(blockIdx.x) * x_stride + at * VE;
+  const T* gr = grad + int64_t(blockIdx.x) * grad_stride + at * VE;
+  T* dxr = dx + int64_t(blockIdx.x) * dx_stride + at * VE;
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i, xr += x_step, gr += g_step)
+    fetch(xr, gr, blockIdx.x + i * step < rows, own + i * stage_bytes);
+  char* read = own;
+  char* written = own + (S - 1) * stage_bytes;
+  float nm = blockIdx.x < rows ? mean[blockIdx.x] : 0.0f, nq = blockIdx.x < rows ? rstd[blockIdx.x] : 0.0f;
+  uint32_t turn = 0;
+  for (uint32_t row = blockIdx.x; row < rows; row += step, turn ^= 1, xr += x_step, gr += g_step, dxr += dx_step) {
+    fetch(xr, gr, row + (S - 1) * step < rows, written);
+    const float m = nm, q = nq;
+    if (row + step < rows) {
+      nm = mean[row + step];
+      nq = rstd[row + step];
+    }
+    copy_wait<S - 1>();
+    float2 h[CH][H], g[CH][H], sum_g = both(0.0f), sum_gh = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (has(i)) {
+        float2 d[H];
+        unpack16<T>(*reinterpret_cast<const uint4*>(read + i * G * 16), h[i]);
+        unpack16<T>(*reinterpret_cast<const uint4*>(read + half + i * G * 16), d);
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+          h[i][e] = mul2(add2(h[i][e], both(-m)), both(q));
+          g[i][e] = mul2(d[e], wv[i][e]);
+          sum_g = add2(sum_g, g[i][e]);
+          sum_gh = fma2(g[i][e], h[i][e], sum_gh);
+          dw[i][e] = fma2(d[e], h[i][e], dw[i][e]);
+          db[i][e] = add2(db[i][e], d[e]);
+        }
+      }
+    written = read;
+    read = read == own + (S - 1) * stage_bytes ? own : read + stage_bytes;
+    // Two sums for the shuffles of one: lanes 0 to 15 end with the first,
+    // lanes 16 to 31 with the second.
+    const float s0 = sum_g.x + sum_g.y, s1 = sum_gh.x + sum_gh.y;
+    float s = lane < 16 ? s0 : s1;
+    s += __shfl_xor_sync(0xffffffffu, lane < 16 ? s1 : s0, 16);
+#pragma unroll
+    for (int k = 8; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+    if ((lane & 15) == 0) part[turn][lane >> 4][warp] = s;
+    __syncthreads();
+    const uint32_t q0 = lane & 15;
+    s = q0 < warps ? part[turn][lane >> 4][q0] : 0.0f;
+    if (q0 + 16 < warps) s += part[turn][lane >> 4][q0 + 16];
+#pragma unroll
+    for (int k = 8; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+    s *= -inverse * q;
+    // q (g - a - h b), with -q a and -q b.
+    const float2 a = both(__shfl_sync(0xffffffffu, s, 0)), b = both(__shfl_sync(0xffffffffu, s, 16));
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (has(i)) {
+#pragma unroll
+        for (int e = 0; e < H; ++e) h[i][e] = fma2(h[i][e], b, fma2(g[i][e], both(q), a));
+        *reinterpret_cast<uint4*>(dxr + i * G * VE) = pack16<T>(h[i]);
+      }
+  }
+  if (!parts) return;
+  float* out = parts + uint64_t(blockIdx.x) * 2 * dim;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const uint32_t c = (at + i * G) * VE;
+    if (c < dim)
+#pragma unroll
+      for (int e = 0; e < H; ++e) {
+        out[c + 2 * e] = dw[i][e].x;
+        out[c + 2 * e + 1] = dw[i][e].y;
+        out[dim + c + 2 * e] = db[i][e].x;
+        out[dim + c + 2 * e + 1] = db[i][e].y;
+      }
+  }
+}
+
+// The same for many rows of 16-byte pieces, a block of 512 threads at most R
+// rows at a time: the rows' 2 R sums are reduced together, each shuffle halving
+// how many of them a lane holds, and share their barrier. The next R rows are
+// under way into shared memory.
+template <class T, class P, int R, bool FULL>
+__global__ void __launch_bounds__(512, 1)
+    norm_grad_rows_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x,
+                          int64_t x_stride, const float* __restrict__ mean, const float* __restrict__ rstd,
+                          uint32_t rows, uint32_t dim, const P* __restrict__ w, T* __restrict__ dx,
+                          int64_t dx_stride, float* __restrict__ parts) {
+  constexpr int VE = 16 / sizeof(T), CH = 8 / VE, H = VE / 2, V = 2 * R, L = 32 / V, W = 16 / L;
+  extern __shared__ uint4 ring[];  // [2][R][2][CH][threads]
+  __shared__ __align__(16) float part[2][V][16];
+  const uint32_t G = blockDim.x, at = threadIdx.x, lane = at & 31, warp = at >> 5;
+  const float inverse = 1.0f / float(dim);
+  const auto has = [&](int i) { return FULL || (at + i * G) * VE < dim; };
+  for (uint32_t i = at; i < 2 * V * 16; i += G) (&part[0][0][0])[i] = 0.0f;
+  __syncthreads();
+  float2 wv[CH][H], dw[CH][H] = {}, db[CH][H] = {};
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const uint32_t c = (at + i * G) * VE;
+#pragma unroll
+    for (int e = 0; e < H; ++e)
+      wv[i][e] = w && c < dim ? make_float2(to_f32(w[c + 2 * e]), to_f32(w[c + 2 * e + 1])) : both(1.0f);
+  }
+  const uint32_t half = CH * G * 16, row_bytes = 2 * half, stage_bytes = R * row_bytes;
+  char* const own = reinterpret_cast<char*>(ring + at);
+  const auto fetch = [&](uint32_t row, char* to) {
+    const T* xs = x + int64_t(row) * x_stride + at * VE;
+    const T* gs = grad + int64_t(row) * grad_stride + at * VE;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (row + r < rows)
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+          if (has(i)) {
+            copy_async16(to + r * row_bytes + i * G * 16, xs + r * x_stride + i * G * VE);
+            copy_async16(to + r * row_bytes + half + i * G * 16, gs + r * grad_stride + i * G * VE);
+          }
+    copy_commit();
+  };
+  const uint32_t step = gridDim.x * R;
+  float nm[R], nq[R];
+  const auto fetch_stats = [&](uint32_t row) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (row + r < rows) {
+        nm[r] = mean[row + r];
+        nq[r] = rstd[row + r];
+      }
+  };
+  fetch(blockIdx.x * R, own);
+  fetch(blockIdx.x * R + step, own + stage_bytes);
+  fetch_stats(blockIdx.x * R);
+  uint32_t turn = 0;
+  for (uint32_t row = blockIdx.x * R; row < rows; row += step, turn ^= 1) {
+    char* const stage = own + turn * stage_bytes;
+    float q[R], val[V];
+    float2 h[R][CH][H], g[R][CH][H];
+    copy_wait<1>();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      val[2 * r] = val[2 * r + 1] = 0.0f;
+      q[r] = nq[r];
+      if (row + r >= rows) continue;
+      const float m = nm[r];
+      float2 sum_g = both(0.0f), sum_gh = both(0.0f);
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        if (has(i)) {
+          float2 d[H];
+          unpack16<T>(*reinterpret_cast<const uint4*>(stage + r * row_bytes + i * G * 16), h[r][i]);
+          unpack16<T>(*reinterpret_cast<const uint4*>(stage + r * row_bytes + half + i * G * 16), d);
+#pragma unroll
+          for (int e = 0; e < H; ++e) {
+            h[r][i][e] = mul2(add2(h[r][i][e], both(-m)), both(q[r]));
+            g[r][i][e] = mul2(d[e], wv[i][e]);
+            sum_g = add2(sum_g, g[r][i][e]);
+            sum_gh = fma2(g[r][i][e], h[r][i][e], sum_gh);
+            dw[i][e] = fma2(d[e], h[r][i][e], dw[i][e]);
+            db[i][e] = add2(db[i][e], d[e]);
+          }
+        }
+      val[2 * r] = sum_g.x + sum_g.y;
+      val[2 * r + 1] = sum_gh.x + sum_gh.y;
+    }
+    fetch(row + 2 * step, stage);  // the thread has read its values out
+    fetch_stats(row + step);
+    float s = warp_sums<V>(val, lane);  // of value lane / L
+    if ((lane & (L - 1)) == 0) part[turn][lane / L][warp] = s;
+    __syncthreads();
+    const auto others = load<float, W>(&part[turn][lane / L][(lane & (L - 1)) * W]);
+    s = others.v[0];
+#pragma unroll
+    for (int j = 1; j < W; ++j) s += others.v[j];
+#pragma unroll
+    for (int j = L / 2; j; j >>= 1) s += __shfl_xor_sync(0xffffffffu, s, j);
+    s *= -inverse;
+    T* to = dx + int64_t(row) * dx_stride + at * VE;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      // q (g - a - h b), with -q a and -q b.
+      const float2 a = both(__shfl_sync(0xffffffffu, s, 2 * r * L) * q[r]);
+      const float2 b = both(__shfl_sync(0xffffffffu, s, (2 * r + 1) * L) * q[r]);
+      if (row + r >= rows) continue;
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        if (has(i)) {
+#pragma unroll
+          for (int e = 0; e < H; ++e) h[r][i][e] = fma2(h[r][i][e], b, fma2(g[r][i][e], both(q[r]), a));
+          *reinterpret_cast<uint4*>(to + r * dx_stride + i * G * VE) = pack16<T>(h[r][i]);
+        }
+    }
+  }
+  if (!parts) return;
+  float* out = parts + uint64_t(blockIdx.x) * 2 * dim;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const uint32_t c = (at + i * G) * VE;
+    if (c < dim)
+#pragma unroll
+      for (int e = 0; e < H; ++e) {
+        out[c + 2 * e] = dw[i][e].x;
+        out[c + 2 * e + 1] = dw[i][e].y;
+        out[dim + c + 2 * e] = db[i][e].x;
+        out[dim + c + 2 * e + 1] = db[i][e].y;
+      }
+  }
+}
+
 // dx for rows that registers do not hold: two passes, a block a row.
 template <class T, class P, int VE>
 __global__ void __launch_bounds__(1024)
@@ -382,7 +792,7 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 bool param_aligned(const void* p, size_t size, uint64_t n) {
-  return reinterpret_cast<uintptr_t>(p) % std::min<size_t>(16, n * size) == 0;
+  return reinterpret_cast<uintptr_t>(p) % std::min<size_t>(32, n * size) == 0;
 }
 
 // Calls f with the widest VE that every matrix and vector allows.
@@ -399,6 +809,15 @@ void with_norm_width(std::initializer_list<Mat> mats, std::initializer_list<cons
   if (fits(kWide)) f(std::integral_constant<int, kWide>());
   else if (kWide > 4 && fits(2)) f(std::integral_constant<int, kWide == 4 ? 1 : 2>());
   else f(std::integral_constant<int, 1>());
+}
+
+// Launches a kernel with more shared memory than a launch has unasked.
+template <class... Params, class... Args>
+void launch_ring(void (*kernel)(Params...), unsigned blocks, unsigned threads, size_t shared, cudaStream_t stream,
+                 Args... args) {
+  if (shared > 46 * 1024)
+    XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)));
+  kernel<<<blocks, threads, shared, stream>>>(args...);
 }
 
 // How norm_grad_kernel takes rows of `dim` values: lanes or threads a row,
@@ -428,14 +847,14 @@ struct GradPlan {
 void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, const void* bias, int param_type,
                 float eps, const Mat& y, float* mean, float* rstd, cudaStream_t stream) {
   if (!rows) return;
-  with_types(x.type, param_type, [&](auto* pt, auto* pp) {
+  with_param_types(x.type, param_type, [&](auto* pt, auto* pp) {
     using T = std::remove_pointer_t<decltype(pt)>;
     using P = std::remove_pointer_t<decltype(pp)>;
     const T* in = static_cast<const T*>(x.data);
     T* out = static_cast<T*>(const_cast<void*>(y.data));
     const P *w = static_cast<const P*>(weight), *b = static_cast<const P*>(bias);
     with_norm_width<T>({x, y}, {weight, bias}, param_type, rows, dim, [&](auto width) {
-      constexpr int VE = decltype(width)::value;
+      constexpr int VE = decltype(width)::value, kWide = 16 / sizeof(T);
       constexpr int kMost = std::min(32 / VE, 16);  // pieces of a thread
       const uint64_t pieces = (dim + VE - 1) / VE;
       const auto go = [&](auto count, auto in_warp, unsigned blocks, unsigned threads, int lg) {
@@ -462,6 +881,21 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
                                                                       eps, out, y.stride, mean, rstd);
         return;
       }
+      if constexpr (VE == kWide) {
+        constexpr int CH = 2;
+        const unsigned threads = blocks_for(pieces, CH * 32) * 32;
+        const bool full = pieces == CH * threads;
+        const auto ring = [&](auto most, auto at_once) {
+          constexpr int MOST = decltype(most)::value, R = decltype(at_once)::value;
+          launch_ring(full ? norm_ring_kernel<T, P, CH, R, MOST, true> : norm_ring_kernel<T, P, CH, R, MOST, false>,
+                      148 * (MOST / threads), threads, size_t(2) * R * CH * threads * 16, stream, in, x.stride,
+                      uint32_t(rows), uint32_t(dim), w, b, eps, out, y.stride, mean, rstd);
+        };
+        if (rows >= 148 * 16 && param_aligned(weight, 32, 1) && param_aligned(bias, 32, 1)) {
+          if (threads <= 512) return ring(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
+          if (threads <= 1024) return ring(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+        }
+      }
       // Many rows: as few threads a row as hold it. Few: as many as it has pieces.
       const uint64_t each = rows >= 148 ? std::min<uint64_t>(kMost, 4) : 1;
       const uint64_t threads = std::min<uint64_t>(1024, ((pieces + each - 1) / each + 31) / 32 * 32);
@@ -481,7 +915,8 @@ void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const
   const bool params = dweight || dbias;
   const GradPlan plan(rows, dim);
   float* parts = params ? static_cast<float*>(workspace) : nullptr;
-  with_types(x.type, param_type, [&](auto* pt, auto* pp) {
+  uint32_t used = plan.blocks;  // parts that are written
+  with_param_types(x.type, param_type, [&](auto* pt, auto* pp) {
     using T = std::remove_pointer_t<decltype(pt)>;
     using P = std::remove_pointer_t<decltype(pp)>;
     const T* g = static_cast<const T*>(grad.data);
@@ -495,6 +930,23 @@ void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const
           norm_grad_kernel<T, P, VE, 8 / VE, true>
               <<<plan.blocks, plan.threads, (kThreads / 32) * 2 * (8u << plan.lg) * 4, stream>>>(
                   g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts, plan.lg);
+        } else if (plan.fits && VE * sizeof(T) == 16 && rows >= plan.blocks * 4ull) {
+          if constexpr (VE * sizeof(T) == 16) {
+            const bool full = dim == plan.threads * 8ull;
+            if (plan.threads <= 512) {
+              constexpr int R = sizeof(T) == 2 ? 4 : 2;
+              launch_ring(full ? norm_grad_rows_kernel<T, P, R, true> : norm_grad_rows_kernel<T, P, R, false>,
+                          148 * (512 / plan.threads), plan.threads, size_t(2) * R * 2 * 8 * sizeof(T) * plan.threads,
+                          stream, g, grad.stride, v, x.stride, mean, rstd, uint32_t(rows), uint32_t(dim), w, out,
+                          dx.stride, parts);
+              used = 148 * (512 / plan.threads);
+            } else {
+              constexpr int S = sizeof(T) == 2 ? 4 : 3;
+              launch_ring(full ? norm_grad_ring_kernel<T, P, S, true> : norm_grad_ring_kernel<T, P, S, false>,
+                          plan.blocks, plan.threads, size_t(S) * 2 * 8 * sizeof(T) * plan.threads, stream, g,
+                          grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts);
+            }
+          }
         } else if (plan.fits) {
           norm_grad_kernel<T, P, VE, 8 / VE, false><<<plan.blocks, plan.threads, 0, stream>>>(
               g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts, 0);
@@ -508,7 +960,7 @@ void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const
       });
     if (params)
       norm_parts_kernel<P><<<blocks_for(2 * dim, 32), kThreads, 0, stream>>>(
-          parts, plan.blocks, uint32_t(dim), static_cast<P*>(dweight), static_cast<P*>(dbias));
+          parts, used, uint32_t(dim), static_cast<P*>(dweight), static_cast<P*>(dbias));
   });
   XGBB_CUDA(cudaGetLastError());
 }

@@ -43,6 +43,98 @@ __device__ __forceinline__ void store(T* p, const float (&f)[N]) {
   *reinterpret_cast<Pack<T, N>*>(p) = o;
 }
 
+// Two float32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// 16 bytes of T as float pairs and back.
+template <class T>
+__device__ __forceinline__ void unpack16(const uint4& p, float2 (&f)[8 / sizeof(T)]) {
+  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+  if constexpr (sizeof(T) == 4) {
+    f[0] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    f[1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __half>)
+        f[i] = __half22float2(reinterpret_cast<const __half2&>(w[i]));
+      else
+        f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ uint4 pack16(const float2 (&f)[8 / sizeof(T)]) {
+  uint4 p;
+  uint32_t w[4];
+  if constexpr (sizeof(T) == 4) {
+    p = make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x),
+                   __float_as_uint(f[1].y));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __float22half2_rn(f[i]);
+        w[i] = reinterpret_cast<const uint32_t&>(h);
+      } else {
+        const __nv_bfloat162 h = __float22bfloat162_rn(f[i]);
+        w[i] = reinterpret_cast<const uint32_t&>(h);
+      }
+    }
+    p = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return p;
+}
+
+// 2 H values of P as float pairs, from an address that is a multiple of their
+// size (32 bytes for eight floats).
+template <class P, int H>
+__device__ __forceinline__ void load_pairs(const P* p, float2 (&f)[H]) {
+  if constexpr (sizeof(P) * H == 16) {
+    asm("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=f"(f[0].x), "=f"(f[0].y), "=f"(f[1].x), "=f"(f[1].y), "=f"(f[2].x), "=f"(f[2].y), "=f"(f[3].x),
+          "=f"(f[3].y)
+        : "l"(p));
+  } else {
+    unpack16<P>(*reinterpret_cast<const uint4*>(p), f);
+  }
+}
+
+// Copies 16 bytes into shared memory behind the thread's back; a thread that
+// waits for its own copies needs no barrier to read them.
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most N of the thread's last groups are under way.
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Division of 32-bit numbers by an invariant divisor: with s = ceil(log2 d)
 // and m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(n, m) + n) >> s, the
 // sum in 33 bits (Granlund and Montgomery, "Division by invariant integers
@@ -88,6 +180,15 @@ void with_types(int a, int b, F&& f) {
     if (a == b) f(pa, pa);
     else if constexpr (std::is_same_v<decltype(pa), float*>) with_type(b, [&](auto* pb) { f(pa, pb); });
     else f(pa, static_cast<float*>(nullptr));
+  });
+}
+
+// The same where b is a's type or float.
+template <class F>
+void with_param_types(int a, int b, F&& f) {
+  with_type(a, [&](auto* pa) {
+    if (a == b) f(pa, pa);
+    else if constexpr (!std::is_same_v<decltype(pa), float*>) f(pa, static_cast<float*>(nullptr));
   });
 }
 
