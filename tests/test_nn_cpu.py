@@ -91,8 +91,9 @@ REFUSED = [
     (lambda: nn.embedding_backward(F((3, 2)), K(3), 4, out=F((5, 2))), "out must have the shape"),
     (lambda: nn.embedding_backward(F((4, 2)), K(3), 4, out=F((4, 2))), "shape of the lookup"),
     (lambda: nn.embedding_backward(F((3, 2)), K(3), 4, accumulate=True), "accumulate needs out"),
-    (lambda: nn.embedding_backward(F((3, 2)), K(3), 4, out=F((4, 2), ptr=8192)), "workspace must be given"),
-    (lambda: nn.embedding_backward(F((3, 2)), K(3), 4, out=F((4, 2), ptr=8192), workspace=F((8,))), "workspace must be"),
+    (lambda: nn.embedding_backward(F((1 << 17, 2)), K(1 << 17), 4, out=F((4, 2), ptr=8192)), "workspace must be given"),
+    (lambda: nn.embedding_backward(F((1 << 17, 2)), K(1 << 17), 4, out=F((4, 2), ptr=8192), workspace=F((8,))),
+     "workspace must be"),
     (lambda: nn.embedding_backward(F((3, 2)), K(3), 1 << 31, out=F((1 << 31, 2))), "vocab"),
     (lambda: nn.embedding_backward(F((1 << 16, 2)), K(1 << 16, 1 << 16), 4, bag=True, out=F((4, 2))), "tokens"),
     (lambda: nn.embedding_scale_backward(F((3, 2)), K(3), F((4, 3)), out=F((3,))), "shape of the lookup"),
@@ -121,13 +122,14 @@ def test_wrong_arguments_are_refused(at):
 
 def test_library_refuses_before_it_touches_a_device():
     # Types that do not pair up, an index type that is none, a workspace that is missing, not aligned or too small.
-    need = nn.embedding_backward_workspace(3, 1, 4, 2)
+    rows = 1 << 17
+    need = nn.embedding_backward_workspace(rows, 1, 4, 2)
 
     def backward(**kw):
         a = dict(grad_type=1, token_type=7, out_type=1, workspace=4096, size=need)
         a.update(kw)
         ret = _LIB.XGBBEmbeddingBackward(nn._pack_embedding_backward(
-            8192, 0, 3, 1, 1, 0, 0, 0, a["token_type"], 1.0, 4096, 16384, a["workspace"], 0, a["size"], 4, 2, 2, 2,
+            8192, 0, rows, 1, 1, 0, 0, 0, a["token_type"], 1.0, 4096, 16384, a["workspace"], 0, a["size"], 4, 2, 2, 2,
             a["grad_type"], a["out_type"], 0, -1))
         return ret, _LIB.XGBGetLastError().decode()
 
@@ -167,4 +169,4 @@ def test_workspace_sizes_are_refused_like_the_calls():
         nn.layer_norm_backward_workspace(3, 0)
     assert _LIB.XGBBLayerNormBackwardWorkspace(3, 4, None) == -1
     size = ctypes.c_size_t()
-    assert _LIB.XGBBEmbeddingBackwardWorkspace(3, 2, 5, 4, ctypes.byref(size)) == 0 and size.value > 0
+    assert _LIB.XGBBEmbeddingBackwardWorkspace(1 << 17, 2, 5, 4, ctypes.byref(size)) == 0 and size.value > 0

@@ -334,6 +334,207 @@ __global__ void __launch_bounds__(kThreads)
   store<O, VE>(to, acc);
 }
 
+// Few tokens, in one launch: block (x, y) owns the table's rows [x span, x span
+// + span) in a tile of columns. It picks its rows' tokens out of all n, sorts
+// them, (row << kShift | position), in shared memory, zeroes the rows that have
+// none, and sums the others: groups of 2^lg lanes take equal shares of the
+// sorted list, and what crosses shares is joined through shared memory, in the
+// shares' order. No row is written by two blocks. step: the distance of one
+// token from the next where it is the same for all, else 0.
+constexpr int kFewThreads = 512;
+constexpr int kShift = 15;
+constexpr uint32_t kFewTokens = 1u << kShift;
+
+template <class T, class O, int VE, bool SCALED>
+__global__ void __launch_bounds__(kFewThreads, 2)
+    few_kernel(const T* __restrict__ grad, int64_t grad_stride, Tokens k, int64_t step, FastDiv per_row, uint32_t n,
+               uint32_t vocab, uint32_t span, Scales s, float scale, uint32_t dim, O* __restrict__ out,
+               int64_t out_stride, bool accumulate, int lg) {
+  constexpr int U = 4, kBatch = 8;
+  extern __shared__ __align__(16) uint32_t space[];
+  __shared__ uint32_t total;
+  __shared__ int32_t first_row[kFewThreads], last_row[kFewThreads];  // of a group's share; -1: none
+  float* head = reinterpret_cast<float*>(space);  // [2][threads][VE]: sums that came in, sums that go on
+  float* tail = head + kFewThreads * VE;
+  uint32_t* present = space + 2 * kFewThreads * VE;  // a bit a row
+  uint32_t* list = present + (span + 31) / 32;
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t row0 = blockIdx.x * span, rows_here = min(span, vocab - row0);
+
+  // The rows' tokens, in any order: all entries differ, so the sort gives one.
+  for (uint32_t i = threadIdx.x; i < (span + 31) / 32; i += kFewThreads) present[i] = 0;
+  if (threadIdx.x == 0) total = 0;
+  __syncthreads();
+  const auto where = [&](uint32_t i) {
+    if (step) return int64_t(i) * step;
+    const uint32_t r = per_row.div(i);
+    return int64_t(r) * k.stride_row + int64_t(i - r * per_row.d) * k.stride_col;
+  };
+  for (uint32_t i0 = threadIdx.x - lane; i0 < n; i0 += kFewThreads * kBatch) {
+    uint64_t local[kBatch];  // past rows_here: another block's token, or nobody's
+    if (k.type == kI64) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const uint32_t at = i0 + i * kFewThreads + lane;
+        local[i] = at < n ? uint64_t(static_cast<const int64_t*>(k.data)[where(at)]) : ~0ull;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const uint32_t at = i0 + i * kFewThreads + lane;
+        local[i] = at < n ? uint64_t(int64_t(static_cast<const int32_t*>(k.data)[where(at)])) : ~0ull;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const bool mine = local[i] - row0 < rows_here;
+      const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+      if (!votes) continue;
+      uint32_t base = 0;
+      if (lane == 0) base = atomicAdd(&total, uint32_t(__popc(votes)));
+      base = __shfl_sync(0xffffffffu, base, 0);
+      if (mine) {
+        const uint32_t r = uint32_t(local[i] - row0);
+        list[base + __popc(votes & ((1u << lane) - 1))] = r << kShift | (i0 + i * kFewThreads + lane);
+        atomicOr(&present[r >> 5], 1u << (r & 31));
+      }
+    }
+  }
+  __syncthreads();
+
+  const uint32_t G = 1u << lg, me = threadIdx.x & (G - 1), group = threadIdx.x >> lg, groups = kFewThreads >> lg;
+  const uint32_t col = (blockIdx.y * G + me) * VE;
+  O* const mine_out = out + int64_t(row0) * out_stride + col;
+  const auto zero_absent = [&] {
+    const float zero[VE] = {};
+    if (!accumulate && col < dim)
+      for (uint32_t r = group; r < rows_here; r += groups)
+        if (!(present[r >> 5] >> (r & 31) & 1)) store<O, VE>(mine_out + int64_t(r) * out_stride, zero);
+  };
+  // Half of the blocks zero first and half last, so that reading and writing
+  // overlap on an SM that holds two.
+  const bool zero_first = (blockIdx.y * gridDim.x + blockIdx.x) * 2 < gridDim.x * gridDim.y;
+  if (zero_first) zero_absent();
+
+  // By counting the smaller entries where they are few, else a bitonic network
+  // whose comparators all point upwards (then what lies past the end need not
+  // exist). A warp's comparators of a span of 64 or less touch its own 64
+  // entries alone.
+  const uint32_t count = total;
+  if (count <= kFewThreads) {
+    uint32_t mine = 0, rank = 0;
+    if (threadIdx.x < count) {
+      mine = list[threadIdx.x];
+#pragma unroll 8
+      for (uint32_t j = 0; j < count; ++j) rank += list[j] < mine;
+    }
+    __syncthreads();
+    if (threadIdx.x < count) list[rank] = mine;
+    __syncthreads();
+  } else {
+    int bits = 32 - __clz(count - 1);
+    const uint32_t pairs = 1u << (bits - 1);
+    const auto order = [&](uint32_t i, uint32_t j) {
+      if (j < count) {
+        const uint32_t a = list[i], b = list[j];
+        if (a > b) {
+          list[i] = b;
+          list[j] = a;
+        }
+      }
+    };
+    for (int block = 1; block <= bits; ++block) {  // runs of 2^block entries
+      for (uint32_t p = threadIdx.x; p < pairs; p += kFewThreads) {
+        const uint32_t i = p >> (block - 1) << block | (p & ((1u << (block - 1)) - 1));
+        order(i, i ^ ((1u << block) - 1));
+      }
+      for (int half = block - 2; half >= 0; --half) {
+        if (half >= 5) __syncthreads();
+        else __syncwarp();
+        for (uint32_t p = threadIdx.x; p < pairs; p += kFewThreads) {
+          const uint32_t i = p >> half << (half + 1) | (p & ((1u << half) - 1));
+          order(i, i + (1u << half));
+        }
+      }
+      if (block >= 6) __syncthreads();
+      else __syncwarp();
+    }
+    __syncthreads();
+  }
+
+  const auto write = [&](int32_t local, const float(&sum)[VE]) {
+    if (col >= dim) return;
+    O* to = mine_out + int64_t(local) * out_stride;
+    float y[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) y[e] = sum[e] * scale;
+    if (accumulate) {
+      const auto old = load<O, VE>(to);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) y[e] += old.f(e);
+    }
+    store<O, VE>(to, y);
+  };
+
+  const uint32_t share = (count + groups - 1) / groups;
+  const uint32_t begin = min(count, group * share), end = min(count, begin + share);
+  const int32_t before = begin && begin < end ? int32_t(list[begin - 1] >> kShift) : -1;
+  const int32_t after = begin < end && end < count ? int32_t(list[end] >> kShift) : -1;
+  float acc[VE] = {};
+  int32_t current = -1;
+  bool from_before = false;
+  for (uint32_t j = begin; j < end; j += U) {
+    Pack<T, VE> v[U];
+    float f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t at = list[min(j + u, end - 1)] & (kFewTokens - 1), r = per_row.div(at);
+      if (SCALED) f[u] = s.data[int64_t(r) * s.stride_row + int64_t(at - r * per_row.d) * s.stride_col];
+      if (col < dim) v[u] = load<T, VE>(grad + int64_t(r) * grad_stride + col);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (j + u < end) {
+        const int32_t local = int32_t(list[j + u] >> kShift);
+        if (local != current) {
+          if (current >= 0) {
+            if (from_before) store<float, VE>(head + threadIdx.x * VE, acc);
+            else write(current, acc);
+          }
+#pragma unroll
+          for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
+          current = local;
+          from_before = j + u == begin && local == before;
+        }
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] = SCALED ? fmaf(f[u], v[u].f(e), acc[e]) : acc[e] + v[u].f(e);
+      }
+    }
+  }
+  const bool goes_on = current >= 0 && current == after;
+  if (current >= 0) {
+    if (from_before) store<float, VE>(head + threadIdx.x * VE, acc);
+    else if (goes_on) store<float, VE>(tail + threadIdx.x * VE, acc);
+    else write(current, acc);
+  }
+  if (me == 0) {
+    first_row[group] = begin < end ? int32_t(list[begin] >> kShift) : -1;
+    last_row[group] = goes_on ? current : -1;
+  }
+  __syncthreads();
+  // The group in whose share a row began joins it.
+  if (goes_on && !from_before) {
+    for (uint32_t g = group + 1; g < groups && first_row[g] == current; ++g) {
+      const auto more = load<float, VE>(head + ((g << lg) + me) * VE);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[e] += more.v[e];
+      if (last_row[g] != current) break;
+    }
+    write(current, acc);
+  }
+  if (!zero_first) zero_absent();
+}
+
 // Zeros into rows of `dim` values.
 template <class O, int VE>
 __global__ void __launch_bounds__(kThreads)
@@ -348,14 +549,56 @@ __global__ void __launch_bounds__(kThreads)
 
 }  // namespace
 
+// The distance from each token to the next, or 0 where it varies.
+int64_t token_step(const Tokens& k) {
+  if (k.per_row == 1) return k.stride_row;
+  return k.rows == 1 || k.stride_row == int64_t(k.per_row) * k.stride_col ? k.stride_col : 0;
+}
+
+// Shared memory of few_kernel, and its grid: rows of a block, blocks, column tiles.
+struct FewPlan {
+  int lg = 0;
+  uint32_t tiles, span, blocks;
+  size_t shared;
+  FewPlan(uint32_t n, uint64_t vocab, uint64_t pieces, int ve) {
+    while (lg < 5 && (1ull << lg) < pieces) ++lg;
+    tiles = blocks_for(pieces, 1u << lg);
+    // About two blocks an SM: each reads all tokens.
+    const uint64_t ranges = std::max<uint64_t>(1, 296 / tiles);
+    span = uint32_t(std::min<uint64_t>(std::max<uint64_t>((vocab + ranges - 1) / ranges, 1), 1u << (32 - kShift)));
+    blocks = blocks_for(vocab, span);
+    shared = size_t(2) * kFewThreads * ve * 4 + (span + 31) / 32 * 4 + size_t(n) * 4;
+  }
+};
+
 size_t embedding_backward_workspace(const Tokens& k, uint64_t, uint64_t dim) {
-  return Layout(k.rows * k.per_row, dim).bytes;
+  const uint64_t n = k.rows * k.per_row;
+  return n <= kFewTokens ? 0 : Layout(n, dim).bytes;
 }
 
 void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64_t dim, float scale,
                         const Scales& s, const Mat& out, bool accumulate, void* workspace,
                         cudaStream_t stream) {
   const uint32_t n = uint32_t(k.rows * k.per_row);
+  if (n && n <= kFewTokens) {
+    with_types(grad.type, out.type, [&](auto* pt, auto* po) {
+      using T = std::remove_pointer_t<decltype(pt)>;
+      using O = std::remove_pointer_t<decltype(po)>;
+      with_width<T>(grad, k.rows, out, vocab, dim, [&](auto width) {
+        constexpr int VE = decltype(width)::value;
+        const FewPlan plan(n, vocab, dim / VE, VE);
+        const auto kernel = s.data ? few_kernel<T, O, VE, true> : few_kernel<T, O, VE, false>;
+        if (plan.shared > 40 * 1024)
+          XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan.shared)));
+        kernel<<<dim3(plan.blocks, plan.tiles), kFewThreads, plan.shared, stream>>>(
+            static_cast<const T*>(grad.data), grad.stride, k, token_step(k), FastDiv(uint32_t(k.per_row)), n,
+            uint32_t(vocab), plan.span, s, scale, uint32_t(dim), static_cast<O*>(const_cast<void*>(out.data)),
+            out.stride, accumulate, plan.lg);
+      });
+    });
+    XGBB_CUDA(cudaGetLastError());
+    return;
+  }
   const Layout at(n, dim);
   char* w = static_cast<char*>(workspace);
   const auto u32 = [&](size_t offset) { return reinterpret_cast<uint32_t*>(w + offset); };
