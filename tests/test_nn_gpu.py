@@ -83,7 +83,9 @@ def test_bag_gradients(shape, types):
 # two digits of the sort reach.
 @pytest.mark.parametrize("rows,vocab,dim", [(255, 1, 8), (256, 2, 8), (257, 1, 3), (4095, 255, 8), (4096, 256, 8),
                                             (4097, 257, 8), (20000, 1, 40), (20011, 2, 33), (50000, 65535, 4),
-                                            (50000, 65536, 4), (3000, 70000, 2), (600001, 300, 8)])
+                                            (50000, 65536, 4), (3000, 70000, 2), (600001, 300, 8), (4200, 70000, 160),
+                                            (13000, 17, 300), (24576, 1 << 20, 4), (24577, 900, 24),
+                                            (100000, 1 << 17, 12), (250000, 3, 520)])
 def test_sorted_gradient(rows, vocab, dim):
     g = _gen(3, rows, vocab, dim)
     grad = _matrix(g, rows, dim, F32)

@@ -2,12 +2,13 @@
 //
 //   dW[v] (+)= a * sum over the (r, t) with k[r][t] == v of s[r][t] dy[r]
 //
-// The (token, position) pairs are sorted by token with a stable radix sort,
-// so that a token's positions lie side by side and in their own order. Equal
-// shares of the sorted list are then summed, and a token that crosses from
-// one share into the next is joined from the shares' partial sums. Every sum
-// has a fixed order: equal inputs give equal bits, and a frequent token costs
-// no more than many rare ones. Sums are float32, rounded once when written.
+// The present (token, position) pairs are sorted by token with a stable radix
+// sort, so that a token's positions lie side by side and in their own order.
+// Equal shares of the sorted list are then summed, and a token that crosses
+// from one share into the next is joined from the shares' partial sums. Every
+// sum has a fixed order: equal inputs give equal bits, and a frequent token
+// costs no more than many rare ones. Sums are float32, rounded once when
+// written.
 #include <algorithm>
 
 #include "nn_device.cuh"
@@ -21,12 +22,29 @@ constexpr int kItems = 16;                  // entries a thread holds of a sort 
 constexpr int kTile = kThreads * kItems;    // 4096
 constexpr int kDigits = 256;
 constexpr int kSortBlocks = 592;            // most blocks of a sort pass: 4 an SM
-constexpr uint32_t kShare = 256;            // sorted entries that one group of lanes sums
+constexpr int kOneThreads = 1024;           // of the sort in one block
+constexpr uint32_t kOneTokens = kOneThreads * 24;  // what its registers hold
+constexpr uint32_t kNone = 0xffffffffu;
 
 uint32_t sort_blocks(uint64_t n) {
   const uint64_t tiles = (n + kTile - 1) / kTile;
   return uint32_t(tiles < kSortBlocks ? tiles : kSortBlocks);
 }
+
+// How the sorted list is shared out: 2^lg lanes move a row's columns, or a tile
+// of them, and sum `share` entries. Long lists give every thread of a full card
+// one share, short ones 32 entries a share.
+struct SharePlan {
+  int lg = 0;
+  uint32_t tiles, share, shares;
+  SharePlan(uint64_t n, uint64_t pieces) {
+    while (lg < 5 && (1ull << lg) < pieces) ++lg;
+    tiles = blocks_for(pieces, 1u << lg);
+    const uint64_t even = ((n << lg) * tiles) / (148 * 2048);
+    share = uint32_t(std::min<uint64_t>(std::max<uint64_t>(32, even / 8 * 8), 1024));
+    shares = blocks_for(n, share);
+  }
+};
 
 // Where the parts of the workspace lie.
 struct Layout {
@@ -39,52 +57,80 @@ struct Layout {
       return p;
     };
     for (int i = 0; i < 2; ++i) {
-      keys[i] = take(n * 4);
-      values[i] = take(n * 4);
+      keys[i] = take(n * 4 + 32);
+      values[i] = take(n * 4 + 32);
     }
     hist = take(size_t(kDigits) * sort_blocks(n) * 4);
-    totals = take(kDigits * 4);
-    const uint64_t shares = (n + kShare - 1) / kShare;
+    totals = take((kDigits + 1) * 4);  // the digits' entries; all present entries
+    // Wider pieces make fewer lanes, fewer lanes longer shares or as long ones.
+    const uint64_t shares = SharePlan(n, (dim + 7) / 8).shares;
     head = take(shares * dim * 4);
     tail = take(shares * dim * 4);
     bytes = at;
   }
 };
 
-// The sort's entries: pass 0 reads the tokens themselves (a token that is
-// missing or past the table gets the key `vocab`, after all others; its value
-// is its position in [rows][per_row]), later passes what the pass before
-// wrote.
+// The sort's entries. The first pass reads the tokens themselves: the key of
+// one that is missing or past the table is kNone, and it is left out; the value
+// is the position in [rows][per_row], or the row. `step`: the distance of one
+// token from the next where it is the same for all, else 0. Later passes read
+// what the pass before wrote.
+enum Read { kTokens32, kTokens64, kSorted };
 struct Source {
   Tokens k;
   FastDiv per_row;
+  int64_t step;
   uint32_t vocab;
+  bool rows;
   const uint32_t* keys;
   const uint32_t* values;
-  __device__ __forceinline__ uint32_t key(uint32_t i) const {
-    if (keys) return keys[i];
-    const uint32_t r = per_row.div(i), t = i - r * per_row.d;
-    const int64_t w = load_token(k.data, k.type == kI64, int64_t(r) * k.stride_row + int64_t(t) * k.stride_col);
-    return w >= 0 && w < int64_t(vocab) ? uint32_t(w) : vocab;
+  // The keys of entries first, first + STRIDE, ..., those from `end` on none. The
+  // loads are issued together: nothing asks for a value between them.
+  template <int READ, int N, int STRIDE>
+  __device__ __forceinline__ void load_keys(uint64_t first, uint64_t end, uint32_t (&key)[N]) const {
+    if constexpr (READ == kSorted) {
+      const uint32_t* from = keys + first;
+#pragma unroll
+      for (int i = 0; i < N; ++i) key[i] = first + i * STRIDE < end ? from[i * STRIDE] : kNone;
+    } else {
+      using Token = std::conditional_t<READ == kTokens64, int64_t, int32_t>;
+      constexpr int BATCH = N < 8 ? N : 8;
+      const Token* data = static_cast<const Token*>(k.data);
+#pragma unroll
+      for (int i0 = 0; i0 < N; i0 += BATCH) {
+        Token w[BATCH];
+        if (step) {
+          const Token* from = data + int64_t(first + i0 * STRIDE) * step;
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i)
+            if (i0 + i < N)
+              w[i] = first + (i0 + i) * STRIDE < end ? from[i * (STRIDE * step)] : Token(-1);
+        } else {
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const uint32_t at = uint32_t(first) + (i0 + i) * STRIDE;
+            const uint32_t r = per_row.div(at);
+            if (i0 + i < N)
+              w[i] = first + (i0 + i) * STRIDE < end
+                         ? data[int64_t(r) * k.stride_row + int64_t(at - r * per_row.d) * k.stride_col]
+                         : Token(-1);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+          if (i0 + i < N) key[i0 + i] = uint64_t(int64_t(w[i])) < vocab ? uint32_t(w[i]) : kNone;
+      }
+    }
   }
-  __device__ __forceinline__ uint32_t value(uint32_t i) const { return values ? values[i] : i; }
+  template <int READ>
+  __device__ __forceinline__ uint32_t value(uint32_t i) const {
+    if constexpr (READ == kSorted) return values[i];
+    else return rows ? per_row.div(i) : i;
+  }
 };
 
-// Block b sorts the tiles [b * per, (b + 1) * per). hist[digit][block].
-__global__ void __launch_bounds__(kThreads)
-    sort_hist_kernel(Source src, uint32_t n, uint32_t per, int shift, uint32_t* __restrict__ hist) {
-  __shared__ uint32_t count[kDigits];
-  count[threadIdx.x] = 0;
-  __syncthreads();
-  const uint64_t begin = uint64_t(blockIdx.x) * per * kTile;
-  const uint64_t end = min(uint64_t(n), begin + uint64_t(per) * kTile);
-  for (uint64_t i = begin + threadIdx.x; i < end; i += kThreads)
-    atomicAdd(&count[(src.key(uint32_t(i)) >> shift) & (kDigits - 1)], 1u);
-  __syncthreads();
-  hist[threadIdx.x * gridDim.x + blockIdx.x] = count[threadIdx.x];
-}
-
 // Exclusive sum of one value a thread over the block; `total` gets the sum.
+template <int WARPS>
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t& total) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t x = v;
@@ -99,11 +145,57 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
   uint32_t before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     if (w < int(warp)) before += warp_sums[w];
     total += warp_sums[w];
   }
   return before + x - v;
+}
+
+// A warp's next 32 entries: each one's rank among the warp's entries of its digit
+// so far, which `count` holds. The lanes of a digit find each other by the bits
+// that they set in mask[digit], zero before and after (warp-level multisplit;
+// Ashkiani et al., "GPU multisplit", 2016).
+template <class C>
+__device__ __forceinline__ uint32_t next_rank(uint32_t digit, bool in, uint32_t* mask, C* count) {
+  const uint32_t bit = 1u << (threadIdx.x & 31);
+  if (in) atomicOr(&mask[digit], bit);
+  __syncwarp();
+  uint32_t same = 0, rank = 0;
+  if (in) {
+    same = mask[digit];
+    rank = count[digit] + __popc(same & (bit - 1));
+  }
+  __syncwarp();
+  if (same >> 1 < bit && in) {  // the digit's highest lane
+    count[digit] = C(rank + 1);
+    mask[digit] = 0;
+  }
+  __syncwarp();
+  return rank;
+}
+
+// Block b sorts the tiles [b * per, (b + 1) * per). hist[digit][block].
+template <int READ>
+__global__ void __launch_bounds__(kThreads)
+    sort_hist_kernel(Source src, const uint32_t* __restrict__ present, uint32_t n, uint32_t per, int shift,
+                     uint32_t* __restrict__ hist) {
+  constexpr int U = 8;
+  __shared__ uint32_t count[kDigits];
+  count[threadIdx.x] = 0;
+  __syncthreads();
+  if (READ == kSorted) n = *present;
+  const uint64_t begin = uint64_t(blockIdx.x) * per * kTile;
+  const uint64_t end = min(uint64_t(n), begin + uint64_t(per) * kTile);
+  for (uint64_t i = begin + threadIdx.x; i < end; i += kThreads * U) {
+    uint32_t key[U];
+    src.load_keys<READ, U, kThreads>(i, end, key);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (key[u] != kNone) atomicAdd(&count[(key[u] >> shift) & (kDigits - 1)], 1u);
+  }
+  __syncthreads();
+  hist[threadIdx.x * gridDim.x + blockIdx.x] = count[threadIdx.x];
 }
 
 // Block d: the exclusive sums of digit d's counts over the sort's blocks, in
@@ -117,7 +209,7 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t i = b + threadIdx.x;
     const uint32_t v = i < blocks ? h[i] : 0;
     uint32_t total;
-    const uint32_t x = block_scan(v, warp_sums, total);
+    const uint32_t x = block_scan<kWarps>(v, warp_sums, total);
     if (i < blocks) h[i] = before + x;
     before += total;
   }
@@ -125,213 +217,423 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Ranks a tile's entries by digit, stably: warp w holds entries [512 w, 512
-// w + 512) of it, 32 at a time; the lanes that share a digit find each other
-// by ballots over its 8 bits (warp-level multisplit; Ashkiani et al., "GPU
-// multisplit", 2016), and each warp counts its own digits. The tile is put in
-// order in shared memory and leaves it in runs of equal digits.
-__global__ void __launch_bounds__(kThreads)
-    sort_scatter_kernel(Source src, uint32_t n, uint32_t per, int shift, const uint32_t* __restrict__ hist,
-                        const uint32_t* __restrict__ totals, uint32_t* __restrict__ keys_out,
-                        uint32_t* __restrict__ values_out) {
-  __shared__ uint32_t next[kDigits];           // where the digit's next entry of this block goes
-  __shared__ uint32_t local[kDigits];          // where the digit begins in the ordered tile
-  __shared__ uint32_t count[kWarps][kDigits];  // the warp's entries of the digit, then those of the warps before it
+// w + 512) of it, 32 at a time, and counts its own digits. The tile is put in
+// order in shared memory and leaves it in runs of equal digits, while the next
+// tile's keys are on their way. The first pass tells how many entries are
+// present.
+template <int READ>
+__global__ void __launch_bounds__(kThreads, 4)
+    sort_scatter_kernel(Source src, uint32_t* __restrict__ present, uint32_t n, uint32_t per, int shift,
+                        const uint32_t* __restrict__ hist, const uint32_t* __restrict__ totals,
+                        uint32_t* __restrict__ keys_out, uint32_t* __restrict__ values_out) {
+  __shared__ uint32_t to[kDigits];            // where the digit's entries go, less their place in the ordered tile
+  __shared__ uint32_t count[kWarps][kDigits];  // the warp's entries of the digit, then where they begin in the tile
   __shared__ uint32_t warp_sums[kWarps];
   __shared__ uint32_t keys[kTile], values[kTile];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = threadIdx.x;
-  uint32_t unused;
-  next[d] = block_scan(totals[d], warp_sums, unused) + hist[d * gridDim.x + blockIdx.x];
-  const uint64_t first = uint64_t(blockIdx.x) * per;
-  for (uint32_t tile = 0; tile < per; ++tile) {
-    const uint64_t begin = (first + tile) * kTile;
-    if (begin >= n) break;
-    const uint32_t here = uint32_t(min(uint64_t(kTile), n - begin));
+  if (READ == kSorted) n = *present;
+  uint32_t all;
+  uint32_t next = block_scan<kWarps>(totals[d], warp_sums, all) + hist[d * gridDim.x + blockIdx.x];
+  if (READ != kSorted && blockIdx.x == 0 && d == 0) *present = all;
+  uint32_t* const masks = keys;  // [warps][digits], while the tile is ranked
+  const uint32_t mine = warp * (kItems * 32) + lane;
+  uint64_t begin = uint64_t(blockIdx.x) * per * kTile;
+  const uint64_t end = min(uint64_t(n), begin + uint64_t(per) * kTile);
+  uint32_t key[kItems], rank[kItems];
+  src.load_keys<READ, kItems, 32>(begin + mine, end, key);
+  for (; begin < end; begin += kTile) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) count[w][d] = 0;
+    for (int w = 0; w < kWarps; ++w) count[w][d] = masks[w * kDigits + d] = 0;
     __syncthreads();
-    uint32_t key[kItems], value[kItems], rank[kItems];
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const uint32_t at = warp * (kItems * 32) + i * 32 + lane;
-      key[i] = at < here ? src.key(uint32_t(begin) + at) : 0xffffffffu;
-      value[i] = at < here ? src.value(uint32_t(begin) + at) : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const uint32_t at = warp * (kItems * 32) + i * 32 + lane;
-      const uint32_t digit = (key[i] >> shift) & (kDigits - 1);
-      uint32_t same = __ballot_sync(0xffffffffu, at < here);
-#pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        const uint32_t set = __ballot_sync(0xffffffffu, (digit >> b) & 1u);
-        same &= (digit >> b) & 1u ? set : ~set;
-      }
-      if (at < here) rank[i] = count[warp][digit] + __popc(same & ((1u << lane) - 1));
-      __syncwarp();
-      if (at < here && (same >> lane) == 1u) count[warp][digit] += __popc(same);
-      __syncwarp();
-    }
+    for (int i = 0; i < kItems; ++i)
+      rank[i] = next_rank((key[i] >> shift) & (kDigits - 1), key[i] != kNone, masks + warp * kDigits, count[warp]);
     __syncthreads();
-    uint32_t total = 0;
+    uint32_t total = 0, tile_total;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) total += count[w][d];
+    const uint32_t local = block_scan<kWarps>(total, warp_sums, tile_total);
+    uint32_t at = local;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const uint32_t c = count[w][d];
-      count[w][d] = total;
-      total += c;
+      count[w][d] = at;
+      at += c;
     }
-    local[d] = block_scan(total, warp_sums, unused);
+    to[d] = next - local;
+    next += total;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const uint32_t at = warp * (kItems * 32) + i * 32 + lane;
-      if (at < here) {
-        const uint32_t digit = (key[i] >> shift) & (kDigits - 1);
-        const uint32_t p = local[digit] + count[warp][digit] + rank[i];
+    for (int i = 0; i < kItems; ++i)
+      if (key[i] != kNone) {
+        const uint32_t p = count[warp][(key[i] >> shift) & (kDigits - 1)] + rank[i];
         keys[p] = key[i];
-        values[p] = value[i];
+        values[p] = src.value<READ>(uint32_t(begin) + mine + i * 32);
+      }
+    src.load_keys<READ, kItems, 32>(begin + kTile + mine, end, key);
+    __syncthreads();
+    for (uint32_t p = threadIdx.x; p < tile_total; p += kThreads) {
+      const uint32_t k = keys[p], q = to[(k >> shift) & (kDigits - 1)] + p;
+      keys_out[q] = k;
+      values_out[q] = values[p];
+    }
+    __syncthreads();
+  }
+}
+
+// The whole sort of up to 1024 ITEMS entries in one block, which holds them in
+// registers, (key, position) with 16-bit positions and ranks, and passes them
+// through shared memory after each pass.
+template <int READ, int ITEMS>
+__global__ void __launch_bounds__(kOneThreads)
+    sort_one_kernel(Source src, uint32_t n, int passes, uint32_t* __restrict__ present,
+                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ values_out) {
+  constexpr int kOneWarps = kOneThreads / 32;
+  extern __shared__ __align__(16) uint32_t space[];
+  uint32_t* keys = space;                                                       // [1024 ITEMS]
+  uint16_t* at = reinterpret_cast<uint16_t*>(keys + kOneThreads * ITEMS);       // [1024 ITEMS]
+  uint16_t* count = at + kOneThreads * ITEMS;                                   // [warps][digits]
+  uint32_t* mask = reinterpret_cast<uint32_t*>(count + kOneWarps * kDigits);    // [warps][digits]
+  __shared__ uint32_t local[kDigits], warp_sums[kOneWarps];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t mine = warp * (ITEMS * 32) + lane;
+  uint32_t key[ITEMS], both[ITEMS];  // both: rank << 16 | position
+  src.load_keys<READ, ITEMS, 32>(mine, n, key);
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) both[i] = mine + i * 32;
+  for (uint32_t i = threadIdx.x; i < kOneWarps * kDigits; i += kOneThreads) mask[i] = 0;
+  uint32_t all = n;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * 8;
+    if (pass) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t p = mine + i * 32;
+        key[i] = p < all ? keys[p] : kNone;
+        both[i] = p < all ? at[p] : 0;
       }
     }
+    for (uint32_t i = threadIdx.x; i < kOneWarps * kDigits / 2; i += kOneThreads)
+      reinterpret_cast<uint32_t*>(count)[i] = 0;
     __syncthreads();
-    for (uint32_t p = threadIdx.x; p < here; p += kThreads) {
-      const uint32_t digit = (keys[p] >> shift) & (kDigits - 1);
-      const uint32_t to = next[digit] + (p - local[digit]);
-      keys_out[to] = keys[p];
-      values_out[to] = values[p];
+    uint16_t* const own = count + warp * kDigits;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      both[i] |= next_rank((key[i] >> shift) & (kDigits - 1), key[i] != kNone, mask + warp * kDigits, own) << 16;
+    __syncthreads();
+    uint32_t total = 0;
+    if (threadIdx.x < kDigits)
+#pragma unroll 8
+      for (int w = 0; w < kOneWarps; ++w) {
+        const uint32_t c = count[w * kDigits + threadIdx.x];
+        count[w * kDigits + threadIdx.x] = uint16_t(total);
+        total += c;
+      }
+    const uint32_t before = block_scan<kOneWarps>(total, warp_sums, all);
+    if (threadIdx.x < kDigits) local[threadIdx.x] = before;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (key[i] != kNone) {
+        const uint32_t digit = (key[i] >> shift) & (kDigits - 1);
+        const uint32_t p = local[digit] + own[digit] + (both[i] >> 16);
+        keys[p] = key[i];
+        at[p] = uint16_t(both[i]);
+      }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *present = all;
+  for (uint32_t p = threadIdx.x; p < all; p += kOneThreads) {
+    keys_out[p] = keys[p];
+    values_out[p] = src.value<READ>(at[p]);
+  }
+}
+
+// A row's values summed up: pairs of float32 where T comes in 16 bytes.
+template <class T, int VE>
+struct Sum {
+  static constexpr bool kPairs = sizeof(T) * VE == 16;
+  float2 two[kPairs ? VE / 2 : 1];
+  float one[kPairs ? 1 : VE];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (float2& v : two) v = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (float& v : one) v = 0.0f;
+  }
+  template <bool SCALED>
+  __device__ __forceinline__ void add(const Pack<T, VE>& p, float f) {
+    if constexpr (kPairs) {
+      float2 v[VE / 2];
+      unpack16<T>(reinterpret_cast<const uint4&>(p), v);
+#pragma unroll
+      for (int e = 0; e < VE / 2; ++e)
+        two[e] = SCALED ? fma2(make_float2(f, f), v[e], two[e]) : add2(two[e], v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) one[e] = SCALED ? fmaf(f, p.f(e), one[e]) : one[e] + p.f(e);
     }
+  }
+  __device__ __forceinline__ void get(float (&f)[VE]) const {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = kPairs ? (e % 2 ? two[kPairs ? e / 2 : 0].y : two[kPairs ? e / 2 : 0].x) : one[kPairs ? 0 : e];
+  }
+};
+
+// scale times a row's sum, into the row.
+template <class O, int VE>
+__device__ __forceinline__ void write_row(O* to, const float (&sum)[VE], float scale, bool accumulate) {
+  float y[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) y[e] = sum[e] * scale;
+  if (accumulate) {
+    const auto old = load<O, VE>(to);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) y[e] += old.f(e);
+  }
+  store_global<O, VE>(to, y);
+}
+
+// Rows without a token, in front of the others' sums: block b looks up the rows
+// [b 256, b 256 + 256) in the sorted keys, a row a thread, and zeroes the absent
+// ones: wide ones by copies behind the threads' backs, narrow ones together.
+constexpr uint32_t kZeroBytes = 8192;
+template <class O, int VE>
+__device__ __forceinline__ void zero_absent(const uint32_t* __restrict__ keys, uint32_t n, uint32_t vocab, uint32_t dim,
+                                            O* __restrict__ out, int64_t out_stride, bool bulk, uint32_t block,
+                                            uint4* zeros) {
+  __shared__ uint32_t absent[kWarps];
+  const uint32_t row = block * kThreads + threadIdx.x;
+  if (bulk) {
+    for (uint32_t i = threadIdx.x; i < kZeroBytes / 16; i += kThreads) zeros[i] = make_uint4(0, 0, 0, 0);
+    bulk_fence();
+  }
+  uint32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (keys[mid] < row) lo = mid + 1;
+    else hi = mid;
+  }
+  const bool none = row < vocab && (lo == n || keys[lo] != row);
+  if (bulk) {
     __syncthreads();
-    next[d] += total;
+    const uint32_t row_bytes = dim * sizeof(O);
+    if (none) {
+      char* to = reinterpret_cast<char*>(out + int64_t(row) * out_stride);
+      for (uint32_t at = 0; at < row_bytes; at += kZeroBytes) bulk_store(to + at, zeros, min(kZeroBytes, row_bytes - at));
+    }
+    bulk_wait_all();
+    return;
+  }
+  const uint32_t votes = __ballot_sync(0xffffffffu, none);
+  if ((threadIdx.x & 31) == 0) absent[threadIdx.x >> 5] = votes;
+  __syncthreads();
+  const float zero[VE] = {};
+  const uint32_t pieces = dim / VE;
+  for (uint64_t i = threadIdx.x; i < uint64_t(pieces) * kThreads; i += kThreads) {
+    const uint32_t r = uint32_t(i / pieces);
+    if (absent[r >> 5] >> (r & 31) & 1)
+      store_global<O, VE>(out + int64_t(block * kThreads + r) * out_stride + (i - uint64_t(r) * pieces) * VE, zero);
   }
 }
 
 // Groups of G = 2^lg lanes own VE columns a lane (blockIdx.y: the tile of
-// columns) and sum kShare sorted entries each, eight gathers in flight. A
-// token that lies in one share whole goes to its row; the sum of one that
-// came in from the share before goes to head[share], of one that goes on into
-// the next to tail[share] (a share inside one token has its sum in head).
-template <class T, class O, int VE>
-__global__ void __launch_bounds__(kThreads)
+// columns) and sum `share` sorted entries each, eight gathers in flight and the
+// next entries' keys ahead of them. A token that lies in one share whole goes to
+// its row; the sum of one that came in from the share before goes to
+// head[share], of one that goes on into the next to tail[share] (a share inside
+// one token has its sum in head). The first `zero_blocks` blocks zero the rows
+// without a token.
+template <class T, class O, int VE, bool SCALED>
+__global__ void __launch_bounds__(kThreads, 3)
     share_sum_kernel(const T* __restrict__ grad, int64_t grad_stride, const uint32_t* __restrict__ keys,
-                     const uint32_t* __restrict__ values, uint32_t n, uint32_t vocab, FastDiv per_row, Scales s,
-                     float scale, uint32_t dim, O* __restrict__ out, int64_t out_stride, bool accumulate,
-                     float* __restrict__ head, float* __restrict__ tail, int lg) {
+                     const uint32_t* __restrict__ values, const uint32_t* __restrict__ present, uint32_t share_size,
+                     uint32_t vocab, FastDiv per_row, Scales s, float scale, uint32_t dim, O* __restrict__ out,
+                     int64_t out_stride, bool accumulate, float* __restrict__ head, float* __restrict__ tail, int lg,
+                     uint32_t zero_blocks, bool bulk) {
   constexpr int U = 8;
+  __shared__ uint4 zeros[kZeroBytes / 16];
+  const uint32_t n = *present;
+  if (blockIdx.x < zero_blocks) {
+    if (blockIdx.y == 0) zero_absent<O, VE>(keys, n, vocab, dim, out, out_stride, bulk, blockIdx.x, zeros);
+    return;
+  }
   const uint32_t G = 1u << lg, lane = threadIdx.x & (G - 1);
-  const uint64_t share = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) >> lg;
+  const uint64_t share = (uint64_t(blockIdx.x - zero_blocks) * kThreads + threadIdx.x) >> lg;
   const uint32_t col = (blockIdx.y * G + lane) * VE;
-  const uint64_t begin = share * kShare;
-  const uint32_t here = begin < n ? uint32_t(min(uint64_t(kShare), n - begin)) : 0;
-  const uint32_t before = here && begin ? keys[begin - 1] : 0xffffffffu;
-  const uint32_t after = here && begin + here < n ? keys[begin + here] : 0xffffffffu;
-  float acc[VE] = {};
-  uint32_t current = 0xffffffffu;
+  const uint64_t begin = share * share_size;
+  if (begin >= n || col >= dim) return;
+  const uint32_t here = uint32_t(min(uint64_t(share_size), n - begin));
+  const uint32_t before = begin ? keys[begin - 1] : kNone;
+  const uint32_t after = begin + here < n ? keys[begin + here] : kNone;
+  const T* const columns = grad + col;
+  Sum<T, VE> acc;
+  acc.clear();
+  uint32_t current = kNone;
   bool from_before = false;
-  const auto finish = [&](bool goes_on) {  // the sum of token `current` is whole, or goes on
-    if (current < vocab && col < dim) {
-      if (from_before || goes_on) {
-        float* to = (from_before ? head : tail) + share * dim + col;
-        store<float, VE>(to, acc);
-      } else {
-        O* to = out + int64_t(current) * out_stride + col;
-        float y[VE];
-#pragma unroll
-        for (int e = 0; e < VE; ++e) y[e] = acc[e] * scale;
-        if (accumulate) {
-          const auto old = load<O, VE>(to);
-#pragma unroll
-          for (int e = 0; e < VE; ++e) y[e] += old.f(e);
-        }
-        store<O, VE>(to, y);
-      }
-    }
-  };
-  for (uint32_t j0 = 0; __any_sync(0xffffffffu, j0 < here); j0 += U) {
-    // Lane q of a group (of 8 lanes or more) reads entry q; narrower groups
-    // read all eight in each lane.
-    uint32_t key[U], row[U];
-    float f[U];
+  // Entries come eight at a time; what lies past the end is read but not used.
+  uint4 k0 = *reinterpret_cast<const uint4*>(keys + begin), k1 = *reinterpret_cast<const uint4*>(keys + begin + 4);
+  uint4 v0 = *reinterpret_cast<const uint4*>(values + begin), v1 = *reinterpret_cast<const uint4*>(values + begin + 4);
+  for (uint32_t j0 = 0; j0 < here; j0 += U) {
+    const uint32_t key[U] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+    const uint32_t value[U] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
     Pack<T, VE> v[U];
+    float f[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = j0 + u < here;
-      key[u] = in ? keys[begin + j0 + u] : 0xffffffffu;
-      const uint32_t value = in ? values[begin + j0 + u] : 0;
-      row[u] = per_row.div(value);
-      f[u] = 1.0f;
-      if (s.data && key[u] < vocab)
-        f[u] = s.data[int64_t(row[u]) * s.stride_row + int64_t(value - row[u] * per_row.d) * s.stride_col];
+    for (int u = 0; u < U; ++u)
+      if (j0 + u < here) {
+        uint32_t row = value[u];
+        if (SCALED) {
+          row = per_row.div(value[u]);
+          f[u] = s.data[int64_t(row) * s.stride_row + int64_t(value[u] - row * per_row.d) * s.stride_col];
+        }
+        v[u] = load<T, VE>(columns + int64_t(row) * grad_stride);
+      }
+    if (j0 + U < here) {
+      k0 = *reinterpret_cast<const uint4*>(keys + begin + j0 + U);
+      k1 = *reinterpret_cast<const uint4*>(keys + begin + j0 + U + 4);
+      v0 = *reinterpret_cast<const uint4*>(values + begin + j0 + U);
+      v1 = *reinterpret_cast<const uint4*>(values + begin + j0 + U + 4);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (key[u] < vocab && col < dim) v[u] = load<T, VE>(grad + int64_t(row[u]) * grad_stride + col);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (key[u] >= vocab) continue;
-      if (key[u] != current) {
-        finish(false);
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
-        current = key[u];
-        from_before = j0 + u == 0 && key[u] == before;
+      if (j0 + u < here) {
+        if (key[u] != current) {
+          if (current != kNone) {
+            float y[VE];
+            acc.get(y);
+            if (from_before) store_global<float, VE>(head + share * dim + col, y);
+            else write_row<O, VE>(out + int64_t(current) * out_stride + col, y, scale, accumulate);
+          }
+          acc.clear();
+          current = key[u];
+          from_before = j0 + u == 0 && key[u] == before;
+        }
+        acc.template add<SCALED>(v[u], SCALED ? f[u] : 1.0f);
       }
-#pragma unroll
-      for (int e = 0; e < VE; ++e) acc[e] = fmaf(f[u], v[u].f(e), acc[e]);
-    }
   }
-  finish(here && current == after);
+  float y[VE];
+  acc.get(y);
+  if (from_before) store_global<float, VE>(head + share * dim + col, y);
+  else if (current == after) store_global<float, VE>(tail + share * dim + col, y);
+  else write_row<O, VE>(out + int64_t(current) * out_stride + col, y, scale, accumulate);
 }
 
-// Block x: the token that begins in share x and goes on after it, if there is
-// one: its partial sums, joined over the block's groups in a fixed order.
+// Tokens that cross shares. A block looks at 64 shares, eight a warp: of each
+// token that begins in one of them and goes on after it, the partial sums are
+// added up in the shares' order by the warp, or by the block's warps together
+// (each every eighth share, then the warps in order) where there are over 32.
+// blockIdx.y: 32 pieces of the columns.
+constexpr uint32_t kJoinShares = 64, kLongRun = 32;
 template <class O, int VE>
 __global__ void __launch_bounds__(kThreads)
-    join_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t vocab, float scale, uint32_t dim,
-                O* __restrict__ out, int64_t out_stride, bool accumulate, const float* __restrict__ head,
-                const float* __restrict__ tail, int lg) {
-  __shared__ float part[kThreads * VE];
-  const uint32_t share = blockIdx.x;
-  const uint64_t begin = uint64_t(share) * kShare, end = begin + kShare;
-  if (end >= n) return;
-  const uint32_t token = keys[end - 1];
-  if (token >= vocab || keys[end] != token) return;
-  if (begin && keys[begin] == token && keys[begin - 1] == token) return;  // it began before
-  uint32_t lo = uint32_t(end), hi = n;  // the first entry of a later token
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (keys[mid] == token) lo = mid + 1;
-    else hi = mid;
-  }
-  const uint32_t last = (lo - 1) / kShare;
-  const uint32_t G = 1u << lg, lane = threadIdx.x & (G - 1), group = threadIdx.x >> lg, groups = kThreads >> lg;
-  const uint32_t col = (blockIdx.y * G + lane) * VE;
-  float acc[VE] = {};
-  if (col < dim) {
-    if (group == 0) {
-      const auto v = load<float, VE>(tail + uint64_t(share) * dim + col);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) acc[e] = v.f(e);
-    }
-    for (uint32_t q = share + 1 + group; q <= last; q += groups) {
-      const auto v = load<float, VE>(head + uint64_t(q) * dim + col);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) acc[e] += v.f(e);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < VE; ++e) part[threadIdx.x * VE + e] = acc[e];
+    join_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ present, uint32_t share_size,
+                float scale, uint32_t dim, O* __restrict__ out, int64_t out_stride, bool accumulate,
+                const float* __restrict__ head, const float* __restrict__ tail) {
+  constexpr int U = 8;
+  __shared__ uint32_t long_share[kJoinShares], long_last[kJoinShares], long_count;
+  __shared__ float part[kWarps][32 * VE];
+  const uint32_t n = *present, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t first = blockIdx.x * kJoinShares;
+  if (uint64_t(first + 1) * share_size >= n) return;
+  if (threadIdx.x == 0) long_count = 0;
   __syncthreads();
-  if (group != 0 || col >= dim) return;
-  for (uint32_t g = 1; g < groups; ++g)
-#pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] += part[(threadIdx.x + (g << lg)) * VE + e];
-  O* to = out + int64_t(token) * out_stride + col;
-#pragma unroll
-  for (int e = 0; e < VE; ++e) acc[e] *= scale;
-  if (accumulate) {
-    const auto old = load<O, VE>(to);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] += old.f(e);
+  // Lane i < 8 looks at the warp's share i.
+  uint32_t last = 0, token = kNone;
+  const uint32_t mine = first + warp * 8 + lane;
+  if (lane < 8 && uint64_t(mine + 1) * share_size < n) {
+    const uint32_t begin = mine * share_size, end = begin + share_size;
+    token = keys[end];
+    if (keys[end - 1] != token || (begin && keys[begin] == token && keys[begin - 1] == token)) {
+      token = kNone;
+    } else {
+      last = mine + 1;  // the share that its last entry is in
+      uint32_t tries = 0;
+      while (tries++ < 8 && uint64_t(last + 1) * share_size < n && keys[(last + 1) * share_size] == token) ++last;
+      if (tries > 8) {
+        uint32_t lo = last * share_size, hi = n;
+        while (lo < hi) {
+          const uint32_t mid = lo + (hi - lo) / 2;
+          if (keys[mid] == token) lo = mid + 1;
+          else hi = mid;
+        }
+        last = (lo - 1) / share_size;
+      }
+    }
   }
-  store<O, VE>(to, acc);
+  for (uint32_t i = 0; i < 8; ++i) {
+    const uint32_t t = __shfl_sync(0xffffffffu, token, i), to = __shfl_sync(0xffffffffu, last, i);
+    const uint32_t share = first + warp * 8 + i;
+    if (t == kNone) continue;
+    if (to - share > kLongRun) {
+      if (lane == 0) {
+        const uint32_t at = atomicAdd(&long_count, 1u);
+        long_share[at] = share;
+        long_last[at] = to;
+      }
+      continue;
+    }
+    const uint32_t c = (blockIdx.y * 32 + lane) * VE;
+    if (c < dim) {
+      const auto begun = load<float, VE>(tail + uint64_t(share) * dim + c);
+      float acc[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[e] = begun.v[e];
+#pragma unroll 8
+      for (uint32_t q = share + 1; q <= to; ++q) {
+        const auto v = load<float, VE>(head + uint64_t(q) * dim + c);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] += v.v[e];
+      }
+      write_row<O, VE>(out + int64_t(t) * out_stride + c, acc, scale, accumulate);
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = 0; i < long_count; ++i) {
+    const uint32_t share = long_share[i], to = long_last[i], t = keys[uint64_t(share + 1) * share_size];
+    const uint32_t c = (blockIdx.y * 32 + lane) * VE;
+    float acc[VE] = {};
+    if (c < dim) {
+      if (warp == 0) {
+        const auto begun = load<float, VE>(tail + uint64_t(share) * dim + c);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] = begun.v[e];
+      }
+      for (uint32_t q = share + 1 + warp; q <= to; q += kWarps * U) {
+        Pack<float, VE> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (q + u * kWarps <= to) v[u] = load<float, VE>(head + uint64_t(q + u * kWarps) * dim + c);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (q + u * kWarps <= to)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[e] += v[u].v[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) part[warp][lane * VE + e] = acc[e];
+    __syncthreads();
+    if (warp == 0 && c < dim) {
+      for (int w = 1; w < kWarps; ++w)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] += part[w][lane * VE + e];
+      write_row<O, VE>(out + int64_t(t) * out_stride + c, acc, scale, accumulate);
+    }
+    __syncthreads();
+  }
+}
+
+// Zeros into rows of `dim` values, where there is no token at all.
+template <class O, int VE>
+__global__ void __launch_bounds__(kThreads)
+    zero_rows_kernel(O* __restrict__ out, int64_t stride, uint32_t pieces, FastDiv div, uint64_t total) {
+  const float zero[VE] = {};
+  for (uint64_t i = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i < total;
+       i += uint64_t(gridDim.x) * kThreads) {
+    const uint64_t row = total <= 0xffffffffull ? div.div(uint32_t(i)) : i / pieces;
+    store_global<O, VE>(out + int64_t(row) * stride + (i - row * pieces) * VE, zero);
+  }
 }
 
 // Few tokens, in one launch: block (x, y) owns the table's rows [x span, x span
@@ -343,26 +645,30 @@ __global__ void __launch_bounds__(kThreads)
 // token from the next where it is the same for all, else 0.
 constexpr int kFewThreads = 512;
 constexpr int kShift = 15;
-constexpr uint32_t kFewTokens = 1u << kShift;
+constexpr uint32_t kFewTokens = 4096;
 
 template <class T, class O, int VE, bool SCALED>
 __global__ void __launch_bounds__(kFewThreads, 2)
     few_kernel(const T* __restrict__ grad, int64_t grad_stride, Tokens k, int64_t step, FastDiv per_row, uint32_t n,
                uint32_t vocab, uint32_t span, Scales s, float scale, uint32_t dim, O* __restrict__ out,
-               int64_t out_stride, bool accumulate, int lg) {
+               int64_t out_stride, bool accumulate, bool bulk, int lg) {
   constexpr int U = 4, kBatch = 8;
   extern __shared__ __align__(16) uint32_t space[];
   __shared__ uint32_t total;
   __shared__ int32_t first_row[kFewThreads], last_row[kFewThreads];  // of a group's share; -1: none
   float* head = reinterpret_cast<float*>(space);  // [2][threads][VE]: sums that came in, sums that go on
   float* tail = head + kFewThreads * VE;
-  uint32_t* present = space + 2 * kFewThreads * VE;  // a bit a row
+  uint32_t* zeros = space + 2 * kFewThreads * VE;  // what absent rows are copied from
+  uint32_t* present = zeros + (bulk ? kZeroBytes / 4 : 0);  // a bit a row
   uint32_t* list = present + (span + 31) / 32;
   const uint32_t lane = threadIdx.x & 31;
   const uint32_t row0 = blockIdx.x * span, rows_here = min(span, vocab - row0);
 
   // The rows' tokens, in any order: all entries differ, so the sort gives one.
   for (uint32_t i = threadIdx.x; i < (span + 31) / 32; i += kFewThreads) present[i] = 0;
+  if (bulk)
+    for (uint32_t i = threadIdx.x; i < kZeroBytes / 4; i += kFewThreads) zeros[i] = 0;
+  bulk_fence();
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
   const auto where = [&](uint32_t i) {
@@ -405,16 +711,22 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const uint32_t G = 1u << lg, me = threadIdx.x & (G - 1), group = threadIdx.x >> lg, groups = kFewThreads >> lg;
   const uint32_t col = (blockIdx.y * G + me) * VE;
   O* const mine_out = out + int64_t(row0) * out_stride + col;
-  const auto zero_absent = [&] {
+  // Absent rows: wide ones whole, a share of the range's rows for each column
+  // tile, written behind the threads' backs while they sort and sum; narrow ones
+  // by plain stores.
+  if (!accumulate && bulk) {
+    const uint32_t row_bytes = dim * sizeof(O);
+    const uint32_t last = uint32_t(uint64_t(rows_here) * (blockIdx.y + 1) / gridDim.y);
+    for (uint32_t r = uint32_t(uint64_t(rows_here) * blockIdx.y / gridDim.y) + threadIdx.x; r < last; r += kFewThreads)
+      if (!(present[r >> 5] >> (r & 31) & 1)) {
+        char* to = reinterpret_cast<char*>(out + int64_t(row0 + r) * out_stride);
+        for (uint32_t at = 0; at < row_bytes; at += kZeroBytes) bulk_store(to + at, zeros, min(kZeroBytes, row_bytes - at));
+      }
+  } else if (!accumulate && col < dim) {
     const float zero[VE] = {};
-    if (!accumulate && col < dim)
-      for (uint32_t r = group; r < rows_here; r += groups)
-        if (!(present[r >> 5] >> (r & 31) & 1)) store<O, VE>(mine_out + int64_t(r) * out_stride, zero);
-  };
-  // Half of the blocks zero first and half last, so that reading and writing
-  // overlap on an SM that holds two.
-  const bool zero_first = (blockIdx.y * gridDim.x + blockIdx.x) * 2 < gridDim.x * gridDim.y;
-  if (zero_first) zero_absent();
+    for (uint32_t r = group; r < rows_here; r += groups)
+      if (!(present[r >> 5] >> (r & 31) & 1)) store_global<O, VE>(mine_out + int64_t(r) * out_stride, zero);
+  }
 
   // By counting the smaller entries where they are few, else a bitonic network
   // whose comparators all point upwards (then what lies past the end need not
@@ -473,7 +785,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 #pragma unroll
       for (int e = 0; e < VE; ++e) y[e] += old.f(e);
     }
-    store<O, VE>(to, y);
+    store_global<O, VE>(to, y);
   };
 
   const uint32_t share = (count + groups - 1) / groups;
@@ -488,7 +800,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     float f[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t at = list[min(j + u, end - 1)] & (kFewTokens - 1), r = per_row.div(at);
+      const uint32_t at = list[min(j + u, end - 1)] & ((1u << kShift) - 1), r = per_row.div(at);
       if (SCALED) f[u] = s.data[int64_t(r) * s.stride_row + int64_t(at - r * per_row.d) * s.stride_col];
       if (col < dim) v[u] = load<T, VE>(grad + int64_t(r) * grad_stride + col);
     }
@@ -532,22 +844,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     }
     write(current, acc);
   }
-  if (!zero_first) zero_absent();
+  if (bulk) bulk_wait_all();
 }
-
-// Zeros into rows of `dim` values.
-template <class O, int VE>
-__global__ void __launch_bounds__(kThreads)
-    zero_rows_kernel(O* __restrict__ out, int64_t stride, uint32_t pieces, FastDiv div, uint64_t total) {
-  const float zero[VE] = {};
-  for (uint64_t i = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i < total;
-       i += uint64_t(gridDim.x) * kThreads) {
-    const uint64_t row = total <= 0xffffffffull ? div.div(uint32_t(i)) : i / pieces;
-    store<O, VE>(out + int64_t(row) * stride + (i - row * pieces) * VE, zero);
-  }
-}
-
-}  // namespace
 
 // The distance from each token to the next, or 0 where it varies.
 int64_t token_step(const Tokens& k) {
@@ -560,16 +858,25 @@ struct FewPlan {
   int lg = 0;
   uint32_t tiles, span, blocks;
   size_t shared;
-  FewPlan(uint32_t n, uint64_t vocab, uint64_t pieces, int ve) {
+  FewPlan(uint32_t n, uint64_t vocab, uint64_t pieces, int ve, bool bulk) {
     while (lg < 5 && (1ull << lg) < pieces) ++lg;
     tiles = blocks_for(pieces, 1u << lg);
     // About two blocks an SM: each reads all tokens.
     const uint64_t ranges = std::max<uint64_t>(1, 296 / tiles);
     span = uint32_t(std::min<uint64_t>(std::max<uint64_t>((vocab + ranges - 1) / ranges, 1), 1u << (32 - kShift)));
     blocks = blocks_for(vocab, span);
-    shared = size_t(2) * kFewThreads * ve * 4 + (span + 31) / 32 * 4 + size_t(n) * 4;
+    shared = size_t(2) * kFewThreads * ve * 4 + (bulk ? kZeroBytes : 0) + (span + 31) / 32 * 4 + size_t(n) * 4;
   }
 };
+
+// Whether whole rows can be zeroed by copies of 16-byte multiples, and are wide
+// enough for it.
+bool bulk_rows(const Mat& out, uint64_t vocab, uint64_t dim) {
+  const size_t e = type_size(out.type);
+  return dim * e >= 512 && dim * e % 16 == 0 && row_aligned(out.data, out.stride, vocab, e, 16 / e);
+}
+
+}  // namespace
 
 size_t embedding_backward_workspace(const Tokens& k, uint64_t, uint64_t dim) {
   const uint64_t n = k.rows * k.per_row;
@@ -580,68 +887,95 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
                         const Scales& s, const Mat& out, bool accumulate, void* workspace,
                         cudaStream_t stream) {
   const uint32_t n = uint32_t(k.rows * k.per_row);
-  if (n && n <= kFewTokens) {
-    with_types(grad.type, out.type, [&](auto* pt, auto* po) {
-      using T = std::remove_pointer_t<decltype(pt)>;
-      using O = std::remove_pointer_t<decltype(po)>;
-      with_width<T>(grad, k.rows, out, vocab, dim, [&](auto width) {
-        constexpr int VE = decltype(width)::value;
-        const FewPlan plan(n, vocab, dim / VE, VE);
-        const auto kernel = s.data ? few_kernel<T, O, VE, true> : few_kernel<T, O, VE, false>;
-        if (plan.shared > 40 * 1024)
-          XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan.shared)));
-        kernel<<<dim3(plan.blocks, plan.tiles), kFewThreads, plan.shared, stream>>>(
-            static_cast<const T*>(grad.data), grad.stride, k, token_step(k), FastDiv(uint32_t(k.per_row)), n,
-            uint32_t(vocab), plan.span, s, scale, uint32_t(dim), static_cast<O*>(const_cast<void*>(out.data)),
-            out.stride, accumulate, plan.lg);
-      });
-    });
-    XGBB_CUDA(cudaGetLastError());
-    return;
-  }
+  const FastDiv per_row(uint32_t(n ? k.per_row : 1));
   const Layout at(n, dim);
   char* w = static_cast<char*>(workspace);
   const auto u32 = [&](size_t offset) { return reinterpret_cast<uint32_t*>(w + offset); };
-  int from = 0;
-  if (n) {
-    const uint32_t blocks = sort_blocks(n), tiles = blocks_for(n, kTile), per = (tiles + blocks - 1) / blocks;
-    const uint32_t grid = (tiles + per - 1) / per;
-    for (int shift = 0; shift < 32 && (shift == 0 || vocab >> shift); shift += 8) {
-      const Source src{k, FastDiv(uint32_t(k.per_row)), uint32_t(vocab), shift ? u32(at.keys[from]) : nullptr,
-                       shift ? u32(at.values[from]) : nullptr};
-      const int to = shift ? from ^ 1 : 0;
-      sort_hist_kernel<<<grid, kThreads, 0, stream>>>(src, n, per, shift, u32(at.hist));
-      sort_scan_kernel<<<kDigits, kThreads, 0, stream>>>(u32(at.hist), grid, u32(at.totals));
-      sort_scatter_kernel<<<grid, kThreads, 0, stream>>>(src, n, per, shift, u32(at.hist), u32(at.totals),
-                                                         u32(at.keys[to]), u32(at.values[to]));
-      from = to;
+  int sorted = 0;
+  if (n > kFewTokens) {
+    Source src{k, per_row, token_step(k), uint32_t(vocab), s.data == nullptr, nullptr, nullptr};
+    uint32_t* present = u32(at.totals) + kDigits;
+    int passes = 1;
+    while (passes < 4 && (vocab - 1) >> (8 * passes)) ++passes;
+    const auto first_read = [&](auto&& f) {
+      if (k.type == kI64) f(std::integral_constant<int, kTokens64>());
+      else f(std::integral_constant<int, kTokens32>());
+    };
+    if (n <= kOneTokens) {
+      first_read([&](auto read) {
+        const auto go = [&](auto items) {
+          constexpr int ITEMS = decltype(items)::value;
+          const auto kernel = sort_one_kernel<decltype(read)::value, ITEMS>;
+          const size_t shared = size_t(kOneThreads) * ITEMS * 6 + kOneThreads / 32 * kDigits * 6;
+          if (shared > 40 * 1024)
+            XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)));
+          kernel<<<1, kOneThreads, shared, stream>>>(src, n, passes, present, u32(at.keys[0]), u32(at.values[0]));
+        };
+        if (n <= kOneThreads * 4) go(std::integral_constant<int, 4>());
+        else if (n <= kOneThreads * 12) go(std::integral_constant<int, 12>());
+        else go(std::integral_constant<int, 24>());
+      });
+    } else {
+      const uint32_t blocks = sort_blocks(n), tiles = blocks_for(n, kTile), per = (tiles + blocks - 1) / blocks;
+      const uint32_t grid = (tiles + per - 1) / per;
+      for (int pass = 0; pass < passes; ++pass) {
+        const auto go = [&](auto read) {
+          constexpr int READ = decltype(read)::value;
+          const int to = pass ? sorted ^ 1 : 0;
+          sort_hist_kernel<READ><<<grid, kThreads, 0, stream>>>(src, present, n, per, pass * 8, u32(at.hist));
+          sort_scan_kernel<<<kDigits, kThreads, 0, stream>>>(u32(at.hist), grid, u32(at.totals));
+          sort_scatter_kernel<READ><<<grid, kThreads, 0, stream>>>(src, present, n, per, pass * 8, u32(at.hist),
+                                                                   u32(at.totals), u32(at.keys[to]),
+                                                                   u32(at.values[to]));
+          sorted = to;
+        };
+        if (pass) go(std::integral_constant<int, kSorted>());
+        else first_read(go);
+        src.keys = u32(at.keys[sorted]);
+        src.values = u32(at.values[sorted]);
+      }
     }
   }
   with_types(grad.type, out.type, [&](auto* pt, auto* po) {
     using T = std::remove_pointer_t<decltype(pt)>;
     using O = std::remove_pointer_t<decltype(po)>;
+    const T* g = static_cast<const T*>(grad.data);
     O* y = static_cast<O*>(const_cast<void*>(out.data));
     with_width<T>(grad, k.rows, out, vocab, dim, [&](auto width) {
       constexpr int VE = decltype(width)::value;
       const uint64_t pieces = dim / VE;
-      if (!accumulate) {
+      if (!n) {
         const uint64_t total = vocab * pieces;
-        zero_rows_kernel<O, VE><<<unsigned(std::min<uint64_t>(blocks_for(total, kThreads), 148 * 8)), kThreads, 0,
-                                  stream>>>(y, out.stride, uint32_t(pieces), FastDiv(uint32_t(pieces)), total);
+        if (!accumulate)
+          zero_rows_kernel<O, VE><<<unsigned(std::min<uint64_t>((total + kThreads - 1) / kThreads, 148 * 8)), kThreads,
+                                    0, stream>>>(y, out.stride, uint32_t(pieces), FastDiv(uint32_t(pieces)), total);
+        return;
       }
-      if (!n) return;
-      int lg = 0;
-      while (lg < 5 && (1ull << lg) < pieces) ++lg;
-      const uint32_t column_tiles = blocks_for(pieces, 1u << lg), shares = blocks_for(n, kShare);
+      const bool bulk = !accumulate && bulk_rows(out, vocab, dim);
+      if (n <= kFewTokens) {
+        const FewPlan plan(n, vocab, pieces, VE, bulk);
+        const auto kernel = s.data ? few_kernel<T, O, VE, true> : few_kernel<T, O, VE, false>;
+        if (plan.shared > 40 * 1024)
+          XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan.shared)));
+        kernel<<<dim3(plan.blocks, plan.tiles), kFewThreads, plan.shared, stream>>>(
+            g, grad.stride, k, token_step(k), per_row, n, uint32_t(vocab), plan.span, s, scale, uint32_t(dim), y,
+            out.stride, accumulate, bulk, plan.lg);
+        return;
+      }
+      const SharePlan plan(n, pieces);
+      const uint32_t* present = u32(at.totals) + kDigits;
       float* head = reinterpret_cast<float*>(w + at.head);
       float* tail = reinterpret_cast<float*>(w + at.tail);
-      share_sum_kernel<T, O, VE><<<dim3(blocks_for(shares, kThreads >> lg), column_tiles), kThreads, 0, stream>>>(
-          static_cast<const T*>(grad.data), grad.stride, u32(at.keys[from]), u32(at.values[from]), n,
-          uint32_t(vocab), FastDiv(uint32_t(k.per_row)), s, scale, uint32_t(dim), y, out.stride, accumulate, head,
-          tail, lg);
-      if (shares > 1)
-        join_kernel<O, VE><<<dim3(shares, column_tiles), kThreads, 0, stream>>>(
-            u32(at.keys[from]), n, uint32_t(vocab), scale, uint32_t(dim), y, out.stride, accumulate, head, tail, lg);
+      const uint32_t zero_blocks = accumulate ? 0 : blocks_for(vocab, kThreads);
+      const auto kernel = s.data ? share_sum_kernel<T, O, VE, true> : share_sum_kernel<T, O, VE, false>;
+      kernel<<<dim3(zero_blocks + blocks_for(plan.shares, kThreads >> plan.lg), plan.tiles), kThreads, 0, stream>>>(
+          g, grad.stride, u32(at.keys[sorted]), u32(at.values[sorted]), present, plan.share, uint32_t(vocab), per_row,
+          s, scale, uint32_t(dim), y, out.stride, accumulate, head, tail, plan.lg, zero_blocks, bulk);
+      constexpr int JOIN = VE >= 4 ? 4 : VE;
+      if (plan.shares > 1)
+        join_kernel<O, JOIN><<<dim3(blocks_for(plan.shares, kJoinShares), blocks_for(dim, 32 * JOIN)), kThreads, 0,
+                               stream>>>(
+            u32(at.keys[sorted]), present, plan.share, scale, uint32_t(dim), y, out.stride, accumulate, head, tail);
     });
   });
   XGBB_CUDA(cudaGetLastError());

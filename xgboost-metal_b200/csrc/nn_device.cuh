@@ -25,7 +25,7 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // N consecutive values moved as one access of up to 16 bytes each. The
-// address has to be a multiple of min(16, N * sizeof(T)).
+// address has to be a multiple of min(32, N * sizeof(T)).
 template <class T, int N>
 struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
   T v[N];
@@ -41,6 +41,31 @@ __device__ __forceinline__ void store(T* p, const float (&f)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(f[i]);
   *reinterpret_cast<Pack<T, N>*>(p) = o;
+}
+
+// The same in global memory, where eight floats are one access of 32 bytes.
+template <class T, int N>
+__device__ __forceinline__ void store_global(T* p, const float (&f)[N]) {
+  if constexpr (sizeof(T) * N == 32) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]),
+                 "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                 : "memory");
+  } else {
+    store<T, N>(p, f);
+  }
+}
+
+// Shared memory to global memory behind the threads' backs, both and the size
+// in multiples of 16 bytes. What the threads wrote to the source has to be
+// fenced before, and the issuing thread waits for its copies before it ends.
+__device__ __forceinline__ void bulk_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bulk_store(void* to, const void* from, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to),
+               "r"(uint32_t(__cvta_generic_to_shared(from))), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() {
+  asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // Two float32 operations in one instruction.
@@ -155,9 +180,9 @@ __device__ __forceinline__ int64_t load_token(const void* data, bool wide, int64
   return wide ? static_cast<const int64_t*>(data)[at] : int64_t(static_cast<const int32_t*>(data)[at]);
 }
 
-// Whether every row starts at a multiple of n values' bytes, or of 16.
+// Whether every row starts at a multiple of n values' bytes, or of 32.
 inline bool row_aligned(const void* p, int64_t stride, uint64_t rows, size_t size, uint64_t n) {
-  const size_t b = n * size < 16 ? n * size : 16;
+  const size_t b = n * size < 32 ? n * size : 32;
   return reinterpret_cast<uintptr_t>(p) % b == 0 && (rows <= 1 || (stride * int64_t(size)) % int64_t(b) == 0);
 }
 
