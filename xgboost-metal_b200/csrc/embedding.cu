@@ -53,17 +53,18 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int j = 0; j < VE; ++j)
       y[j] = uint64_t(token[u]) < vocab ? f[u] * v[u].f(j) : token[u] < 0 ? 0.0f : nan;
-    store<O, VE>(out + int64_t(row[u]) * out_stride + piece[u] * VE, y);
+    store_global<O, VE>(out + int64_t(row[u]) * out_stride + piece[u] * VE, y);
   }
 }
 
 // A bag a row: 2^lg lanes own a row's columns (or a tile of them), VE values
 // each; S = 2^ls such groups share a row's tokens, a contiguous span each, and
 // add their sums up in shared memory, first span first. A group reads its
-// tokens K to a lane and hands them round by shuffles, eight gathers in flight.
-template <class T, class O, int VE, int K>
-__global__ void __launch_bounds__(kThreads)
-    bag_kernel(Tokens k, const T* __restrict__ table, int64_t table_stride, uint64_t vocab, uint32_t dim,
+// tokens K to a lane, a step ahead, and hands them round by shuffles, eight
+// gathers in flight.
+template <class T, class O, int VE, int K, bool SCALED>
+__global__ void __launch_bounds__(kThreads, (Sum<T, VE>::kPairs && K == 1 ? 4 : 2))
+    bag_kernel(Tokens k, const T* __restrict__ table, int64_t table_stride, uint32_t vocab, uint32_t dim,
                float scale, Scales s, O* __restrict__ out, int64_t out_stride, int lg, int ls, float nan) {
   constexpr int U = 8;
   __shared__ float part[kThreads * VE];
@@ -72,23 +73,39 @@ __global__ void __launch_bounds__(kThreads)
   const uint64_t row = uint64_t(blockIdx.x) * (kThreads >> (lg + ls)) + (group >> ls);
   const uint32_t col = (blockIdx.y * G + lane) * VE;
   const bool wide = k.type == kI64;
-  const int64_t T_all = int64_t(k.per_row), per = (T_all + S - 1) >> ls;
-  const int64_t t_end = row < k.rows ? min(T_all, per * (span + 1)) : 0;
-  const int64_t token_row = int64_t(row) * k.stride_row, scale_row = int64_t(row) * s.stride_row;
-  float acc[VE] = {};
+  const uint32_t count = uint32_t(k.per_row), per = (count + S - 1) >> ls;
+  const uint32_t begin = min(count, per * span), end = row < k.rows ? min(count, begin + per) : 0;
+  // Lanes past the last column read the last piece, and write nothing.
+  const T* const columns = table + min(col, dim - VE);
+  const char* const tokens = static_cast<const char*>(k.data) + int64_t(row) * k.stride_row * (wide ? 8 : 4);
+  const float* const scales = SCALED ? s.data + int64_t(row) * s.stride_row : nullptr;
+  Sum<T, VE> acc;
+  acc.clear();
   bool bad = false;
-  for (int64_t t0 = per * span; __any_sync(0xffffffffu, t0 < t_end); t0 += G * K) {
-    int token[K];
-    float f[K];
+  int token[K], next[K];  // -1: missing, past the table, or past the span
+  float f[K], next_f[K];
+  const auto fetch = [&](uint32_t t0) {
 #pragma unroll
     for (int i = 0; i < K; ++i) {
-      const int64_t t = t0 + i * int(G) + lane;
+      const uint32_t t = t0 + i * G + lane;
       int64_t w = -1;
-      if (t < t_end) w = load_token(k.data, wide, token_row + t * k.stride_col);
-      f[i] = s.data && w >= 0 ? s.data[scale_row + t * s.stride_col] : 1.0f;
+      if (t < end) w = load_token(tokens, wide, int64_t(t) * k.stride_col);
+      next[i] = uint64_t(w) < vocab ? int(w) : -1;
       bad |= w >= int64_t(vocab);
-      token[i] = w >= 0 && w < int64_t(vocab) ? int(w) : -1;
+      if (SCALED) next_f[i] = next[i] >= 0 ? scales[int64_t(t) * s.stride_col] : 0.0f;
     }
+  };
+  fetch(begin);
+  for (uint32_t t0 = begin; __any_sync(0xffffffffu, t0 < end); t0 += G * K) {
+    bool whole = true;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      token[i] = next[i];
+      whole = whole && token[i] >= 0;
+      if (SCALED) f[i] = next_f[i];
+    }
+    whole = __all_sync(0xffffffffu, whole);
+    fetch(t0 + G * K);
     const uint32_t steps = K > 1 ? 8 : G;
     for (uint32_t j = 0; j < steps; j += U) {
       Pack<T, VE> v[U];
@@ -98,34 +115,43 @@ __global__ void __launch_bounds__(kThreads)
       for (int u = 0; u < U; ++u) {
         const int slot = K > 1 ? u / (8 / K) : 0, from = K > 1 ? u % (8 / K) : int(j) + u;
         at[u] = __shfl_sync(0xffffffffu, token[slot], from, G);
-        ff[u] = __shfl_sync(0xffffffffu, f[slot], from, G);
-        if (at[u] >= 0 && col < dim) v[u] = load<T, VE>(table + at[u] * table_stride + col);
+        if (SCALED) ff[u] = __shfl_sync(0xffffffffu, f[slot], from, G);
       }
+      if (whole) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (at[u] >= 0)
+        for (int u = 0; u < U; ++u) v[u] = load<T, VE>(columns + at[u] * table_stride);
 #pragma unroll
-          for (int e = 0; e < VE; ++e) acc[e] = fmaf(ff[u], v[u].f(e), acc[e]);
+        for (int u = 0; u < U; ++u) acc.template add<SCALED>(v[u], SCALED ? ff[u] : 1.0f);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (at[u] >= 0) v[u] = load<T, VE>(columns + at[u] * table_stride);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (at[u] >= 0) acc.template add<SCALED>(v[u], SCALED ? ff[u] : 1.0f);
+      }
     }
   }
   // A token past the table anywhere in the group's span.
   for (uint32_t m = 1; m < G; m <<= 1) bad |= __shfl_xor_sync(0xffffffffu, int(bad), m) != 0;
+  float sum[VE];
+  acc.get(sum);
   if (bad)
 #pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] = nan;
+    for (int e = 0; e < VE; ++e) sum[e] = nan;
   if (S > 1) {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) part[threadIdx.x * VE + e] = acc[e];
+    for (int e = 0; e < VE; ++e) part[threadIdx.x * VE + e] = sum[e];
     __syncthreads();
     if (span == 0)
       for (uint32_t q = 1; q < S; ++q)
 #pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] += part[(threadIdx.x + (q << lg)) * VE + e];
+        for (int e = 0; e < VE; ++e) sum[e] += part[(threadIdx.x + (q << lg)) * VE + e];
   }
   if (span == 0 && row < k.rows && col < dim) {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] *= scale;
-    store<O, VE>(out + int64_t(row) * out_stride + col, acc);
+    for (int e = 0; e < VE; ++e) sum[e] *= scale;
+    store_global<O, VE>(out + int64_t(row) * out_stride + col, sum);
   }
 }
 
@@ -184,8 +210,10 @@ void embedding(const Tokens& k, const Mat& table, uint64_t vocab, uint64_t dim, 
       while (lg + ls < 8 && k.rows * tiles << (lg + ls) < 148 * 1024 && k.per_row >> (ls + 1) >= 8) ++ls;
       const dim3 grid(blocks_for(k.rows, kThreads >> (lg + ls)), tiles);
       const auto go = [&](auto kk) {
-        bag_kernel<T, O, VE, decltype(kk)::value><<<grid, kThreads, 0, stream>>>(
-            k, w, table.stride, vocab, uint32_t(dim), scale, s, y, out.stride, lg, ls, kNaN);
+        constexpr int K = decltype(kk)::value;
+        const auto kernel = s.data ? bag_kernel<T, O, VE, K, true> : bag_kernel<T, O, VE, K, false>;
+        kernel<<<grid, kThreads, 0, stream>>>(k, w, table.stride, uint32_t(vocab), uint32_t(dim), scale, s, y,
+                                              out.stride, lg, ls, kNaN);
       };
       if (lg >= 3) go(std::integral_constant<int, 1>());
       else if (lg == 2) go(std::integral_constant<int, 2>());

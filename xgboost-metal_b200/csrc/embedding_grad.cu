@@ -32,16 +32,16 @@ uint32_t sort_blocks(uint64_t n) {
 }
 
 // How the sorted list is shared out: 2^lg lanes move a row's columns, or a tile
-// of them, and sum `share` entries. Long lists give every thread of a full card
-// one share, short ones 32 entries a share.
+// of them, and sum `share` entries. Long lists give each of the 1024 threads that
+// an SM holds one share, short ones 32 entries a share.
 struct SharePlan {
   int lg = 0;
   uint32_t tiles, share, shares;
   SharePlan(uint64_t n, uint64_t pieces) {
     while (lg < 5 && (1ull << lg) < pieces) ++lg;
     tiles = blocks_for(pieces, 1u << lg);
-    const uint64_t even = ((n << lg) * tiles) / (148 * 2048);
-    share = uint32_t(std::min<uint64_t>(std::max<uint64_t>(32, even / 8 * 8), 1024));
+    const uint64_t even = ((n << lg) * tiles + 148 * 1024 - 1) / (148 * 1024);
+    share = uint32_t(std::min<uint64_t>(std::max<uint64_t>(32, (even + 7) / 8 * 8), 4096));
     shares = blocks_for(n, share);
   }
 };
@@ -57,8 +57,8 @@ struct Layout {
       return p;
     };
     for (int i = 0; i < 2; ++i) {
-      keys[i] = take(n * 4 + 32);
-      values[i] = take(n * 4 + 32);
+      keys[i] = take(n * 4 + 512);  // a round of 32 lanes may read past the end
+      values[i] = take(n * 4 + 512);
     }
     hist = take(size_t(kDigits) * sort_blocks(n) * 4);
     totals = take((kDigits + 1) * 4);  // the digits' entries; all present entries
@@ -349,37 +349,6 @@ __global__ void __launch_bounds__(kOneThreads)
   }
 }
 
-// A row's values summed up: pairs of float32 where T comes in 16 bytes.
-template <class T, int VE>
-struct Sum {
-  static constexpr bool kPairs = sizeof(T) * VE == 16;
-  float2 two[kPairs ? VE / 2 : 1];
-  float one[kPairs ? 1 : VE];
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (float2& v : two) v = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (float& v : one) v = 0.0f;
-  }
-  template <bool SCALED>
-  __device__ __forceinline__ void add(const Pack<T, VE>& p, float f) {
-    if constexpr (kPairs) {
-      float2 v[VE / 2];
-      unpack16<T>(reinterpret_cast<const uint4&>(p), v);
-#pragma unroll
-      for (int e = 0; e < VE / 2; ++e)
-        two[e] = SCALED ? fma2(make_float2(f, f), v[e], two[e]) : add2(two[e], v[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) one[e] = SCALED ? fmaf(f, p.f(e), one[e]) : one[e] + p.f(e);
-    }
-  }
-  __device__ __forceinline__ void get(float (&f)[VE]) const {
-#pragma unroll
-    for (int e = 0; e < VE; ++e) f[e] = kPairs ? (e % 2 ? two[kPairs ? e / 2 : 0].y : two[kPairs ? e / 2 : 0].x) : one[kPairs ? 0 : e];
-  }
-};
-
 // scale times a row's sum, into the row.
 template <class O, int VE>
 __device__ __forceinline__ void write_row(O* to, const float (&sum)[VE], float scale, bool accumulate) {
@@ -438,85 +407,129 @@ __device__ __forceinline__ void zero_absent(const uint32_t* __restrict__ keys, u
 }
 
 // Groups of G = 2^lg lanes own VE columns a lane (blockIdx.y: the tile of
-// columns) and sum `share` sorted entries each, eight gathers in flight and the
-// next entries' keys ahead of them. A token that lies in one share whole goes to
-// its row; the sum of one that came in from the share before goes to
-// head[share], of one that goes on into the next to tail[share] (a share inside
-// one token has its sum in head). The first `zero_blocks` blocks zero the rows
-// without a token.
+// columns) and sum `share` sorted entries each. The lanes read four entries
+// each, a round ahead, and hand them round by shuffles; a round that lies in one
+// token, as most do where tokens are frequent, is summed without a look at its
+// keys. A token that lies in one share whole goes to its row; the sum of one
+// that came in from the share before goes to head[share], of one that goes on
+// into the next to tail[share] (a share inside one token has its sum in head).
+// The first `zero_blocks` blocks zero the rows without a token.
 template <class T, class O, int VE, bool SCALED>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 4)
     share_sum_kernel(const T* __restrict__ grad, int64_t grad_stride, const uint32_t* __restrict__ keys,
                      const uint32_t* __restrict__ values, const uint32_t* __restrict__ present, uint32_t share_size,
                      uint32_t vocab, FastDiv per_row, Scales s, float scale, uint32_t dim, O* __restrict__ out,
                      int64_t out_stride, bool accumulate, float* __restrict__ head, float* __restrict__ tail, int lg,
                      uint32_t zero_blocks, bool bulk) {
-  constexpr int U = 8;
   __shared__ uint4 zeros[kZeroBytes / 16];
   const uint32_t n = *present;
   if (blockIdx.x < zero_blocks) {
     if (blockIdx.y == 0) zero_absent<O, VE>(keys, n, vocab, dim, out, out_stride, bulk, blockIdx.x, zeros);
     return;
   }
-  const uint32_t G = 1u << lg, lane = threadIdx.x & (G - 1);
+  const uint32_t G = 1u << lg, lane = threadIdx.x & (G - 1), E = 4 * G;
+  const uint32_t mask = (G == 32 ? ~0u : (1u << G) - 1) << (threadIdx.x & 31 & ~(G - 1));
   const uint64_t share = (uint64_t(blockIdx.x - zero_blocks) * kThreads + threadIdx.x) >> lg;
   const uint32_t col = (blockIdx.y * G + lane) * VE;
   const uint64_t begin = share * share_size;
-  if (begin >= n || col >= dim) return;
+  if (begin >= n) return;  // the whole group
   const uint32_t here = uint32_t(min(uint64_t(share_size), n - begin));
   const uint32_t before = begin ? keys[begin - 1] : kNone;
   const uint32_t after = begin + here < n ? keys[begin + here] : kNone;
-  const T* const columns = grad + col;
+  // Lanes past the last column read the last piece, and write nothing.
+  const T* const columns = grad + min(col, dim - VE);
   Sum<T, VE> acc;
   acc.clear();
   uint32_t current = kNone;
   bool from_before = false;
-  // Entries come eight at a time; what lies past the end is read but not used.
-  uint4 k0 = *reinterpret_cast<const uint4*>(keys + begin), k1 = *reinterpret_cast<const uint4*>(keys + begin + 4);
-  uint4 v0 = *reinterpret_cast<const uint4*>(values + begin), v1 = *reinterpret_cast<const uint4*>(values + begin + 4);
-  for (uint32_t j0 = 0; j0 < here; j0 += U) {
-    const uint32_t key[U] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
-    const uint32_t value[U] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-    Pack<T, VE> v[U];
-    float f[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (j0 + u < here) {
-        uint32_t row = value[u];
-        if (SCALED) {
-          row = per_row.div(value[u]);
-          f[u] = s.data[int64_t(row) * s.stride_row + int64_t(value[u] - row * per_row.d) * s.stride_col];
-        }
-        v[u] = load<T, VE>(columns + int64_t(row) * grad_stride);
-      }
-    if (j0 + U < here) {
-      k0 = *reinterpret_cast<const uint4*>(keys + begin + j0 + U);
-      k1 = *reinterpret_cast<const uint4*>(keys + begin + j0 + U + 4);
-      v0 = *reinterpret_cast<const uint4*>(values + begin + j0 + U);
-      v1 = *reinterpret_cast<const uint4*>(values + begin + j0 + U + 4);
+  const auto finish = [&](bool goes_on) {
+    if (current == kNone || col >= dim) return;
+    float y[VE];
+    acc.get(y);
+    if (from_before || goes_on) store_global<float, VE>((from_before ? head : tail) + share * dim + col, y);
+    else write_row<O, VE>(out + int64_t(current) * out_stride + col, y, scale, accumulate);
+  };
+  // What a round reads past the list's end is not used.
+  const uint4* key4 = reinterpret_cast<const uint4*>(keys + begin) + lane;
+  const uint4* value4 = reinterpret_cast<const uint4*>(values + begin) + lane;
+  uint4 next_key = *key4, next_value = *value4;
+  for (uint32_t r0 = 0; r0 < here; r0 += E) {
+    const uint4 key = next_key;
+    uint4 row = next_value;
+    float4 f = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+    if (r0 + E < here) {
+      key4 += G;
+      value4 += G;
+      next_key = *key4;
+      next_value = *value4;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (j0 + u < here) {
-        if (key[u] != current) {
-          if (current != kNone) {
-            float y[VE];
-            acc.get(y);
-            if (from_before) store_global<float, VE>(head + share * dim + col, y);
-            else write_row<O, VE>(out + int64_t(current) * out_stride + col, y, scale, accumulate);
-          }
-          acc.clear();
-          current = key[u];
-          from_before = j0 + u == 0 && key[u] == before;
+    if (SCALED) {
+      const auto look = [&](uint32_t i, uint32_t& value) {
+        float v = 0.0f;
+        if (r0 + lane * 4 + i < here) {
+          const uint32_t r = per_row.div(value);
+          v = s.data[int64_t(r) * s.stride_row + int64_t(value - r * per_row.d) * s.stride_col];
+          value = r;
         }
-        acc.template add<SCALED>(v[u], SCALED ? f[u] : 1.0f);
+        return v;
+      };
+      f.x = look(0, row.x);
+      f.y = look(1, row.y);
+      f.z = look(2, row.z);
+      f.w = look(3, row.w);
+    }
+    const bool one = r0 + E <= here && __shfl_sync(mask, key.w, G - 1, G) == current;
+    if (one) {
+#pragma unroll 2
+      for (uint32_t q = 0; q < G; ++q) {
+        const uint32_t at[4] = {__shfl_sync(mask, row.x, q, G), __shfl_sync(mask, row.y, q, G),
+                                __shfl_sync(mask, row.z, q, G), __shfl_sync(mask, row.w, q, G)};
+        float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+        if (SCALED) {
+          g[0] = __shfl_sync(mask, f.x, q, G);
+          g[1] = __shfl_sync(mask, f.y, q, G);
+          g[2] = __shfl_sync(mask, f.z, q, G);
+          g[3] = __shfl_sync(mask, f.w, q, G);
+        }
+        Pack<T, VE> v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = load<T, VE>(columns + int64_t(at[u]) * grad_stride);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc.template add<SCALED>(v[u], g[u]);
       }
+      continue;
+    }
+    for (uint32_t q = 0; q < G && r0 + q * 4 < here; ++q) {
+      const uint32_t k[4] = {__shfl_sync(mask, key.x, q, G), __shfl_sync(mask, key.y, q, G),
+                             __shfl_sync(mask, key.z, q, G), __shfl_sync(mask, key.w, q, G)};
+      const uint32_t at[4] = {__shfl_sync(mask, row.x, q, G), __shfl_sync(mask, row.y, q, G),
+                              __shfl_sync(mask, row.z, q, G), __shfl_sync(mask, row.w, q, G)};
+      float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+      if (SCALED) {
+        g[0] = __shfl_sync(mask, f.x, q, G);
+        g[1] = __shfl_sync(mask, f.y, q, G);
+        g[2] = __shfl_sync(mask, f.z, q, G);
+        g[3] = __shfl_sync(mask, f.w, q, G);
+      }
+      const uint32_t left = here - (r0 + q * 4);
+      Pack<T, VE> v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (u < left) v[u] = load<T, VE>(columns + int64_t(at[u]) * grad_stride);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (u < left) {
+          if (k[u] != current) {
+            finish(false);
+            acc.clear();
+            current = k[u];
+            from_before = r0 + q + u == 0 && k[u] == before;
+          }
+          acc.template add<SCALED>(v[u], g[u]);
+        }
+    }
   }
-  float y[VE];
-  acc.get(y);
-  if (from_before) store_global<float, VE>(head + share * dim + col, y);
-  else if (current == after) store_global<float, VE>(tail + share * dim + col, y);
-  else write_row<O, VE>(out + int64_t(current) * out_stride + col, y, scale, accumulate);
+  finish(current == after);
 }
 
 // Tokens that cross shares. A block looks at 64 shares, eight a warp: of each

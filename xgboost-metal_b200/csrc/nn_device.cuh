@@ -147,6 +147,37 @@ __device__ __forceinline__ void load_pairs(const P* p, float2 (&f)[H]) {
   }
 }
 
+// A row's values summed up: pairs of float32 where T comes in 16 bytes.
+template <class T, int VE>
+struct Sum {
+  static constexpr bool kPairs = sizeof(T) * VE == 16;
+  float2 two[kPairs ? VE / 2 : 1];
+  float one[kPairs ? 1 : VE];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (float2& v : two) v = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (float& v : one) v = 0.0f;
+  }
+  template <bool SCALED>
+  __device__ __forceinline__ void add(const Pack<T, VE>& p, float f) {
+    if constexpr (kPairs) {
+      float2 v[VE / 2];
+      unpack16<T>(reinterpret_cast<const uint4&>(p), v);
+#pragma unroll
+      for (int e = 0; e < VE / 2; ++e)
+        two[e] = SCALED ? fma2(make_float2(f, f), v[e], two[e]) : add2(two[e], v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) one[e] = SCALED ? fmaf(f, p.f(e), one[e]) : one[e] + p.f(e);
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[VE]) const {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = kPairs ? (e % 2 ? two[kPairs ? e / 2 : 0].y : two[kPairs ? e / 2 : 0].x) : one[kPairs ? 0 : e];
+  }
+};
+
 // Copies 16 bytes into shared memory behind the thread's back; a thread that
 // waits for its own copies needs no barrier to read them.
 __device__ __forceinline__ void copy_async16(void* to, const void* from) {
