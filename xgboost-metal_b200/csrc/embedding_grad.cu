@@ -25,6 +25,7 @@ constexpr int kSortBlocks = 592;            // most blocks of a sort pass: 4 an 
 constexpr int kOneThreads = 1024;           // of the sort in one block
 constexpr uint32_t kOneTokens = kOneThreads * 24;  // what its registers hold
 constexpr uint32_t kNone = 0xffffffffu;
+constexpr uint32_t kZeroBytes = 8192;              // zeros that wide rows are copied from
 
 uint32_t sort_blocks(uint64_t n) {
   const uint64_t tiles = (n + kTile - 1) / kTile;
@@ -281,24 +282,83 @@ __global__ void __launch_bounds__(kThreads, 4)
   }
 }
 
+// The rows without a token, for blocks beside a block that sorts: block b of
+// `blocks` looks through all tokens for those of its equal share of the rows and
+// zeroes the others: wide rows by copies behind the threads' backs, narrow ones
+// by plain stores. No block at all where there is nothing to zero.
+struct Rows {
+  char* data;
+  int64_t stride;  // bytes
+  uint32_t bytes, item;
+  bool bulk;
+};
+template <int READ>
+__device__ __forceinline__ void zero_rows_beside(const Source& src, uint32_t n, const Rows& rows, uint32_t block,
+                                                 uint32_t blocks, uint32_t* space) {
+  constexpr int U = 8;
+  const uint32_t first = uint32_t(uint64_t(src.vocab) * block / blocks);
+  const uint32_t here = uint32_t(uint64_t(src.vocab) * (block + 1) / blocks) - first;
+  uint32_t* zeros = space;
+  uint32_t* present = space + kZeroBytes / 4;  // a bit a row
+  const uint32_t batch_rows = 32 * 1024;       // rows that the bits are for at a time
+  for (uint32_t i = threadIdx.x; i < kZeroBytes / 4; i += kOneThreads) zeros[i] = 0;
+  bulk_fence();
+  for (uint32_t r0 = 0; r0 < here; r0 += batch_rows) {
+    const uint32_t count = min(batch_rows, here - r0), row0 = first + r0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < (count + 31) / 32; i += kOneThreads) present[i] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kOneThreads * U) {
+      uint32_t key[U];
+      src.load_keys<READ, U, kOneThreads>(i, n, key);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (key[u] - row0 < count) atomicOr(&present[(key[u] - row0) >> 5], 1u << ((key[u] - row0) & 31));
+    }
+    __syncthreads();
+    if (rows.bulk) {
+      for (uint32_t r = threadIdx.x; r < count; r += kOneThreads)
+        if (!(present[r >> 5] >> (r & 31) & 1)) {
+          char* to = rows.data + int64_t(row0 + r) * rows.stride;
+          for (uint32_t at = 0; at < rows.bytes; at += kZeroBytes)
+            bulk_store(to + at, zeros, min(kZeroBytes, rows.bytes - at));
+        }
+    } else {
+      const uint32_t items = rows.bytes / rows.item, lane = threadIdx.x & 31;
+      for (uint32_t r = threadIdx.x >> 5; r < count; r += kOneThreads / 32)
+        if (!(present[r >> 5] >> (r & 31) & 1)) {
+          char* to = rows.data + int64_t(row0 + r) * rows.stride;
+          for (uint32_t i = lane; i < items; i += 32) {
+            if (rows.item == 4) reinterpret_cast<uint32_t*>(to)[i] = 0;
+            else reinterpret_cast<uint16_t*>(to)[i] = 0;
+          }
+        }
+    }
+  }
+  bulk_wait_all();
+}
+
 // The whole sort of up to 1024 ITEMS entries in one block, which holds them in
 // registers, (key, position) with 16-bit positions and ranks, and passes them
-// through shared memory after each pass.
+// through shared memory after each pass. The other blocks zero the rows that
+// have no token meanwhile.
 template <int READ, int ITEMS>
 __global__ void __launch_bounds__(kOneThreads)
     sort_one_kernel(Source src, uint32_t n, int passes, uint32_t* __restrict__ present,
-                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ values_out) {
+                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ values_out, Rows rows) {
   constexpr int kOneWarps = kOneThreads / 32;
   extern __shared__ __align__(16) uint32_t space[];
+  if (blockIdx.x) return zero_rows_beside<READ>(src, n, rows, blockIdx.x - 1, gridDim.x - 1, space);
   uint32_t* keys = space;                                                       // [1024 ITEMS]
   uint16_t* at = reinterpret_cast<uint16_t*>(keys + kOneThreads * ITEMS);       // [1024 ITEMS]
   uint16_t* count = at + kOneThreads * ITEMS;                                   // [warps][digits]
   uint32_t* mask = reinterpret_cast<uint32_t*>(count + kOneWarps * kDigits);    // [warps][digits]
-  __shared__ uint32_t local[kDigits], warp_sums[kOneWarps];
+  __shared__ uint32_t warp_sums[kOneWarps];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t mine = warp * (ITEMS * 32) + lane;
+  const uint32_t turns = (n + kOneThreads - 1) / kOneThreads;  // at most ITEMS
+  const uint32_t mine = warp * (turns * 32) + lane;
   uint32_t key[ITEMS], both[ITEMS];  // both: rank << 16 | position
-  src.load_keys<READ, ITEMS, 32>(mine, n, key);
+  src.load_keys<READ, ITEMS, 32>(mine, min(n, (warp + 1) * turns * 32), key);
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) both[i] = mine + i * 32;
   for (uint32_t i = threadIdx.x; i < kOneWarps * kDigits; i += kOneThreads) mask[i] = 0;
@@ -309,8 +369,9 @@ __global__ void __launch_bounds__(kOneThreads)
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         const uint32_t p = mine + i * 32;
-        key[i] = p < all ? keys[p] : kNone;
-        both[i] = p < all ? at[p] : 0;
+        const bool in = i < turns && p < all;
+        key[i] = in ? keys[p] : kNone;
+        both[i] = in ? at[p] : 0;
       }
     }
     for (uint32_t i = threadIdx.x; i < kOneWarps * kDigits / 2; i += kOneThreads)
@@ -319,24 +380,28 @@ __global__ void __launch_bounds__(kOneThreads)
     uint16_t* const own = count + warp * kDigits;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
-      both[i] |= next_rank((key[i] >> shift) & (kDigits - 1), key[i] != kNone, mask + warp * kDigits, own) << 16;
+      if (i < turns)
+        both[i] |= next_rank((key[i] >> shift) & (kDigits - 1), key[i] != kNone, mask + warp * kDigits, own) << 16;
     __syncthreads();
-    uint32_t total = 0;
-    if (threadIdx.x < kDigits)
-#pragma unroll 8
-      for (int w = 0; w < kOneWarps; ++w) {
-        const uint32_t c = count[w * kDigits + threadIdx.x];
-        count[w * kDigits + threadIdx.x] = uint16_t(total);
-        total += c;
-      }
-    const uint32_t before = block_scan<kOneWarps>(total, warp_sums, all);
-    if (threadIdx.x < kDigits) local[threadIdx.x] = before;
+    // A digit's warps, eight to a thread: their counts' sums, then their places.
+    const uint32_t digit = threadIdx.x >> 2, w0 = (threadIdx.x & 3) * 8;
+    uint32_t c[8], eight = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      c[w] = count[(w0 + w) * kDigits + digit];
+      eight += c[w];
+    }
+    uint32_t place = block_scan<kOneWarps>(eight, warp_sums, all);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      count[(w0 + w) * kDigits + digit] = uint16_t(place);
+      place += c[w];
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
       if (key[i] != kNone) {
-        const uint32_t digit = (key[i] >> shift) & (kDigits - 1);
-        const uint32_t p = local[digit] + own[digit] + (both[i] >> 16);
+        const uint32_t p = own[(key[i] >> shift) & (kDigits - 1)] + (both[i] >> 16);
         keys[p] = key[i];
         at[p] = uint16_t(both[i]);
       }
@@ -366,7 +431,6 @@ __device__ __forceinline__ void write_row(O* to, const float (&sum)[VE], float s
 // Rows without a token, in front of the others' sums: block b looks up the rows
 // [b 256, b 256 + 256) in the sorted keys, a row a thread, and zeroes the absent
 // ones: wide ones by copies behind the threads' backs, narrow ones together.
-constexpr uint32_t kZeroBytes = 8192;
 template <class O, int VE>
 __device__ __forceinline__ void zero_absent(const uint32_t* __restrict__ keys, uint32_t n, uint32_t vocab, uint32_t dim,
                                             O* __restrict__ out, int64_t out_stride, bool bulk, uint32_t block,
@@ -532,87 +596,66 @@ __global__ void __launch_bounds__(kThreads, 4)
   finish(current == after);
 }
 
-// Tokens that cross shares. A block looks at 64 shares, eight a warp: of each
-// token that begins in one of them and goes on after it, the partial sums are
-// added up in the shares' order by the warp, or by the block's warps together
-// (each every eighth share, then the warps in order) where there are over 32.
-// blockIdx.y: 32 pieces of the columns.
-constexpr uint32_t kJoinShares = 64, kLongRun = 32;
+// Tokens that cross shares. A warp looks at one share: of the token that begins
+// in it and goes on after it, if there is one, the partial sums are added up in
+// the shares' order by the warp, or by the block's warps together (each every
+// eighth share, then the warps in order) where there are over 32. blockIdx.y: 32
+// pieces of the columns.
+constexpr uint32_t kLongRun = 32;
 template <class O, int VE>
 __global__ void __launch_bounds__(kThreads)
     join_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ present, uint32_t share_size,
                 float scale, uint32_t dim, O* __restrict__ out, int64_t out_stride, bool accumulate,
                 const float* __restrict__ head, const float* __restrict__ tail) {
   constexpr int U = 8;
-  __shared__ uint32_t long_share[kJoinShares], long_last[kJoinShares], long_count;
+  __shared__ uint32_t long_share[kWarps], long_last[kWarps];
   __shared__ float part[kWarps][32 * VE];
   const uint32_t n = *present, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t first = blockIdx.x * kJoinShares;
-  if (uint64_t(first + 1) * share_size >= n) return;
-  if (threadIdx.x == 0) long_count = 0;
-  __syncthreads();
-  // Lane i < 8 looks at the warp's share i.
-  uint32_t last = 0, token = kNone;
-  const uint32_t mine = first + warp * 8 + lane;
-  if (lane < 8 && uint64_t(mine + 1) * share_size < n) {
-    const uint32_t begin = mine * share_size, end = begin + share_size;
+  const uint32_t share = blockIdx.x * kWarps + warp, c = (blockIdx.y * 32 + lane) * VE;
+  if (uint64_t(blockIdx.x * kWarps + 1) * share_size >= n) return;  // no share of the block goes on
+  uint32_t last = share, token = kNone;  // the share that the token's last entry is in
+  if (uint64_t(share + 1) * share_size < n) {
+    const uint32_t begin = share * share_size, end = begin + share_size;
     token = keys[end];
-    if (keys[end - 1] != token || (begin && keys[begin] == token && keys[begin - 1] == token)) {
-      token = kNone;
+    const bool begun = keys[end - 1] == token;
+    const bool earlier = begin && keys[begin] == token && keys[begin - 1] == token;
+    if (begun && !earlier) {
+      // The next shares that begin with the token, 32 at a look.
+      uint32_t same;
+      do {
+        const uint64_t at = uint64_t(last + 1 + lane) * share_size;
+        same = __ballot_sync(0xffffffffu, at < n && keys[at] == token);
+        last += same == ~0u ? 32 : __ffs(~same) - 1;
+      } while (same == ~0u);
     } else {
-      last = mine + 1;  // the share that its last entry is in
-      uint32_t tries = 0;
-      while (tries++ < 8 && uint64_t(last + 1) * share_size < n && keys[(last + 1) * share_size] == token) ++last;
-      if (tries > 8) {
-        uint32_t lo = last * share_size, hi = n;
-        while (lo < hi) {
-          const uint32_t mid = lo + (hi - lo) / 2;
-          if (keys[mid] == token) lo = mid + 1;
-          else hi = mid;
-        }
-        last = (lo - 1) / share_size;
-      }
+      token = kNone;
     }
   }
-  for (uint32_t i = 0; i < 8; ++i) {
-    const uint32_t t = __shfl_sync(0xffffffffu, token, i), to = __shfl_sync(0xffffffffu, last, i);
-    const uint32_t share = first + warp * 8 + i;
-    if (t == kNone) continue;
-    if (to - share > kLongRun) {
-      if (lane == 0) {
-        const uint32_t at = atomicAdd(&long_count, 1u);
-        long_share[at] = share;
-        long_last[at] = to;
-      }
-      continue;
-    }
-    const uint32_t c = (blockIdx.y * 32 + lane) * VE;
-    if (c < dim) {
-      const auto begun = load<float, VE>(tail + uint64_t(share) * dim + c);
-      float acc[VE];
+  const bool is_long = last - share > kLongRun;
+  if (lane == 0) {
+    long_share[warp] = is_long ? share : kNone;
+    long_last[warp] = last;
+  }
+  const auto add = [&](float(&acc)[VE], const float* from) {
+    const auto v = load<float, VE>(from);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) acc[e] = begun.v[e];
+    for (int e = 0; e < VE; ++e) acc[e] += v.v[e];
+  };
+  if (token != kNone && !is_long && c < dim) {
+    float acc[VE] = {};
+    add(acc, tail + uint64_t(share) * dim + c);
 #pragma unroll 8
-      for (uint32_t q = share + 1; q <= to; ++q) {
-        const auto v = load<float, VE>(head + uint64_t(q) * dim + c);
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] += v.v[e];
-      }
-      write_row<O, VE>(out + int64_t(t) * out_stride + c, acc, scale, accumulate);
-    }
+    for (uint32_t q = share + 1; q <= last; ++q) add(acc, head + uint64_t(q) * dim + c);
+    write_row<O, VE>(out + int64_t(token) * out_stride + c, acc, scale, accumulate);
   }
   __syncthreads();
-  for (uint32_t i = 0; i < long_count; ++i) {
-    const uint32_t share = long_share[i], to = long_last[i], t = keys[uint64_t(share + 1) * share_size];
-    const uint32_t c = (blockIdx.y * 32 + lane) * VE;
+  for (int i = 0; i < kWarps; ++i) {
+    const uint32_t from = long_share[i], to = long_last[i];
+    if (from == kNone) continue;
     float acc[VE] = {};
     if (c < dim) {
-      if (warp == 0) {
-        const auto begun = load<float, VE>(tail + uint64_t(share) * dim + c);
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] = begun.v[e];
-      }
-      for (uint32_t q = share + 1 + warp; q <= to; q += kWarps * U) {
+      if (warp == 0) add(acc, tail + uint64_t(from) * dim + c);
+      for (uint32_t q = from + 1 + warp; q <= to; q += kWarps * U) {
         Pack<float, VE> v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -631,7 +674,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int w = 1; w < kWarps; ++w)
 #pragma unroll
         for (int e = 0; e < VE; ++e) acc[e] += part[w][lane * VE + e];
-      write_row<O, VE>(out + int64_t(t) * out_stride + c, acc, scale, accumulate);
+      write_row<O, VE>(out + int64_t(keys[uint64_t(from + 1) * share_size]) * out_stride + c, acc, scale, accumulate);
     }
     __syncthreads();
   }
@@ -922,7 +965,11 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
           const size_t shared = size_t(kOneThreads) * ITEMS * 6 + kOneThreads / 32 * kDigits * 6;
           if (shared > 40 * 1024)
             XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)));
-          kernel<<<1, kOneThreads, shared, stream>>>(src, n, passes, present, u32(at.keys[0]), u32(at.values[0]));
+          const size_t e = type_size(out.type);
+          const Rows rows{static_cast<char*>(const_cast<void*>(out.data)), out.stride * int64_t(e), uint32_t(dim * e),
+                          uint32_t(e), bulk_rows(out, vocab, dim)};
+          kernel<<<accumulate ? 1 : unsigned(1 + std::min<uint64_t>(147, vocab)), kOneThreads, shared, stream>>>(
+              src, n, passes, present, u32(at.keys[0]), u32(at.values[0]), rows);
         };
         if (n <= kOneThreads * 4) go(std::integral_constant<int, 4>());
         else if (n <= kOneThreads * 12) go(std::integral_constant<int, 12>());
@@ -979,14 +1026,14 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
       const uint32_t* present = u32(at.totals) + kDigits;
       float* head = reinterpret_cast<float*>(w + at.head);
       float* tail = reinterpret_cast<float*>(w + at.tail);
-      const uint32_t zero_blocks = accumulate ? 0 : blocks_for(vocab, kThreads);
+      const uint32_t zero_blocks = accumulate || n <= kOneTokens ? 0 : blocks_for(vocab, kThreads);
       const auto kernel = s.data ? share_sum_kernel<T, O, VE, true> : share_sum_kernel<T, O, VE, false>;
       kernel<<<dim3(zero_blocks + blocks_for(plan.shares, kThreads >> plan.lg), plan.tiles), kThreads, 0, stream>>>(
           g, grad.stride, u32(at.keys[sorted]), u32(at.values[sorted]), present, plan.share, uint32_t(vocab), per_row,
           s, scale, uint32_t(dim), y, out.stride, accumulate, head, tail, plan.lg, zero_blocks, bulk);
       constexpr int JOIN = VE >= 4 ? 4 : VE;
       if (plan.shares > 1)
-        join_kernel<O, JOIN><<<dim3(blocks_for(plan.shares, kJoinShares), blocks_for(dim, 32 * JOIN)), kThreads, 0,
+        join_kernel<O, JOIN><<<dim3(blocks_for(plan.shares, kWarps), blocks_for(dim, 32 * JOIN)), kThreads, 0,
                                stream>>>(
             u32(at.keys[sorted]), present, plan.share, scale, uint32_t(dim), y, out.stride, accumulate, head, tail);
     });
