@@ -693,73 +693,61 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Few tokens, in one launch: block (x, y) owns the table's rows [x span, x span
-// + span) in a tile of columns. It picks its rows' tokens out of all n, sorts
-// them, (row << kShift | position), in shared memory, zeroes the rows that have
-// none, and sums the others: groups of 2^lg lanes take equal shares of the
-// sorted list, and what crosses shares is joined through shared memory, in the
-// shares' order. No row is written by two blocks. step: the distance of one
-// token from the next where it is the same for all, else 0.
+// + span) in a tile of columns. It picks its rows' tokens out of all n, in their
+// order, sorts them by row in shared memory, zeroes the rows that have none, and
+// sums the others: groups of 2^lg lanes take equal shares of the sorted list,
+// and what crosses shares is joined through shared memory, in the shares' order.
+// No row is written by two blocks. An entry is row << kShift | position.
 constexpr int kFewThreads = 512;
-constexpr int kShift = 15;
-constexpr uint32_t kFewTokens = 4096;
+constexpr int kFewWarps = kFewThreads / 32;
+constexpr int kShift = 13;
+constexpr uint32_t kFewTokens = 1u << kShift;
+constexpr int kFewTurns = kFewTokens / kFewThreads;  // entries a lane sorts
+constexpr uint32_t kFewCounts = kFewWarps * kDigits * 4;
 
 template <class T, class O, int VE, bool SCALED>
 __global__ void __launch_bounds__(kFewThreads, 2)
-    few_kernel(const T* __restrict__ grad, int64_t grad_stride, Tokens k, int64_t step, FastDiv per_row, uint32_t n,
-               uint32_t vocab, uint32_t span, Scales s, float scale, uint32_t dim, O* __restrict__ out,
-               int64_t out_stride, bool accumulate, bool bulk, int lg) {
+    few_kernel(const T* __restrict__ grad, int64_t grad_stride, Source src, uint32_t n, uint32_t span, Scales s,
+               float scale, uint32_t dim, O* __restrict__ out, int64_t out_stride, bool accumulate, bool bulk, int lg) {
   constexpr int U = 4, kBatch = 8;
   extern __shared__ __align__(16) uint32_t space[];
-  __shared__ uint32_t total;
+  __shared__ uint32_t warp_sums[kFewWarps];
   __shared__ int32_t first_row[kFewThreads], last_row[kFewThreads];  // of a group's share; -1: none
-  float* head = reinterpret_cast<float*>(space);  // [2][threads][VE]: sums that came in, sums that go on
-  float* tail = head + kFewThreads * VE;
-  uint32_t* zeros = space + 2 * kFewThreads * VE;  // what absent rows are copied from
-  uint32_t* present = zeros + (bulk ? kZeroBytes / 4 : 0);  // a bit a row
+  // While sorting, counts and masks; then sums that came in and sums that go on, [threads][VE] each.
+  uint32_t* const counts = space;
+  uint32_t* const masks = space + kFewCounts / 4;
+  float* const head = reinterpret_cast<float*>(space);
+  float* const tail = head + kFewThreads * VE;
+  uint32_t* const zeros = space + max(2 * kFewThreads * VE, int(2 * kFewCounts / 4));
+  uint32_t* const present = zeros + (bulk ? kZeroBytes / 4 : 0);  // a bit a row
   uint32_t* list = present + (span + 31) / 32;
-  const uint32_t lane = threadIdx.x & 31;
-  const uint32_t row0 = blockIdx.x * span, rows_here = min(span, vocab - row0);
+  const uint32_t turns = (n + kFewThreads - 1) / kFewThreads, per = turns * 32;
+  uint32_t* other = list + kFewWarps * per;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t row0 = blockIdx.x * span, rows_here = min(span, src.vocab - row0);
 
-  // The rows' tokens, in any order: all entries differ, so the sort gives one.
+  // Warp w looks at the tokens [w per, w per + per) and keeps its rows' there.
   for (uint32_t i = threadIdx.x; i < (span + 31) / 32; i += kFewThreads) present[i] = 0;
   if (bulk)
     for (uint32_t i = threadIdx.x; i < kZeroBytes / 4; i += kFewThreads) zeros[i] = 0;
   bulk_fence();
-  if (threadIdx.x == 0) total = 0;
   __syncthreads();
-  const auto where = [&](uint32_t i) {
-    if (step) return int64_t(i) * step;
-    const uint32_t r = per_row.div(i);
-    return int64_t(r) * k.stride_row + int64_t(i - r * per_row.d) * k.stride_col;
-  };
-  for (uint32_t i0 = threadIdx.x - lane; i0 < n; i0 += kFewThreads * kBatch) {
-    uint64_t local[kBatch];  // past rows_here: another block's token, or nobody's
-    if (k.type == kI64) {
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const uint32_t at = i0 + i * kFewThreads + lane;
-        local[i] = at < n ? uint64_t(static_cast<const int64_t*>(k.data)[where(at)]) : ~0ull;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const uint32_t at = i0 + i * kFewThreads + lane;
-        local[i] = at < n ? uint64_t(int64_t(static_cast<const int32_t*>(k.data)[where(at)])) : ~0ull;
-      }
-    }
+  uint32_t own = 0;
+  const uint32_t from = warp * per, to = min(n, from + per);
+  for (uint32_t i0 = from; i0 < to; i0 += 32 * kBatch) {
+    uint32_t key[kBatch];
+    if (src.k.type == kI64) src.load_keys<kTokens64, kBatch, 32>(i0 + lane, to, key);
+    else src.load_keys<kTokens32, kBatch, 32>(i0 + lane, to, key);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const bool mine = local[i] - row0 < rows_here;
+      const uint32_t r = key[i] - row0;
+      const bool mine = r < rows_here;  // kNone - row0 is past any row
       const uint32_t votes = __ballot_sync(0xffffffffu, mine);
-      if (!votes) continue;
-      uint32_t base = 0;
-      if (lane == 0) base = atomicAdd(&total, uint32_t(__popc(votes)));
-      base = __shfl_sync(0xffffffffu, base, 0);
       if (mine) {
-        const uint32_t r = uint32_t(local[i] - row0);
-        list[base + __popc(votes & ((1u << lane) - 1))] = r << kShift | (i0 + i * kFewThreads + lane);
+        list[from + own + __popc(votes & ((1u << lane) - 1))] = r << kShift | (i0 + i * 32 + lane);
         atomicOr(&present[r >> 5], 1u << (r & 31));
       }
+      own += __popc(votes);
     }
   }
   __syncthreads();
@@ -775,8 +763,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     const uint32_t last = uint32_t(uint64_t(rows_here) * (blockIdx.y + 1) / gridDim.y);
     for (uint32_t r = uint32_t(uint64_t(rows_here) * blockIdx.y / gridDim.y) + threadIdx.x; r < last; r += kFewThreads)
       if (!(present[r >> 5] >> (r & 31) & 1)) {
-        char* to = reinterpret_cast<char*>(out + int64_t(row0 + r) * out_stride);
-        for (uint32_t at = 0; at < row_bytes; at += kZeroBytes) bulk_store(to + at, zeros, min(kZeroBytes, row_bytes - at));
+        char* row = reinterpret_cast<char*>(out + int64_t(row0 + r) * out_stride);
+        for (uint32_t at = 0; at < row_bytes; at += kZeroBytes) bulk_store(row + at, zeros, min(kZeroBytes, row_bytes - at));
       }
   } else if (!accumulate && col < dim) {
     const float zero[VE] = {};
@@ -784,81 +772,93 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       if (!(present[r >> 5] >> (r & 31) & 1)) store_global<O, VE>(mine_out + int64_t(r) * out_stride, zero);
   }
 
-  // By counting the smaller entries where they are few, else a bitonic network
-  // whose comparators all point upwards (then what lies past the end need not
-  // exist). A warp's comparators of a span of 64 or less touch its own 64
-  // entries alone.
-  const uint32_t count = total;
-  if (count <= kFewThreads) {
-    uint32_t mine = 0, rank = 0;
+  // In the order of rows and, within a row, of positions.
+  if (lane == 0) warp_sums[warp] = own;
+  __syncthreads();
+  uint32_t count = 0, earlier = 0;
+#pragma unroll
+  for (int w = 0; w < kFewWarps; ++w) {
+    if (w < int(warp)) earlier += warp_sums[w];
+    count += warp_sums[w];
+  }
+  const bool by_counting = count <= kFewThreads / 2;
+  if (by_counting) {  // few entries: each one's place is the number of smaller ones
+    for (uint32_t i = lane; i < own; i += 32) other[earlier + i] = list[from + i];
+    __syncthreads();
     if (threadIdx.x < count) {
-      mine = list[threadIdx.x];
+      const uint32_t mine = other[threadIdx.x];
+      uint32_t place = 0;
 #pragma unroll 8
-      for (uint32_t j = 0; j < count; ++j) rank += list[j] < mine;
-    }
-    __syncthreads();
-    if (threadIdx.x < count) list[rank] = mine;
-    __syncthreads();
-  } else {
-    int bits = 32 - __clz(count - 1);
-    const uint32_t pairs = 1u << (bits - 1);
-    const auto order = [&](uint32_t i, uint32_t j) {
-      if (j < count) {
-        const uint32_t a = list[i], b = list[j];
-        if (a > b) {
-          list[i] = b;
-          list[j] = a;
-        }
-      }
-    };
-    for (int block = 1; block <= bits; ++block) {  // runs of 2^block entries
-      for (uint32_t p = threadIdx.x; p < pairs; p += kFewThreads) {
-        const uint32_t i = p >> (block - 1) << block | (p & ((1u << (block - 1)) - 1));
-        order(i, i ^ ((1u << block) - 1));
-      }
-      for (int half = block - 2; half >= 0; --half) {
-        if (half >= 5) __syncthreads();
-        else __syncwarp();
-        for (uint32_t p = threadIdx.x; p < pairs; p += kFewThreads) {
-          const uint32_t i = p >> half << (half + 1) | (p & ((1u << half) - 1));
-          order(i, i + (1u << half));
-        }
-      }
-      if (block >= 6) __syncthreads();
-      else __syncwarp();
+      for (uint32_t j = 0; j < count; ++j) place += other[j] < mine;
+      list[place] = mine;
     }
     __syncthreads();
   }
+  // Else stably by the row's digits, the first pass out of each warp's own part.
+  uint32_t begin_here = from, end_here = from + own;
+  for (int shift = kShift; !by_counting && (shift == kShift || (rows_here - 1) >> (shift - kShift)); shift += 8) {
+    uint32_t* const my_counts = counts + warp * kDigits;
+    for (uint32_t i = threadIdx.x; i < kFewCounts / 4; i += kFewThreads) counts[i] = masks[i] = 0;
+    if (shift > kShift) {
+      const uint32_t each = (count + kFewThreads - 1) / kFewThreads * 32;
+      begin_here = min(count, warp * each);
+      end_here = min(count, begin_here + each);
+    }
+    __syncthreads();
+    uint32_t entry[kFewTurns], rank[kFewTurns];
+#pragma unroll
+    for (int i = 0; i < kFewTurns; ++i)
+      if (begin_here + i * 32 < end_here) {
+        const bool in = begin_here + i * 32 + lane < end_here;
+        entry[i] = in ? list[begin_here + i * 32 + lane] : 0;
+        rank[i] = next_rank((entry[i] >> shift) & (kDigits - 1), in, masks + warp * kDigits, my_counts);
+      }
+    __syncthreads();
+    const uint32_t digit = threadIdx.x >> 1, w0 = (threadIdx.x & 1) * 8;
+    uint32_t c[8], eight = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      c[w] = counts[(w0 + w) * kDigits + digit];
+      eight += c[w];
+    }
+    uint32_t place = block_scan<kFewWarps>(eight, warp_sums, count);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      counts[(w0 + w) * kDigits + digit] = place;
+      place += c[w];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kFewTurns; ++i)
+      if (begin_here + i * 32 + lane < end_here)
+        other[my_counts[(entry[i] >> shift) & (kDigits - 1)] + rank[i]] = entry[i];
+    __syncthreads();
+    uint32_t* const sorted = other;
+    other = list;
+    list = sorted;
+  }
 
   const auto write = [&](int32_t local, const float(&sum)[VE]) {
-    if (col >= dim) return;
-    O* to = mine_out + int64_t(local) * out_stride;
-    float y[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) y[e] = sum[e] * scale;
-    if (accumulate) {
-      const auto old = load<O, VE>(to);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) y[e] += old.f(e);
-    }
-    store_global<O, VE>(to, y);
+    if (col < dim) write_row<O, VE>(mine_out + int64_t(local) * out_stride, sum, scale, accumulate);
   };
-
   const uint32_t share = (count + groups - 1) / groups;
   const uint32_t begin = min(count, group * share), end = min(count, begin + share);
   const int32_t before = begin && begin < end ? int32_t(list[begin - 1] >> kShift) : -1;
   const int32_t after = begin < end && end < count ? int32_t(list[end] >> kShift) : -1;
-  float acc[VE] = {};
+  Sum<T, VE> acc;
+  acc.clear();
+  float sum[VE];
   int32_t current = -1;
   bool from_before = false;
+  const T* const columns = grad + min(col, dim - VE);
   for (uint32_t j = begin; j < end; j += U) {
     Pack<T, VE> v[U];
     float f[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t at = list[min(j + u, end - 1)] & ((1u << kShift) - 1), r = per_row.div(at);
-      if (SCALED) f[u] = s.data[int64_t(r) * s.stride_row + int64_t(at - r * per_row.d) * s.stride_col];
-      if (col < dim) v[u] = load<T, VE>(grad + int64_t(r) * grad_stride + col);
+      const uint32_t at = list[min(j + u, end - 1)] & (kFewTokens - 1), r = src.per_row.div(at);
+      if (SCALED) f[u] = s.data[int64_t(r) * s.stride_row + int64_t(at - r * src.per_row.d) * s.stride_col];
+      v[u] = load<T, VE>(columns + int64_t(r) * grad_stride);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -866,24 +866,24 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         const int32_t local = int32_t(list[j + u] >> kShift);
         if (local != current) {
           if (current >= 0) {
-            if (from_before) store<float, VE>(head + threadIdx.x * VE, acc);
-            else write(current, acc);
+            acc.get(sum);
+            if (from_before) store<float, VE>(head + threadIdx.x * VE, sum);
+            else write(current, sum);
           }
-#pragma unroll
-          for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
+          acc.clear();
           current = local;
           from_before = j + u == begin && local == before;
         }
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] = SCALED ? fmaf(f[u], v[u].f(e), acc[e]) : acc[e] + v[u].f(e);
+        acc.template add<SCALED>(v[u], SCALED ? f[u] : 1.0f);
       }
     }
   }
+  acc.get(sum);
   const bool goes_on = current >= 0 && current == after;
   if (current >= 0) {
-    if (from_before) store<float, VE>(head + threadIdx.x * VE, acc);
-    else if (goes_on) store<float, VE>(tail + threadIdx.x * VE, acc);
-    else write(current, acc);
+    if (from_before) store<float, VE>(head + threadIdx.x * VE, sum);
+    else if (goes_on) store<float, VE>(tail + threadIdx.x * VE, sum);
+    else write(current, sum);
   }
   if (me == 0) {
     first_row[group] = begin < end ? int32_t(list[begin] >> kShift) : -1;
@@ -895,10 +895,10 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     for (uint32_t g = group + 1; g < groups && first_row[g] == current; ++g) {
       const auto more = load<float, VE>(head + ((g << lg) + me) * VE);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) acc[e] += more.v[e];
+      for (int e = 0; e < VE; ++e) sum[e] += more.v[e];
       if (last_row[g] != current) break;
     }
-    write(current, acc);
+    write(current, sum);
   }
   if (bulk) bulk_wait_all();
 }
@@ -919,9 +919,10 @@ struct FewPlan {
     tiles = blocks_for(pieces, 1u << lg);
     // About two blocks an SM: each reads all tokens.
     const uint64_t ranges = std::max<uint64_t>(1, 296 / tiles);
-    span = uint32_t(std::min<uint64_t>(std::max<uint64_t>((vocab + ranges - 1) / ranges, 1), 1u << (32 - kShift)));
+    span = uint32_t(std::min<uint64_t>(std::max<uint64_t>((vocab + ranges - 1) / ranges, 1), 1u << 16));
     blocks = blocks_for(vocab, span);
-    shared = size_t(2) * kFewThreads * ve * 4 + (bulk ? kZeroBytes : 0) + (span + 31) / 32 * 4 + size_t(n) * 4;
+    shared = std::max<size_t>(2 * kFewThreads * ve * 4, 2 * kFewCounts) + (bulk ? kZeroBytes : 0) +
+             (span + 31) / 32 * 4 + size_t(2) * 4 * ((n + kFewThreads - 1) / kFewThreads * kFewThreads);
   }
 };
 
@@ -948,8 +949,8 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
   char* w = static_cast<char*>(workspace);
   const auto u32 = [&](size_t offset) { return reinterpret_cast<uint32_t*>(w + offset); };
   int sorted = 0;
+  Source src{k, per_row, token_step(k), uint32_t(vocab), s.data == nullptr, nullptr, nullptr};
   if (n > kFewTokens) {
-    Source src{k, per_row, token_step(k), uint32_t(vocab), s.data == nullptr, nullptr, nullptr};
     uint32_t* present = u32(at.totals) + kDigits;
     int passes = 1;
     while (passes < 4 && (vocab - 1) >> (8 * passes)) ++passes;
@@ -1018,8 +1019,7 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
         if (plan.shared > 40 * 1024)
           XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan.shared)));
         kernel<<<dim3(plan.blocks, plan.tiles), kFewThreads, plan.shared, stream>>>(
-            g, grad.stride, k, token_step(k), per_row, n, uint32_t(vocab), plan.span, s, scale, uint32_t(dim), y,
-            out.stride, accumulate, bulk, plan.lg);
+            g, grad.stride, src, n, plan.span, s, scale, uint32_t(dim), y, out.stride, accumulate, bulk, plan.lg);
         return;
       }
       const SharePlan plan(n, pieces);
