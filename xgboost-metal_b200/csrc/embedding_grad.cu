@@ -18,8 +18,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kItems = 16;                  // entries a thread holds of a sort tile
-constexpr int kTile = kThreads * kItems;    // 4096
 constexpr int kDigits = 256;
 constexpr int kSortBlocks = 592;            // most blocks of a sort pass: 4 an SM
 constexpr int kOneThreads = 1024;           // of the sort in one block
@@ -27,14 +25,17 @@ constexpr uint32_t kOneTokens = kOneThreads * 24;  // what its registers hold
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr uint32_t kZeroBytes = 8192;              // zeros that wide rows are copied from
 
+// Entries a thread holds of a sort tile: few, so that short lists fill the card,
+// else as many as leave a block long runs of equal digits to write.
+int sort_items(uint64_t n) { return n <= uint64_t(kSortBlocks) * kThreads * 4 ? 4 : 16; }
 uint32_t sort_blocks(uint64_t n) {
-  const uint64_t tiles = (n + kTile - 1) / kTile;
+  const uint64_t tile = kThreads * sort_items(n), tiles = (n + tile - 1) / tile;
   return uint32_t(tiles < kSortBlocks ? tiles : kSortBlocks);
 }
 
 // How the sorted list is shared out: 2^lg lanes move a row's columns, or a tile
 // of them, and sum `share` entries. Long lists give each of the 1024 threads that
-// an SM holds one share, short ones 32 entries a share.
+// an SM holds one share, short ones 8 entries a share.
 struct SharePlan {
   int lg = 0;
   uint32_t tiles, share, shares;
@@ -42,7 +43,7 @@ struct SharePlan {
     while (lg < 5 && (1ull << lg) < pieces) ++lg;
     tiles = blocks_for(pieces, 1u << lg);
     const uint64_t even = ((n << lg) * tiles + 148 * 1024 - 1) / (148 * 1024);
-    share = uint32_t(std::min<uint64_t>(std::max<uint64_t>(32, (even + 7) / 8 * 8), 4096));
+    share = uint32_t(std::min<uint64_t>(std::max<uint64_t>(8, (even + 7) / 8 * 8), 4096));
     shares = blocks_for(n, share);
   }
 };
@@ -176,7 +177,7 @@ __device__ __forceinline__ uint32_t next_rank(uint32_t digit, bool in, uint32_t*
   return rank;
 }
 
-// Block b sorts the tiles [b * per, (b + 1) * per). hist[digit][block].
+// Block b sorts the entries [b * per, (b + 1) * per). hist[digit][block].
 template <int READ>
 __global__ void __launch_bounds__(kThreads)
     sort_hist_kernel(Source src, const uint32_t* __restrict__ present, uint32_t n, uint32_t per, int shift,
@@ -186,8 +187,7 @@ __global__ void __launch_bounds__(kThreads)
   count[threadIdx.x] = 0;
   __syncthreads();
   if (READ == kSorted) n = *present;
-  const uint64_t begin = uint64_t(blockIdx.x) * per * kTile;
-  const uint64_t end = min(uint64_t(n), begin + uint64_t(per) * kTile);
+  const uint64_t begin = uint64_t(blockIdx.x) * per, end = min(uint64_t(n), begin + per);
   for (uint64_t i = begin + threadIdx.x; i < end; i += kThreads * U) {
     uint32_t key[U];
     src.load_keys<READ, U, kThreads>(i, end, key);
@@ -217,20 +217,21 @@ __global__ void __launch_bounds__(kThreads)
   if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
-// Ranks a tile's entries by digit, stably: warp w holds entries [512 w, 512
-// w + 512) of it, 32 at a time, and counts its own digits. The tile is put in
+// Ranks a tile's entries by digit, stably: each warp holds an equal part of it,
+// 32 entries at a time, and counts its own digits. The tile is put in
 // order in shared memory and leaves it in runs of equal digits, while the next
 // tile's keys are on their way. The first pass tells how many entries are
 // present.
-template <int READ>
+template <int READ, int kItems>
 __global__ void __launch_bounds__(kThreads, 4)
     sort_scatter_kernel(Source src, uint32_t* __restrict__ present, uint32_t n, uint32_t per, int shift,
                         const uint32_t* __restrict__ hist, const uint32_t* __restrict__ totals,
                         uint32_t* __restrict__ keys_out, uint32_t* __restrict__ values_out) {
+  constexpr int kTile = kThreads * kItems;
   __shared__ uint32_t to[kDigits];            // where the digit's entries go, less their place in the ordered tile
   __shared__ uint32_t count[kWarps][kDigits];  // the warp's entries of the digit, then where they begin in the tile
   __shared__ uint32_t warp_sums[kWarps];
-  __shared__ uint32_t keys[kTile], values[kTile];
+  __shared__ uint32_t keys[kTile < kWarps * kDigits ? kWarps * kDigits : kTile], values[kTile];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = threadIdx.x;
   if (READ == kSorted) n = *present;
   uint32_t all;
@@ -238,8 +239,8 @@ __global__ void __launch_bounds__(kThreads, 4)
   if (READ != kSorted && blockIdx.x == 0 && d == 0) *present = all;
   uint32_t* const masks = keys;  // [warps][digits], while the tile is ranked
   const uint32_t mine = warp * (kItems * 32) + lane;
-  uint64_t begin = uint64_t(blockIdx.x) * per * kTile;
-  const uint64_t end = min(uint64_t(n), begin + uint64_t(per) * kTile);
+  uint64_t begin = uint64_t(blockIdx.x) * per;
+  const uint64_t end = min(uint64_t(n), begin + per);
   uint32_t key[kItems], rank[kItems];
   src.load_keys<READ, kItems, 32>(begin + mine, end, key);
   for (; begin < end; begin += kTile) {
@@ -712,7 +713,6 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   constexpr int U = 4, kBatch = 8;
   extern __shared__ __align__(16) uint32_t space[];
   __shared__ uint32_t warp_sums[kFewWarps];
-  __shared__ int32_t first_row[kFewThreads], last_row[kFewThreads];  // of a group's share; -1: none
   // While sorting, counts and masks; then sums that came in and sums that go on, [threads][VE] each.
   uint32_t* const counts = space;
   uint32_t* const masks = space + kFewCounts / 4;
@@ -841,7 +841,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const auto write = [&](int32_t local, const float(&sum)[VE]) {
     if (col < dim) write_row<O, VE>(mine_out + int64_t(local) * out_stride, sum, scale, accumulate);
   };
-  const uint32_t share = (count + groups - 1) / groups;
+  const uint32_t share = max((count + groups - 1) / groups, uint32_t(U));
   const uint32_t begin = min(count, group * share), end = min(count, begin + share);
   const int32_t before = begin && begin < end ? int32_t(list[begin - 1] >> kShift) : -1;
   const int32_t after = begin < end && end < count ? int32_t(list[end] >> kShift) : -1;
@@ -885,18 +885,21 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     else if (goes_on) store<float, VE>(tail + threadIdx.x * VE, sum);
     else write(current, sum);
   }
-  if (me == 0) {
-    first_row[group] = begin < end ? int32_t(list[begin] >> kShift) : -1;
-    last_row[group] = goes_on ? current : -1;
-  }
   __syncthreads();
   // The group in whose share a row began joins it.
   if (goes_on && !from_before) {
-    for (uint32_t g = group + 1; g < groups && first_row[g] == current; ++g) {
+    uint32_t lo = end, hi = count;  // the first entry of a later row
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (int32_t(list[mid] >> kShift) == current) lo = mid + 1;
+      else hi = mid;
+    }
+    const uint32_t last = (lo - 1) / share;
+#pragma unroll 8
+    for (uint32_t g = group + 1; g <= last; ++g) {
       const auto more = load<float, VE>(head + ((g << lg) + me) * VE);
 #pragma unroll
       for (int e = 0; e < VE; ++e) sum[e] += more.v[e];
-      if (last_row[g] != current) break;
     }
     write(current, sum);
   }
@@ -950,6 +953,9 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
   const auto u32 = [&](size_t offset) { return reinterpret_cast<uint32_t*>(w + offset); };
   int sorted = 0;
   Source src{k, per_row, token_step(k), uint32_t(vocab), s.data == nullptr, nullptr, nullptr};
+  // One block sorts where the others have rows to zero meanwhile, for longer than
+  // it takes.
+  const bool beside = n <= kOneTokens && !accumulate && vocab * dim * type_size(out.type) >= 128u << 20;
   if (n > kFewTokens) {
     uint32_t* present = u32(at.totals) + kDigits;
     int passes = 1;
@@ -958,7 +964,7 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
       if (k.type == kI64) f(std::integral_constant<int, kTokens64>());
       else f(std::integral_constant<int, kTokens32>());
     };
-    if (n <= kOneTokens) {
+    if (beside) {
       first_read([&](auto read) {
         const auto go = [&](auto items) {
           constexpr int ITEMS = decltype(items)::value;
@@ -969,25 +975,24 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
           const size_t e = type_size(out.type);
           const Rows rows{static_cast<char*>(const_cast<void*>(out.data)), out.stride * int64_t(e), uint32_t(dim * e),
                           uint32_t(e), bulk_rows(out, vocab, dim)};
-          kernel<<<accumulate ? 1 : unsigned(1 + std::min<uint64_t>(147, vocab)), kOneThreads, shared, stream>>>(
+          kernel<<<unsigned(1 + std::min<uint64_t>(147, vocab)), kOneThreads, shared, stream>>>(
               src, n, passes, present, u32(at.keys[0]), u32(at.values[0]), rows);
         };
-        if (n <= kOneThreads * 4) go(std::integral_constant<int, 4>());
-        else if (n <= kOneThreads * 12) go(std::integral_constant<int, 12>());
+        if (n <= kOneThreads * 12) go(std::integral_constant<int, 12>());
         else go(std::integral_constant<int, 24>());
       });
     } else {
-      const uint32_t blocks = sort_blocks(n), tiles = blocks_for(n, kTile), per = (tiles + blocks - 1) / blocks;
-      const uint32_t grid = (tiles + per - 1) / per;
+      const uint32_t tile = kThreads * sort_items(n), blocks = sort_blocks(n);
+      const uint32_t per = blocks_for(blocks_for(n, tile), blocks) * tile, grid = blocks_for(n, per);
       for (int pass = 0; pass < passes; ++pass) {
         const auto go = [&](auto read) {
           constexpr int READ = decltype(read)::value;
           const int to = pass ? sorted ^ 1 : 0;
           sort_hist_kernel<READ><<<grid, kThreads, 0, stream>>>(src, present, n, per, pass * 8, u32(at.hist));
           sort_scan_kernel<<<kDigits, kThreads, 0, stream>>>(u32(at.hist), grid, u32(at.totals));
-          sort_scatter_kernel<READ><<<grid, kThreads, 0, stream>>>(src, present, n, per, pass * 8, u32(at.hist),
-                                                                   u32(at.totals), u32(at.keys[to]),
-                                                                   u32(at.values[to]));
+          const auto scatter = tile == kThreads * 4 ? sort_scatter_kernel<READ, 4> : sort_scatter_kernel<READ, 16>;
+          scatter<<<grid, kThreads, 0, stream>>>(src, present, n, per, pass * 8, u32(at.hist), u32(at.totals),
+                                                 u32(at.keys[to]), u32(at.values[to]));
           sorted = to;
         };
         if (pass) go(std::integral_constant<int, kSorted>());
@@ -1026,7 +1031,7 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
       const uint32_t* present = u32(at.totals) + kDigits;
       float* head = reinterpret_cast<float*>(w + at.head);
       float* tail = reinterpret_cast<float*>(w + at.tail);
-      const uint32_t zero_blocks = accumulate || n <= kOneTokens ? 0 : blocks_for(vocab, kThreads);
+      const uint32_t zero_blocks = accumulate || beside ? 0 : blocks_for(vocab, kThreads);
       const auto kernel = s.data ? share_sum_kernel<T, O, VE, true> : share_sum_kernel<T, O, VE, false>;
       kernel<<<dim3(zero_blocks + blocks_for(plan.shares, kThreads >> plan.lg), plan.tiles), kThreads, 0, stream>>>(
           g, grad.stride, u32(at.keys[sorted]), u32(at.values[sorted]), present, plan.share, uint32_t(vocab), per_row,
