@@ -7,6 +7,10 @@
 // A token below 0 is missing and adds nothing, whatever its scale holds. A
 // token past the table makes its row's result NaN: nothing is read for it.
 // Sums are float32 in a fixed order, and are rounded once, when written.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "nn_device.cuh"
 
 namespace xgbb::nn {
@@ -58,27 +62,31 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // A bag a row: 2^lg lanes own a row's columns (or a tile of them), VE values
-// each; S = 2^ls such groups share a row's tokens, a contiguous span each, and
-// add their sums up in shared memory, first span first. A group reads its
-// tokens K to a lane, a step ahead, and hands them round by shuffles, eight
-// gathers in flight.
-template <class T, class O, int VE, int K, bool SCALED>
+// each. SPLIT: S = 2^ls such groups share a row's tokens, a contiguous span each,
+// and add their sums up in shared memory, first span first; and the blocks of a
+// cluster, where there are several, share the tokens in the same way. A group
+// reads its tokens K to a lane, a step ahead, and hands them round by shuffles,
+// eight gathers in flight.
+template <class T, class O, int VE, int K, bool SCALED, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, (Sum<T, VE>::kPairs && K == 1 ? 4 : 2))
     bag_kernel(Tokens k, const T* __restrict__ table, int64_t table_stride, uint32_t vocab, uint32_t dim,
                float scale, Scales s, O* __restrict__ out, int64_t out_stride, int lg, int ls, float nan) {
   constexpr int U = 8;
-  __shared__ float part[kThreads * VE];
+  __shared__ float part[SPLIT ? kThreads * VE : 1];
+  const auto cluster = cooperative_groups::this_cluster();
+  const uint32_t blocks = SPLIT ? cluster.num_blocks() : 1, rank = SPLIT ? cluster.block_rank() : 0;
   const uint32_t G = 1u << lg, lane = threadIdx.x & (G - 1), group = threadIdx.x >> lg;
+  if (!SPLIT) ls = 0;
   const uint32_t S = 1u << ls, span = group & (S - 1);
-  const uint64_t row = uint64_t(blockIdx.x) * (kThreads >> (lg + ls)) + (group >> ls);
+  const uint64_t row = uint64_t(blockIdx.x / blocks) * (kThreads >> (lg + ls)) + (group >> ls);
   const uint32_t col = (blockIdx.y * G + lane) * VE;
   const bool wide = k.type == kI64;
-  const uint32_t count = uint32_t(k.per_row), per = (count + S - 1) >> ls;
-  const uint32_t begin = min(count, per * span), end = row < k.rows ? min(count, begin + per) : 0;
+  const uint32_t count = uint32_t(k.per_row), per = (count + S * blocks - 1) / (S * blocks);
+  const uint32_t begin = uint32_t(min(uint64_t(count), uint64_t(per) * (rank * S + span))), end = row < k.rows ? min(count, begin + per) : 0;
   // Lanes past the last column read the last piece, and write nothing.
   const T* const columns = table + min(col, dim - VE);
   const char* const tokens = static_cast<const char*>(k.data) + int64_t(row) * k.stride_row * (wide ? 8 : 4);
-  const float* const scales = SCALED ? s.data + int64_t(row) * s.stride_row : nullptr;
+  const float* const scales = SCALED && (!SPLIT || s.data) ? s.data + int64_t(row) * s.stride_row : nullptr;
   Sum<T, VE> acc;
   acc.clear();
   bool bad = false;
@@ -92,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, (Sum<T, VE>::kPairs && K == 1 ? 4 : 
       if (t < end) w = load_token(tokens, wide, int64_t(t) * k.stride_col);
       next[i] = uint64_t(w) < vocab ? int(w) : -1;
       bad |= w >= int64_t(vocab);
-      if (SCALED) next_f[i] = next[i] >= 0 ? scales[int64_t(t) * s.stride_col] : 0.0f;
+      if (SCALED) next_f[i] = SPLIT && !scales ? 1.0f : next[i] >= 0 ? scales[int64_t(t) * s.stride_col] : 0.0f;
     }
   };
   fetch(begin);
@@ -139,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, (Sum<T, VE>::kPairs && K == 1 ? 4 : 
   if (bad)
 #pragma unroll
     for (int e = 0; e < VE; ++e) sum[e] = nan;
-  if (S > 1) {
+  if (SPLIT && S > 1) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) part[threadIdx.x * VE + e] = sum[e];
     __syncthreads();
@@ -148,6 +156,20 @@ __global__ void __launch_bounds__(kThreads, (Sum<T, VE>::kPairs && K == 1 ? 4 : 
 #pragma unroll
         for (int e = 0; e < VE; ++e) sum[e] += part[(threadIdx.x + (q << lg)) * VE + e];
   }
+  if (SPLIT && blocks > 1) {
+    if (span == 0)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) part[threadIdx.x * VE + e] = sum[e];
+    cluster.sync();
+    if (rank == 0 && span == 0)
+      for (uint32_t q = 1; q < blocks; ++q) {
+        const float* other = cluster.map_shared_rank(part, q);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) sum[e] += other[threadIdx.x * VE + e];
+      }
+    cluster.sync();  // the other blocks' memory is read until here
+    if (rank) return;
+  }
   if (span == 0 && row < k.rows && col < dim) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) sum[e] *= scale;
@@ -155,30 +177,76 @@ __global__ void __launch_bounds__(kThreads, (Sum<T, VE>::kPairs && K == 1 ? 4 : 
   }
 }
 
-// The scales' gradient: 32 lanes a row, which hold the row's gradient in
-// pieces and walk the row's tokens.
+// The scales' gradient: 2^lg lanes own a row's columns, VE values each in as many
+// tiles as it takes, and take a span of the row's tokens, eight at a time. The
+// eight products are reduced together: each shuffle halves how many a lane holds,
+// until the lanes hold different tokens' results.
 template <class T, class O, int VE>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
     scale_grad_kernel(const O* __restrict__ grad, int64_t grad_stride, Tokens k, const T* __restrict__ table,
-                      int64_t table_stride, uint64_t vocab, uint32_t dim, float scale, float* __restrict__ out,
-                      uint64_t total, float nan) {
-  const uint64_t i = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-  if (i >= total) return;
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t row = i / k.per_row, t = i - row * k.per_row;
-  const int64_t w =
-      load_token(k.data, k.type == kI64, int64_t(row) * k.stride_row + int64_t(t) * k.stride_col);
-  float acc = 0.0f;
-  if (w >= 0 && w < int64_t(vocab)) {
-    for (uint32_t c = lane * VE; c < dim; c += 32 * VE) {
-      const auto a = load<T, VE>(table + w * table_stride + c);
-      const auto b = load<O, VE>(grad + int64_t(row) * grad_stride + c);
+                      int64_t table_stride, uint32_t vocab, uint32_t dim, float scale, float* __restrict__ out,
+                      uint32_t span, FastDiv spans, uint64_t groups, int lg, float nan) {
+  constexpr int U = 8;
+  const uint32_t G = 1u << lg, lane = threadIdx.x & (G - 1);
+  const uint64_t group = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) >> lg;
+  const bool here = group < groups;
+  const uint32_t row = here ? spans.div(uint32_t(group)) : 0;
+  const uint32_t begin = here ? (uint32_t(group) - row * spans.d) * span : 0;
+  const uint32_t end = here ? uint32_t(min(k.per_row, uint64_t(begin) + span)) : 0;
+  const bool wide = k.type == kI64;
+  const char* const tokens = static_cast<const char*>(k.data) + int64_t(row) * k.stride_row * (wide ? 8 : 4);
+  const O* const g_row = grad + int64_t(row) * grad_stride;
+  for (uint32_t t0 = begin; __any_sync(0xffffffffu, t0 < end); t0 += U) {
+    int token[U];  // -1: missing, past the table, or past the span
+    if (wide) {
 #pragma unroll
-      for (int e = 0; e < VE; ++e) acc = fmaf(a.f(e), b.f(e), acc);
+      for (int u = 0; u < U; ++u) {
+        const int64_t w =
+            t0 + u < end ? reinterpret_cast<const int64_t*>(tokens)[int64_t(t0 + u) * k.stride_col] : -1;
+        token[u] = uint64_t(w) < vocab ? int(w) : -1;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int w = t0 + u < end ? reinterpret_cast<const int*>(tokens)[int64_t(t0 + u) * k.stride_col] : -1;
+        token[u] = uint32_t(w) < vocab ? w : -1;
+      }
+    }
+    float dot[U] = {};
+    for (uint32_t c = lane * VE; c < dim; c += G * VE) {
+      const auto g = load<O, VE>(g_row + c);
+      Pack<T, VE> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (token[u] >= 0) v[u] = load<T, VE>(table + token[u] * table_stride + c);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (token[u] >= 0)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) dot[u] = fmaf(g.f(e), v[u].f(e), dot[u]);
+    }
+    uint32_t m = G >> 1;
+#pragma unroll
+    for (int n = U / 2; n >= 1; n >>= 1)
+      if (m) {
+        const bool upper = lane & m;
+#pragma unroll
+        for (int i = 0; i < n; ++i)
+          dot[i] = (upper ? dot[i + n] : dot[i]) + __shfl_xor_sync(0xffffffffu, upper ? dot[i] : dot[i + n], m);
+        m >>= 1;
+      }
+    for (; m; m >>= 1) dot[0] += __shfl_xor_sync(0xffffffffu, dot[0], m);
+    // Lane l holds tokens l (8 / G) on, or token l / (G / 8).
+    const uint32_t first = lg < 3 ? lane << (3 - lg) : lane >> (lg - 3);
+    if (lg > 3 && (lane & ((1u << (lg - 3)) - 1))) continue;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (i >= (lg < 3 ? 8 >> lg : 1) || t0 + first + i >= end) break;
+      const uint64_t at = uint64_t(row) * k.per_row + t0 + first + i;
+      const int64_t w = load_token(tokens, wide, (t0 + first + i) * k.stride_col);
+      out[at] = w < int64_t(vocab) ? dot[i] * scale : nan;
     }
   }
-  for (int m = 16; m; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
-  if (lane == 0) out[i] = w < int64_t(vocab) ? acc * scale : nan;
 }
 
 }  // namespace
@@ -208,12 +276,24 @@ void embedding(const Tokens& k, const Mat& table, uint64_t vocab, uint64_t dim, 
       // of the block, down to 8 tokens a group.
       int ls = 0;
       while (lg + ls < 8 && k.rows * tiles << (lg + ls) < 148 * 1024 && k.per_row >> (ls + 1) >= 8) ++ls;
-      const dim3 grid(blocks_for(k.rows, kThreads >> (lg + ls)), tiles);
+      // And over a cluster, where a group still has over 64.
+      const unsigned cluster = ls && k.per_row >> ls > 64 ? 8 : 1;
+      const dim3 grid(blocks_for(k.rows, kThreads >> (lg + ls)) * cluster, tiles);
       const auto go = [&](auto kk) {
         constexpr int K = decltype(kk)::value;
-        const auto kernel = s.data ? bag_kernel<T, O, VE, K, true> : bag_kernel<T, O, VE, K, false>;
-        kernel<<<grid, kThreads, 0, stream>>>(k, w, table.stride, uint32_t(vocab), uint32_t(dim), scale, s, y,
-                                              out.stride, lg, ls, kNaN);
+        const auto kernel = ls ? bag_kernel<T, O, VE, K, true, true>
+                               : s.data ? bag_kernel<T, O, VE, K, true, false> : bag_kernel<T, O, VE, K, false, false>;
+        cudaLaunchAttribute attribute{};
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim = {cluster, 1, 1};
+        cudaLaunchConfig_t config{};
+        config.gridDim = grid;
+        config.blockDim = dim3(kThreads);
+        config.stream = stream;
+        config.attrs = &attribute;
+        config.numAttrs = cluster > 1;
+        XGBB_CUDA(cudaLaunchKernelEx(&config, kernel, k, w, table.stride, uint32_t(vocab), uint32_t(dim), scale, s, y,
+                                     out.stride, lg, ls, kNaN));
       };
       if (lg >= 3) go(std::integral_constant<int, 1>());
       else if (lg == 2) go(std::integral_constant<int, 2>());
@@ -232,9 +312,16 @@ void embedding_scale_backward(const Mat& grad, const Tokens& k, const Mat& table
     using T = std::remove_pointer_t<decltype(pt)>;
     using O = std::remove_pointer_t<decltype(po)>;
     with_width<T>(table, vocab, grad, k.rows, dim, [&](auto width) {
-      scale_grad_kernel<T, O, decltype(width)::value><<<blocks_for(total, kThreads / 32), kThreads, 0, stream>>>(
-          static_cast<const O*>(grad.data), grad.stride, k, static_cast<const T*>(table.data), table.stride, vocab,
-          uint32_t(dim), scale, out, total, kNaN);
+      constexpr int VE = decltype(width)::value;
+      int lg = 0;
+      while (lg < 5 && (VE << lg) < int(std::min<uint64_t>(dim, 1024))) ++lg;
+      // A span of eight tokens where that is what fills the card, longer ones where there are more.
+      uint64_t span = ((total << lg) / (148 * 1024) + 7) / 8 * 8;
+      span = std::min<uint64_t>(std::max<uint64_t>(span, 8), (k.per_row + 7) / 8 * 8);
+      const uint64_t spans = (k.per_row + span - 1) / span, groups = k.rows * spans;
+      scale_grad_kernel<T, O, VE><<<blocks_for(groups, kThreads >> lg), kThreads, 0, stream>>>(
+          static_cast<const O*>(grad.data), grad.stride, k, static_cast<const T*>(table.data), table.stride,
+          uint32_t(vocab), uint32_t(dim), scale, out, uint32_t(span), FastDiv(uint32_t(spans)), groups, lg, kNaN);
     });
   });
   XGBB_CUDA(cudaGetLastError());
