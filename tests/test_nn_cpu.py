@@ -108,8 +108,8 @@ REFUSED = [
     (lambda: nn.layer_norm_backward(F((3, 4)), F((3, 4)), F((3,)), F((3,)), out=F((3, 4))), "neither"),
     (lambda: nn.layer_norm_backward(F((3, 4)), F((3, 4)), F((3,)), F((3,)), out=F((3, 4), ptr=8192),
                                     dweight=F((4,))), "need weight"),
-    (lambda: nn.layer_norm_backward(F((3, 4)), F((3, 4)), F((3,)), F((3,)), F((4,)), out=F((3, 4), ptr=8192),
-                                    dweight=F((4,)), dbias=F((4,))), "workspace must be given"),
+    (lambda: nn.layer_norm_backward(F((3, 400)), F((3, 400)), F((3,)), F((3,)), F((400,)), out=F((3, 400), ptr=8192),
+                                    dweight=F((400,)), dbias=F((400,))), "workspace must be given"),
 ]
 
 

@@ -214,7 +214,7 @@ def test_layer_norm_and_its_gradient(shape, types):
 
 # Rows enough that blocks take many each, of 64 lanes' values or fewer, of whole and of partly filled blocks.
 @pytest.mark.parametrize("rows,dim,a,p", [
-    (5000, 64, F32, F32), (3001, 200, F32, F32), (1203, 1024, F32, F32), (2500, 3, F32, F32), (700, 2048, F32, F32),
+    (5000, 64, F32, F32), (3001, 200, F32, F32), (300, 64, BF16, F32), (2000, 40, F32, F32), (16000, 8, F16, F16), (1203, 1024, F32, F32), (2500, 3, F32, F32), (700, 2048, F32, F32),
     (601, 777, F32, F32), (9001, 512, BF16, F32), (5003, 1000, F16, F16), (2501, 2048, BF16, BF16),
     (2500, 1996, F32, F32), (2401, 4096, F32, F32), (2400, 3080, F16, F32), (2399, 4096, BF16, F32),
     (2403, 8192, BF16, F32), (2402, 8000, F32, F32), (2370, 16384, BF16, BF16), (2369, 16000, F16, F32),

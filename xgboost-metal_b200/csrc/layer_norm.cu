@@ -5,6 +5,8 @@
 //
 // All arithmetic is float32; the variance is the mean square of the centred
 // values, never a difference of two large sums. Results are rounded once.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <initializer_list>
 
@@ -323,13 +325,14 @@ __global__ void __launch_bounds__(1024)
 // of dy h and dy kept in registers from the first row to the last. The next
 // row's values are under way while this one's are summed (packed 16-bit values,
 // whose registers leave room). WARP: 2^lg lanes hold a row, else the block does.
-// parts[block][2][dim] gets the block's sums.
-template <class T, class P, int VE, int CH, bool WARP>
+// parts[block][2][dim] gets the block's sums; ONE: the grid is one cluster, whose
+// blocks add theirs up through each other's shared memory, block 0's first.
+template <class T, class P, int VE, int CH, bool WARP, bool ONE = false>
 __global__ void __launch_bounds__(WARP ? kThreads : 1024, WARP ? 4 : 1)
     norm_grad_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x, int64_t x_stride,
                      const float* __restrict__ mean, const float* __restrict__ rstd, uint64_t rows, uint32_t dim,
                      const P* __restrict__ w, T* __restrict__ dx, int64_t dx_stride, float* __restrict__ parts,
-                     int lg) {
+                     int lg, P* __restrict__ dweight, P* __restrict__ dbias) {
   constexpr bool kAhead = sizeof(T) == 2 && VE == 8;
   constexpr int E = CH * VE;
   __shared__ float part[2][32][2];
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024, WARP ? 4 : 1)
       store<T, VE>(dx + int64_t(row) * dx_stride + c, r);
     }
   }
-  if (!parts) return;
+  if (!parts && !ONE) return;
   float* out = parts + uint64_t(blockIdx.x) * 2 * dim;
   if constexpr (WARP) {
     // The groups' sums: over the warp's lanes, then over the warps in order.
@@ -424,7 +427,21 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024, WARP ? 4 : 1)
       float s = 0.0f;
 #pragma unroll
       for (int q = 0; q < kThreads / 32; ++q) s += sums[q * 2 * width + i];
-      if (c < dim) out[which * dim + c] = s;
+      if (ONE) sums[i] = s;  // the thread's own, and read by no other yet
+      else if (c < dim) out[which * dim + c] = s;
+    }
+    if (ONE) {
+      const auto cluster = cooperative_groups::this_cluster();
+      const uint32_t blocks = cluster.num_blocks();
+      cluster.sync();
+      for (uint32_t i = cluster.block_rank() * kThreads + threadIdx.x; i < 2 * width; i += blocks * kThreads) {
+        const uint32_t which = i / width, c = i % width;
+        float s = 0.0f;
+        for (uint32_t q = 0; q < blocks; ++q) s += cluster.map_shared_rank(sums, q)[i];
+        P* to = which ? dbias : dweight;
+        if (to && c < dim) to[c] = from_f32<P>(s);
+      }
+      cluster.sync();  // the blocks' memory is read until here
     }
   } else {
 #pragma unroll
@@ -764,14 +781,14 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// The parts' sums: 32 columns a block (of dw's and db's 2 dim), each warp
-// every eighth part, then the warps in order.
+// The parts' sums: 32 columns a block (of dw's and db's 2 dim), each warp every
+// 32nd part, then the warps in order.
 template <class P>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(1024)
     norm_parts_kernel(const float* __restrict__ parts, uint32_t count, uint32_t dim, P* __restrict__ dw,
                       P* __restrict__ db) {
-  constexpr int kWarps = kThreads / 32, U = 8;
-  __shared__ float sums[kWarps][32];
+  constexpr int kWarps = 32, U = 4;
+  __shared__ float sums[kWarps][33];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (c < 2 * dim)
@@ -784,11 +801,13 @@ __global__ void __launch_bounds__(kThreads)
     }
   sums[warp][lane] = s;
   __syncthreads();
-  if (warp || c >= 2 * dim) return;
+  s = sums[lane][warp];  // warp w adds up column w
 #pragma unroll
-  for (int q = 1; q < kWarps; ++q) s += sums[q][lane];
-  P* to = c < dim ? dw : db;
-  if (to) to[c < dim ? c : c - dim] = from_f32<P>(s);
+  for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+  const uint32_t mine = blockIdx.x * 32 + warp;
+  if (lane || mine >= 2 * dim) return;
+  P* to = mine < dim ? dw : db;
+  if (to) to[mine < dim ? mine : mine - dim] = from_f32<P>(s);
 }
 
 bool param_aligned(const void* p, size_t size, uint64_t n) {
@@ -823,7 +842,7 @@ void launch_ring(void (*kernel)(Params...), unsigned blocks, unsigned threads, s
 // How norm_grad_kernel takes rows of `dim` values: lanes or threads a row,
 // blocks, and rows that its registers hold.
 struct GradPlan {
-  bool fits, warp;
+  bool fits, warp, one = false, ring = false;  // ring: rows enough to stream, if they come in 16-byte pieces
   int lg = 0;
   uint32_t threads = 0, blocks = 0;
   GradPlan(uint64_t rows, uint64_t dim) : fits(dim <= 8192), warp(dim <= 256) {
@@ -834,11 +853,22 @@ struct GradPlan {
     if (warp) {
       while ((8ull << lg) < dim) ++lg;
       threads = kThreads;
+      // Up to eight turns of eight blocks: one cluster, and one launch.
+      const uint64_t once = kThreads >> lg;
+      if (rows <= once * 64) {
+        one = true;
+        blocks = 1;
+        while (blocks < 8 && blocks * once < rows) blocks *= 2;
+        return;
+      }
       blocks = uint32_t(std::min<uint64_t>(148 * 4, (rows + (kThreads >> lg) - 1) / (kThreads >> lg)));
       return;
     }
     threads = uint32_t((dim + 255) / 256 * 32);
-    blocks = uint32_t(std::min<uint64_t>(148 * (1024 / threads), rows));
+    const uint32_t full = 148 * (1024 / threads);
+    ring = rows >= 4ull * full;
+    // Four rows a block at least: the blocks' parts are read again.
+    blocks = uint32_t(std::min<uint64_t>(full, (rows + 3) / 4));
   }
 };
 
@@ -906,7 +936,8 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
 }
 
 size_t layer_norm_backward_workspace(uint64_t rows, uint64_t dim) {
-  return size_t(GradPlan(rows, dim).blocks) * 2 * dim * 4;
+  const GradPlan plan(rows, dim);
+  return plan.one ? 0 : size_t(plan.blocks) * 2 * dim * 4;
 }
 
 void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const float* rstd, uint64_t rows,
@@ -923,23 +954,39 @@ void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const
     const T* v = static_cast<const T*>(x.data);
     const P* w = static_cast<const P*>(weight);
     T* out = static_cast<T*>(const_cast<void*>(dx.data));
-    if (rows)
+    P *dw = static_cast<P*>(dweight), *db = static_cast<P*>(dbias);
+    if (rows || plan.one)
       with_norm_width<T>({grad, x, dx}, {}, param_type, rows, dim, [&](auto width) {
         constexpr int VE = decltype(width)::value;
-        if (plan.fits && plan.warp) {
+        const size_t sums = (kThreads / 32) * 2 * (size_t(8) << plan.lg) * 4;
+        if (plan.one) {
+          cudaLaunchAttribute attribute{};
+          attribute.id = cudaLaunchAttributeClusterDimension;
+          attribute.val.clusterDim = {plan.blocks, 1, 1};
+          cudaLaunchConfig_t config{};
+          config.gridDim = dim3(plan.blocks);
+          config.blockDim = dim3(kThreads);
+          config.dynamicSmemBytes = sums;
+          config.stream = stream;
+          config.attrs = &attribute;
+          config.numAttrs = 1;
+          XGBB_CUDA(cudaLaunchKernelEx(&config, norm_grad_kernel<T, P, VE, 8 / VE, true, true>, g, grad.stride, v,
+                                       x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride,
+                                       static_cast<float*>(nullptr), plan.lg, dw, db));
+        } else if (plan.fits && plan.warp) {
           norm_grad_kernel<T, P, VE, 8 / VE, true>
-              <<<plan.blocks, plan.threads, (kThreads / 32) * 2 * (8u << plan.lg) * 4, stream>>>(
-                  g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts, plan.lg);
-        } else if (plan.fits && VE * sizeof(T) == 16 && rows >= plan.blocks * 4ull) {
+              <<<plan.blocks, plan.threads, sums, stream>>>(g, grad.stride, v, x.stride, mean, rstd, rows,
+                                                            uint32_t(dim), w, out, dx.stride, parts, plan.lg, nullptr,
+                                                            nullptr);
+        } else if (plan.ring && VE * sizeof(T) == 16) {
           if constexpr (VE * sizeof(T) == 16) {
             const bool full = dim == plan.threads * 8ull;
             if (plan.threads <= 512) {
               constexpr int R = sizeof(T) == 2 ? 4 : 2;
-              launch_ring(full ? norm_grad_rows_kernel<T, P, R, true> : norm_grad_rows_kernel<T, P, R, false>,
-                          148 * (512 / plan.threads), plan.threads, size_t(2) * R * 2 * 8 * sizeof(T) * plan.threads,
-                          stream, g, grad.stride, v, x.stride, mean, rstd, uint32_t(rows), uint32_t(dim), w, out,
-                          dx.stride, parts);
-              used = 148 * (512 / plan.threads);
+              used = 148 * (512 / plan.threads);  // no more than the plan's blocks, which hold twice as many threads
+              launch_ring(full ? norm_grad_rows_kernel<T, P, R, true> : norm_grad_rows_kernel<T, P, R, false>, used,
+                          plan.threads, size_t(2) * R * 2 * 8 * sizeof(T) * plan.threads, stream, g, grad.stride, v,
+                          x.stride, mean, rstd, uint32_t(rows), uint32_t(dim), w, out, dx.stride, parts);
             } else {
               constexpr int S = sizeof(T) == 2 ? 4 : 3;
               launch_ring(full ? norm_grad_ring_kernel<T, P, S, true> : norm_grad_ring_kernel<T, P, S, false>,
@@ -949,7 +996,8 @@ void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const
           }
         } else if (plan.fits) {
           norm_grad_kernel<T, P, VE, 8 / VE, false><<<plan.blocks, plan.threads, 0, stream>>>(
-              g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts, 0);
+              g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts, 0, nullptr,
+              nullptr);
         } else {
           norm_grad_long_kernel<T, P, VE><<<unsigned(rows), 1024, 0, stream>>>(
               g, grad.stride, v, x.stride, mean, rstd, uint32_t(dim), w, out, dx.stride);
@@ -958,9 +1006,9 @@ void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const
                 g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), parts);
         }
       });
-    if (params)
-      norm_parts_kernel<P><<<blocks_for(2 * dim, 32), kThreads, 0, stream>>>(
-          parts, used, uint32_t(dim), static_cast<P*>(dweight), static_cast<P*>(dbias));
+    if (params && !plan.one)
+      norm_parts_kernel<P><<<blocks_for(2 * dim, 32), 1024, 0, stream>>>(
+          parts, used, uint32_t(dim), dw, db);
   });
   XGBB_CUDA(cudaGetLastError());
 }

@@ -21,6 +21,7 @@ inputs give equal bits. These functions have no counterpart in the reference.
 """
 import contextlib
 import ctypes
+import functools
 import json
 import struct
 import sys
@@ -157,7 +158,7 @@ def _scale_grid(scale, tokens, bag):
     the tokens' shape."""
     if scale is None:
         return 0, 0, 0, -1
-    if hasattr(scale, "expand"):
+    if hasattr(scale, "expand") and scale.shape != tokens[1]:
         try:
             scale = scale.expand(tokens[1])
         except RuntimeError as e:
@@ -173,9 +174,9 @@ def _scale_grid(scale, tokens, bag):
 
 
 def _one_device(*devices):
-    device = -1
+    device = devices[0]
     for d in devices:
-        if d >= 0 and d != device:
+        if d != device and d >= 0:
             if device >= 0:
                 raise XGBoostError("the arrays are on different devices")
             device = d
@@ -226,17 +227,29 @@ def _dtype_code(dtype):
         return 0
 
 
+def _new(shape, code, like, what):
+    """(tensor, pointer) of a new result of like's kind."""
+    tensor = like[5]
+    if tensor is None:
+        raise XGBoostError("%s must be given where the inputs are no tensors" % what)
+    if code not in _FLOATS:
+        raise XGBoostError("%s must be float32, float16 or bfloat16" % what)
+    # Sizes one by one are read faster than a tuple of them.
+    if not shape:
+        out = tensor.new_empty((), dtype=_dtypes[code])
+    elif code == like[3]:
+        out = tensor.new_empty(*shape)
+    else:
+        out = tensor.new_empty(*shape, dtype=_dtypes[code])
+    return out, out.data_ptr()
+
+
 def _result(out, shape, code, like, what):
     """(array, pointer, dtype code, row stride, device) of a result: `out`,
     checked, or a new one of like's kind. Any float type does where code is 0."""
     if out is None:
-        tensor = like[5]
-        if tensor is None:
-            raise XGBoostError("%s must be given where the inputs are no tensors" % what)
-        if code not in _FLOATS:
-            raise XGBoostError("%s must be float32, float16 or bfloat16" % what)
-        out = tensor.new_empty(shape) if code == like[3] else tensor.new_empty(shape, dtype=_dtypes[code])
-        return out, out.data_ptr(), code, shape[-1] if shape else 1, like[4]
+        out, ptr = _new(shape, code, like, what)
+        return out, ptr, code, shape[-1] if shape else 1, like[4]
     v = _view(out, what)
     if tuple(v[1]) != tuple(shape):
         raise XGBoostError("%s must have the shape %s" % (what, tuple(shape)))
@@ -246,43 +259,47 @@ def _result(out, shape, code, like, what):
 
 
 def _flat_result(out, shape, code, like, what):
-    """_result for contiguous values."""
-    got = _result(out, shape, code, like, what)
-    if out is not None:
-        v = _view(out, what)
-        n, stride = _flat(v[1], v[2], what)
-        if n > 1 and stride != 1:
-            raise XGBoostError("%s must be contiguous" % what)
-    return got
+    """(array, pointer, device) of a result of contiguous values."""
+    if out is None:
+        out, ptr = _new(shape, code, like, what)
+        return out, ptr, like[4]
+    v = _view(out, what)
+    if tuple(v[1]) != tuple(shape):
+        raise XGBoostError("%s must have the shape %s" % (what, tuple(shape)))
+    if v[3] != code:
+        raise XGBoostError("%s has another type than it must have" % what)
+    n, stride = _flat(v[1], v[2], what)
+    if n > 1 and stride != 1:
+        raise XGBoostError("%s must be contiguous" % what)
+    return out, v[0], v[4]
 
 
 def _vector(a, dim, code, what):
-    """(pointer, dtype code, device) of weight or bias."""
-    ptr, shape, strides, own, device, _ = _view(a, what)
-    if tuple(shape) != (dim,) or (dim > 1 and strides[0] != 1):
+    """The view of weight or bias."""
+    v = _view(a, what)
+    if len(v[1]) != 1 or v[1][0] != dim or (dim > 1 and v[2][0] != 1):
         raise XGBoostError("%s must be %d contiguous values" % (what, dim))
-    if own != code and own != _F32:
+    if v[3] != code and v[3] != _F32:
         raise XGBoostError("%s must be float32 or have x's type" % what)
-    return ptr, own, device
+    return v
 
 
 def _row_values(a, lead, what):
     """(pointer, device) of mean or rstd."""
     ptr, shape, strides, code, device, _ = _view(a, what)
-    if tuple(shape) != tuple(lead):
-        raise XGBoostError("%s must be contiguous, one value a row" % what)
-    n, stride = _flat(shape, strides, what)
-    if n > 1 and stride != 1:
-        raise XGBoostError("%s must be contiguous, one value a row" % what)
     if code != _F32:
         raise XGBoostError("%s must be float32" % what)
-    return ptr, device
+    if shape == lead:
+        if len(shape) == 1 and (strides[0] == 1 or shape[0] == 1):
+            return ptr, device
+        n, stride = _flat(shape, strides, what)
+        if n <= 1 or stride == 1:
+            return ptr, device
+    raise XGBoostError("%s must be contiguous, one value a row" % what)
 
 
 def _space(workspace, size, like):
     """(workspace, pointer) of `size` bytes."""
-    if not size:
-        return None, 0
     if workspace is None:
         if like[5] is None:
             raise XGBoostError("workspace must be given where the inputs are no tensors")
@@ -326,6 +343,7 @@ def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def embedding_backward_workspace(rows, per_row, vocab, dim):
     """Bytes of workspace that embedding_backward needs for `rows` bags of
     `per_row` tokens (1 without `bag`)."""
@@ -357,7 +375,9 @@ def embedding_backward(grad, tokens, vocab, *, scale=1.0, token_scale=None, bag=
     out, y, code, y_stride, y_device = _result(out, (vocab, dim), 0 if out is not None and out_dtype is None else code,
                                                g, "out")
     device = _one_device(g[4], k[4], s_device, y_device)
-    workspace, space = _space(workspace, size, g)
+    space = 0
+    if size:
+        workspace, space = _space(workspace, size, g)
     _call(_LIB.XGBBEmbeddingBackward, _pack_embedding_backward(
         k[0], s, rows, per_row, stride_row, stride_col, s_row, s_col, k[3], scale, g[0], y, space,
         _handle(stream, device, g), size, vocab, dim, g_stride, y_stride, g[3], code, bool(accumulate), device))
@@ -380,7 +400,7 @@ def embedding_scale_backward(grad, tokens, table, *, scale=1.0, bag=False, out=N
     _, g_dim, g_stride = _matrix(g, "grad")
     if g[1][:-1] != lead or g_dim != dim:
         raise XGBoostError("grad must have the shape of the lookup's result")
-    out, y, _, _, y_device = _flat_result(out, tuple(k[1]), _F32, g, "out")
+    out, y, y_device = _flat_result(out, k[1], _F32, g, "out")
     device = _one_device(g[4], k[4], w[4], y_device)
     _call(_LIB.XGBBEmbeddingScaleBackward, _pack_embedding_scale_backward(
         k[0], 0, rows, per_row, stride_row, stride_col, 0, 0, k[3], scale, g[0], w[0], y,
@@ -398,25 +418,31 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
             return layer_norm(x, weight, bias, eps=eps, out=out, mean=mean, rstd=rstd)
     v = _view(x, "x")
     rows, dim, stride = _matrix(v, "x")
-    w, w_code, w_device = (0, 0, -1) if weight is None else _vector(weight, dim, v[3], "weight")
-    b, b_code, b_device = (0, 0, -1) if bias is None else _vector(bias, dim, v[3], "bias")
-    if w_code and b_code and w_code != b_code:
-        raise XGBoostError("weight and bias must have the same type")
+    w = b = None
+    param, w_device, b_device = _F32, -1, -1
+    if weight is not None:
+        w, _, _, param, w_device, _ = _vector(weight, dim, v[3], "weight")
+    if bias is not None:
+        b, _, _, b_code, b_device, _ = _vector(bias, dim, v[3], "bias")
+        if weight is not None and param != b_code:
+            raise XGBoostError("weight and bias must have the same type")
+        param = b_code
     lead = v[1][:-1]
-    out, y, _, y_stride, y_device = _result(out, v[1], v[3], v, "out")
-    if mean is None and rstd is None and v[5] is not None:
-        mean, rstd = v[5].new_empty((2, *lead), dtype=_dtypes[_F32]).unbind()
-        m, q, m_device, q_device = mean.data_ptr(), rstd.data_ptr(), v[4], v[4]
+    if out is None and v[5] is not None and x.is_contiguous():
+        out = sys.modules["torch"].empty_like(x)
+        y, y_stride, y_device = out.data_ptr(), dim, v[4]
     else:
-        mean, m, _, _, m_device = _flat_result(mean, lead, _F32, v, "mean")
-        rstd, q, _, _, q_device = _flat_result(rstd, lead, _F32, v, "rstd")
+        out, y, _, y_stride, y_device = _result(out, v[1], v[3], v, "out")
+    mean, m, m_device = _flat_result(mean, lead, _F32, v, "mean")
+    rstd, q, q_device = _flat_result(rstd, lead, _F32, v, "rstd")
     device = _one_device(v[4], w_device, b_device, y_device, m_device, q_device)
     _call(_LIB.XGBBLayerNorm, _pack_layer_norm(
-        v[0], w, b, y, m, q, _handle(stream, device, v), rows, dim, stride, y_stride, v[3],
-        w_code or b_code or _F32, device, eps))
+        v[0], w or 0, b or 0, y, m, q, _handle(stream, device, v), rows, dim, stride, y_stride, v[3], param, device,
+        eps))
     return out, mean, rstd
 
 
+@functools.lru_cache(maxsize=1024)
 def layer_norm_backward_workspace(rows, dim):
     """Bytes of workspace that layer_norm_backward needs for the gradients of
     weight and bias."""
@@ -442,16 +468,22 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
     lead = v[1][:-1]
     m, m_device = _row_values(mean, lead, "mean")
     q, q_device = _row_values(rstd, lead, "rstd")
-    out, dx, _, dx_stride, dx_device = _result(out, v[1], v[3], v, "out")
+    if out is None and v[5] is not None and x.is_contiguous():
+        out = sys.modules["torch"].empty_like(x)
+        dx, dx_stride, dx_device = out.data_ptr(), dim, v[4]
+    else:
+        out, dx, _, dx_stride, dx_device = _result(out, v[1], v[3], v, "out")
     w = dw = db = space = size = 0
     w_code, w_device, dw_device, db_device = _F32, -1, -1, -1
     if weight is not None:
-        w, w_code, w_device = _vector(weight, dim, v[3], "weight")
-        dweight, dw, _, _, dw_device = _flat_result(dweight, (dim,), w_code, v, "dweight")
+        wv = _vector(weight, dim, v[3], "weight")
+        w, _, _, w_code, w_device, _ = wv
+        dweight, dw, dw_device = _flat_result(dweight, (dim,), w_code, wv, "dweight")
         if bias_grad:
-            dbias, db, _, _, db_device = _flat_result(dbias, (dim,), w_code, v, "dbias")
+            dbias, db, db_device = _flat_result(dbias, (dim,), w_code, wv, "dbias")
         size = layer_norm_backward_workspace(rows, dim)
-        workspace, space = _space(workspace, size, v)
+        if size:
+            workspace, space = _space(workspace, size, v)
     elif dweight is not None or dbias is not None:
         raise XGBoostError("dweight and dbias need weight")
     device = _one_device(v[4], g[4], m_device, q_device, w_device, dx_device, dw_device, db_device)
