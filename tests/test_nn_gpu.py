@@ -218,7 +218,8 @@ def test_layer_norm_and_its_gradient(shape, types):
     (601, 777, F32, F32), (9001, 512, BF16, F32), (5003, 1000, F16, F16), (2501, 2048, BF16, BF16),
     (2500, 1996, F32, F32), (2401, 4096, F32, F32), (2400, 3080, F16, F32), (2399, 4096, BF16, F32),
     (2403, 8192, BF16, F32), (2402, 8000, F32, F32), (2370, 16384, BF16, BF16), (2369, 16000, F16, F32),
-    (300, 9001, F32, F32)])
+    (300, 9001, F32, F32), (300, 20000, BF16, F32), (260, 32768, F32, F32), (2000, 1001, BF16, BF16),
+    (500, 5001, F16, F32), (3000, 33, BF16, F32)])
 def test_many_rows(rows, dim, a, p):
     g = _gen(7, rows, dim)
     x = (torch.randn(rows, dim, generator=g) * 2 + 30 * torch.randn(rows, 1, generator=g)).to(a).to(DEV)

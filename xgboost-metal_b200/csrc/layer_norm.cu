@@ -327,13 +327,13 @@ __global__ void __launch_bounds__(1024)
 // whose registers leave room). WARP: 2^lg lanes hold a row, else the block does.
 // parts[block][2][dim] gets the block's sums; ONE: the grid is one cluster, whose
 // blocks add theirs up through each other's shared memory, block 0's first.
-template <class T, class P, int VE, int CH, bool WARP, bool ONE = false>
-__global__ void __launch_bounds__(WARP ? kThreads : 1024, WARP ? 4 : 1)
+template <class T, class P, int VE, int CH, bool WARP, int MOST, bool ONE = false>
+__global__ void __launch_bounds__(MOST, WARP && VE * sizeof(T) == 16 ? 4 : 1)
     norm_grad_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x, int64_t x_stride,
                      const float* __restrict__ mean, const float* __restrict__ rstd, uint64_t rows, uint32_t dim,
                      const P* __restrict__ w, T* __restrict__ dx, int64_t dx_stride, float* __restrict__ parts,
                      int lg, P* __restrict__ dweight, P* __restrict__ dbias) {
-  constexpr bool kAhead = sizeof(T) == 2 && VE == 8;
+  constexpr bool kAhead = sizeof(T) == 2 && (VE == 8 || MOST < 1024);
   constexpr int E = CH * VE;
   __shared__ float part[2][32][2];
   const uint32_t G = WARP ? 1u << lg : blockDim.x;
@@ -457,126 +457,12 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024, WARP ? 4 : 1)
   }
 }
 
-// The same for many rows of 16-byte pieces, a block a row at a time, with the
-// next S - 1 rows under way into shared memory.
-template <class T, class P, int S, bool FULL>
-__global__ void __launch_bounds__(1024)
-    norm_grad_ring_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x,
-                          int64_t x_stride, const float* __restrict__ mean, const float* __restrict__ rstd,
-                          uint64_t rows, uint32_t dim, const P* __restrict__ w, T* __restrict__ dx,
-                          int64_t dx_stride, float* __restrict__ parts) {
-  constexpr int VE = 16 / sizeof(T), CH = 8 / VE, H = VE / 2;
-  extern __shared__ uint4 ring[];  // [S][2][CH][threads]
-  __shared__ float part[2][2][32];
-  const uint32_t G = blockDim.x, at = threadIdx.x, lane = at & 31, warp = at >> 5, warps = G >> 5;
-  const float inverse = 1.0f / float(dim);
-  float2 wv[CH][H], dw[CH][H] = {}, db[CH][H] = {};
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const uint32_t c = (at + i * G) * VE;
-#pragma unroll
-    for (int e = 0; e < H; ++e)
-      wv[i][e] = w && c < dim ? make_float2(to_f32(w[c + 2 * e]), to_f32(w[c + 2 * e + 1])) : both(1.0f);
-  }
-  const auto has = [&](int i) { return FULL || (at + i * G) * VE < dim; };
-  const uint32_t half = CH * G * 16, stage_bytes = 2 * half;
-  char* const own = reinterpret_cast<char*>(ring + at);
-  const auto fetch = [&](const T* xs, const T* gs, bool there, char* to) {
-    if (there)
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-        if (has(i)) {
-          copy_async16(to + i * G * 16, xs + i * G * VE);
-          copy_async16(to + half + i * G * 16, gs + i * G * VE);
-        }
-    copy_commit();
-  };
-  const uint32_t step = gridDim.x;
-  const int64_t x_step = int64_t(step) * x_stride, g_step = int64_t(step) * grad_stride;
-  const int64_t dx_step = int64_t(step) * dx_stride;
-  const T* xr = x + int64_t(blockIdx.x) * x_stride + at * VE;
-  const T* gr = grad + int64_t(blockIdx.x) * grad_stride + at * VE;
-  T* dxr = dx + int64_t(blockIdx.x) * dx_stride + at * VE;
-#pragma unroll
-  for (int i = 0; i < S - 1; ++i, xr += x_step, gr += g_step)
-    fetch(xr, gr, blockIdx.x + i * step < rows, own + i * stage_bytes);
-  char* read = own;
-  char* written = own + (S - 1) * stage_bytes;
-  float nm = blockIdx.x < rows ? mean[blockIdx.x] : 0.0f, nq = blockIdx.x < rows ? rstd[blockIdx.x] : 0.0f;
-  uint32_t turn = 0;
-  for (uint32_t row = blockIdx.x; row < rows; row += step, turn ^= 1, xr += x_step, gr += g_step, dxr += dx_step) {
-    fetch(xr, gr, row + (S - 1) * step < rows, written);
-    const float m = nm, q = nq;
-    if (row + step < rows) {
-      nm = mean[row + step];
-      nq = rstd[row + step];
-    }
-    copy_wait<S - 1>();
-    float2 h[CH][H], g[CH][H], sum_g = both(0.0f), sum_gh = both(0.0f);
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-      if (has(i)) {
-        float2 d[H];
-        unpack16<T>(*reinterpret_cast<const uint4*>(read + i * G * 16), h[i]);
-        unpack16<T>(*reinterpret_cast<const uint4*>(read + half + i * G * 16), d);
-#pragma unroll
-        for (int e = 0; e < H; ++e) {
-          h[i][e] = mul2(add2(h[i][e], both(-m)), both(q));
-          g[i][e] = mul2(d[e], wv[i][e]);
-          sum_g = add2(sum_g, g[i][e]);
-          sum_gh = fma2(g[i][e], h[i][e], sum_gh);
-          dw[i][e] = fma2(d[e], h[i][e], dw[i][e]);
-          db[i][e] = add2(db[i][e], d[e]);
-        }
-      }
-    written = read;
-    read = read == own + (S - 1) * stage_bytes ? own : read + stage_bytes;
-    // Two sums for the shuffles of one: lanes 0 to 15 end with the first,
-    // lanes 16 to 31 with the second.
-    const float s0 = sum_g.x + sum_g.y, s1 = sum_gh.x + sum_gh.y;
-    float s = lane < 16 ? s0 : s1;
-    s += __shfl_xor_sync(0xffffffffu, lane < 16 ? s1 : s0, 16);
-#pragma unroll
-    for (int k = 8; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    if ((lane & 15) == 0) part[turn][lane >> 4][warp] = s;
-    __syncthreads();
-    const uint32_t q0 = lane & 15;
-    s = q0 < warps ? part[turn][lane >> 4][q0] : 0.0f;
-    if (q0 + 16 < warps) s += part[turn][lane >> 4][q0 + 16];
-#pragma unroll
-    for (int k = 8; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    s *= -inverse * q;
-    // q (g - a - h b), with -q a and -q b.
-    const float2 a = both(__shfl_sync(0xffffffffu, s, 0)), b = both(__shfl_sync(0xffffffffu, s, 16));
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-      if (has(i)) {
-#pragma unroll
-        for (int e = 0; e < H; ++e) h[i][e] = fma2(h[i][e], b, fma2(g[i][e], both(q), a));
-        *reinterpret_cast<uint4*>(dxr + i * G * VE) = pack16<T>(h[i]);
-      }
-  }
-  if (!parts) return;
-  float* out = parts + uint64_t(blockIdx.x) * 2 * dim;
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const uint32_t c = (at + i * G) * VE;
-    if (c < dim)
-#pragma unroll
-      for (int e = 0; e < H; ++e) {
-        out[c + 2 * e] = dw[i][e].x;
-        out[c + 2 * e + 1] = dw[i][e].y;
-        out[dim + c + 2 * e] = db[i][e].x;
-        out[dim + c + 2 * e + 1] = db[i][e].y;
-      }
-  }
-}
-
-// The same for many rows of 16-byte pieces, a block of 512 threads at most R
-// rows at a time: the rows' 2 R sums are reduced together, each shuffle halving
-// how many of them a lane holds, and share their barrier. The next R rows are
-// under way into shared memory.
-template <class T, class P, int R, bool FULL>
+// The same for many rows of 16-byte pieces, a block of 512 threads at most, or a
+// cluster of C of them, R rows at a time: the rows' 2 R sums are reduced together,
+// each shuffle halving how many of them a lane holds, and share their barrier;
+// in a cluster each block leaves its warps' sums with all blocks. The next R
+// rows are under way into shared memory.
+template <class T, class P, int R, int C, bool FULL>
 __global__ void __launch_bounds__(512, 1)
     norm_grad_rows_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x,
                           int64_t x_stride, const float* __restrict__ mean, const float* __restrict__ rstd,
@@ -584,12 +470,20 @@ __global__ void __launch_bounds__(512, 1)
                           int64_t dx_stride, float* __restrict__ parts) {
   constexpr int VE = 16 / sizeof(T), CH = 8 / VE, H = VE / 2, V = 2 * R, L = 32 / V, W = 16 / L;
   extern __shared__ uint4 ring[];  // [2][R][2][CH][threads]
-  __shared__ __align__(16) float part[2][V][16];
-  const uint32_t G = blockDim.x, at = threadIdx.x, lane = at & 31, warp = at >> 5;
+  __shared__ __align__(16) float part[2][C][V][16];
+  const auto cluster = cooperative_groups::this_cluster();
+  const uint32_t rank = C > 1 ? cluster.block_rank() : 0, id = blockIdx.x / C;
+  const auto barrier = [&] {
+    if constexpr (C > 1) cluster.sync();
+    else __syncthreads();
+  };
+  // The block's columns begin at those of the blocks before it.
+  const uint32_t G = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t at = rank * G * CH + threadIdx.x;
   const float inverse = 1.0f / float(dim);
   const auto has = [&](int i) { return FULL || (at + i * G) * VE < dim; };
-  for (uint32_t i = at; i < 2 * V * 16; i += G) (&part[0][0][0])[i] = 0.0f;
-  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < 2 * C * V * 16; i += G) (&part[0][0][0][0])[i] = 0.0f;
+  barrier();
   float2 wv[CH][H], dw[CH][H] = {}, db[CH][H] = {};
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
@@ -599,7 +493,7 @@ __global__ void __launch_bounds__(512, 1)
       wv[i][e] = w && c < dim ? make_float2(to_f32(w[c + 2 * e]), to_f32(w[c + 2 * e + 1])) : both(1.0f);
   }
   const uint32_t half = CH * G * 16, row_bytes = 2 * half, stage_bytes = R * row_bytes;
-  char* const own = reinterpret_cast<char*>(ring + at);
+  char* const own = reinterpret_cast<char*>(ring + threadIdx.x);
   const auto fetch = [&](uint32_t row, char* to) {
     const T* xs = x + int64_t(row) * x_stride + at * VE;
     const T* gs = grad + int64_t(row) * grad_stride + at * VE;
@@ -614,7 +508,7 @@ __global__ void __launch_bounds__(512, 1)
           }
     copy_commit();
   };
-  const uint32_t step = gridDim.x * R;
+  const uint32_t step = gridDim.x / C * R;
   float nm[R], nq[R];
   const auto fetch_stats = [&](uint32_t row) {
 #pragma unroll
@@ -624,11 +518,11 @@ __global__ void __launch_bounds__(512, 1)
         nq[r] = rstd[row + r];
       }
   };
-  fetch(blockIdx.x * R, own);
-  fetch(blockIdx.x * R + step, own + stage_bytes);
-  fetch_stats(blockIdx.x * R);
+  fetch(id * R, own);
+  fetch(id * R + step, own + stage_bytes);
+  fetch_stats(id * R);
   uint32_t turn = 0;
-  for (uint32_t row = blockIdx.x * R; row < rows; row += step, turn ^= 1) {
+  for (uint32_t row = id * R; row < rows; row += step, turn ^= 1) {
     char* const stage = own + turn * stage_bytes;
     float q[R], val[V];
     float2 h[R][CH][H], g[R][CH][H];
@@ -662,12 +556,22 @@ __global__ void __launch_bounds__(512, 1)
     fetch(row + 2 * step, stage);  // the thread has read its values out
     fetch_stats(row + step);
     float s = warp_sums<V>(val, lane);  // of value lane / L
-    if ((lane & (L - 1)) == 0) part[turn][lane / L][warp] = s;
-    __syncthreads();
-    const auto others = load<float, W>(&part[turn][lane / L][(lane & (L - 1)) * W]);
-    s = others.v[0];
+    if ((lane & (L - 1)) == 0) {
+      if constexpr (C > 1) {
 #pragma unroll
-    for (int j = 1; j < W; ++j) s += others.v[j];
+        for (int q = 0; q < C; ++q) *cluster.map_shared_rank(&part[turn][rank][lane / L][warp], q) = s;
+      } else {
+        part[turn][0][lane / L][warp] = s;
+      }
+    }
+    barrier();
+    s = 0.0f;
+#pragma unroll
+    for (int q = 0; q < C; ++q) {
+      const auto others = load<float, W>(&part[turn][q][lane / L][(lane & (L - 1)) * W]);
+#pragma unroll
+      for (int j = 0; j < W; ++j) s += others.v[j];
+    }
 #pragma unroll
     for (int j = L / 2; j; j >>= 1) s += __shfl_xor_sync(0xffffffffu, s, j);
     s *= -inverse;
@@ -688,7 +592,7 @@ __global__ void __launch_bounds__(512, 1)
     }
   }
   if (!parts) return;
-  float* out = parts + uint64_t(blockIdx.x) * 2 * dim;
+  float* out = parts + uint64_t(id) * 2 * dim;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const uint32_t c = (at + i * G) * VE;
@@ -834,22 +738,41 @@ void with_norm_width(std::initializer_list<Mat> mats, std::initializer_list<cons
 template <class... Params, class... Args>
 void launch_ring(void (*kernel)(Params...), unsigned blocks, unsigned threads, size_t shared, cudaStream_t stream,
                  Args... args) {
-  if (shared > 46 * 1024)
+  if (shared > 40 * 1024)
     XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)));
   kernel<<<blocks, threads, shared, stream>>>(args...);
 }
 
-// How norm_grad_kernel takes rows of `dim` values: lanes or threads a row,
-// blocks, and rows that its registers hold.
+// The same in clusters of `cluster` blocks.
+template <class... Params, class... Args>
+void launch_cluster(void (*kernel)(Params...), unsigned blocks, unsigned threads, unsigned cluster, size_t shared,
+                    cudaStream_t stream, Args... args) {
+  if (shared > 40 * 1024)
+    XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)));
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim = {cluster, 1, 1};
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  XGBB_CUDA(cudaLaunchKernelEx(&config, kernel, Params(args)...));
+}
+
+// How the gradient takes rows of `dim` values: in the lanes of a warp (one: in
+// one cluster of blocks), in a block's registers where they hold them, else in
+// passes; and, where there are rows enough and they come in 16-byte pieces, in a
+// stream through shared memory (clusters of `ring` blocks).
 struct GradPlan {
-  bool fits, warp, one = false, ring = false;  // ring: rows enough to stream, if they come in 16-byte pieces
+  bool warp, one = false, fits;
+  uint32_t ring = 0;
   int lg = 0;
-  uint32_t threads = 0, blocks = 0;
-  GradPlan(uint64_t rows, uint64_t dim) : fits(dim <= 8192), warp(dim <= 256) {
-    if (!fits) {
-      blocks = uint32_t(std::min<uint64_t>(296, (rows + 15) / 16));
-      return;
-    }
+  uint32_t threads = 0, blocks = 0;            // of the first forms
+  uint32_t ring_threads = 0, ring_blocks = 0;  // of the stream
+  GradPlan(uint64_t rows, uint64_t dim) : warp(dim <= 256), fits(dim <= 8192) {
     if (warp) {
       while ((8ull << lg) < dim) ++lg;
       threads = kThreads;
@@ -861,15 +784,24 @@ struct GradPlan {
         while (blocks < 8 && blocks * once < rows) blocks *= 2;
         return;
       }
-      blocks = uint32_t(std::min<uint64_t>(148 * 4, (rows + (kThreads >> lg) - 1) / (kThreads >> lg)));
+      blocks = uint32_t(std::min<uint64_t>(148 * 4, (rows + once - 1) / once));
       return;
     }
-    threads = uint32_t((dim + 255) / 256 * 32);
-    const uint32_t full = 148 * (1024 / threads);
-    ring = rows >= 4ull * full;
     // Four rows a block at least: the blocks' parts are read again.
-    blocks = uint32_t(std::min<uint64_t>(full, (rows + 3) / 4));
+    threads = fits ? uint32_t((dim + 255) / 256 * 32) : 1024;
+    blocks = fits ? uint32_t(std::min<uint64_t>(148 * (1024 / threads), (rows + 3) / 4))
+                  : uint32_t(std::min<uint64_t>(296, (rows + 15) / 16));
+    for (uint32_t c = 1; c <= 8; c *= 2) {
+      if (dim > 4096 * c) continue;
+      ring_threads = uint32_t((dim + 256 * c - 1) / (256 * c) * 32);
+      // One block of 512 threads an SM; clusters of four or eight do not fit on
+      // every SM, and on 128 they do.
+      ring_blocks = c <= 2 ? 148 / c * (512 / ring_threads) * c : 128;
+      if (rows >= uint64_t(ring_blocks / c) * 16) ring = c;
+      break;
+    }
   }
+  uint32_t parts() const { return one ? 0 : ring ? std::max(blocks, ring_blocks / ring) : blocks; }
 };
 
 }  // namespace
@@ -885,7 +817,8 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
     const P *w = static_cast<const P*>(weight), *b = static_cast<const P*>(bias);
     with_norm_width<T>({x, y}, {weight, bias}, param_type, rows, dim, [&](auto width) {
       constexpr int VE = decltype(width)::value, kWide = 16 / sizeof(T);
-      constexpr int kMost = std::min(32 / VE, 16);  // pieces of a thread
+      constexpr int kMost = 32 / VE;                    // pieces that a thread may hold
+      constexpr int kSome = VE == 1 ? 8 : 16 / VE;      // pieces that it holds rather than leave them to more lanes
       const uint64_t pieces = (dim + VE - 1) / VE;
       const auto go = [&](auto count, auto in_warp, unsigned blocks, unsigned threads, int lg) {
         norm_kernel<T, P, VE, decltype(count)::value, decltype(in_warp)::value><<<blocks, threads, 0, stream>>>(
@@ -896,17 +829,20 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
         else if (need <= 2) go(std::integral_constant<int, 2>(), in_warp, blocks, threads, lg);
         else if (need <= 4) go(std::integral_constant<int, 4>(), in_warp, blocks, threads, lg);
         else if constexpr (kMost >= 8) {
-          if (need <= 8 || kMost == 8) go(std::integral_constant<int, 8>(), in_warp, blocks, threads, lg);
-          else go(std::integral_constant<int, kMost>(), in_warp, blocks, threads, lg);
+          if (need <= 8) go(std::integral_constant<int, 8>(), in_warp, blocks, threads, lg);
+          else if constexpr (kMost >= 16) {
+            if (need <= 16) go(std::integral_constant<int, 16>(), in_warp, blocks, threads, lg);
+            else go(std::integral_constant<int, kMost>(), in_warp, blocks, threads, lg);
+          }
         }
       };
       if (pieces <= 32 * kMost && rows >= 148) {
         int lg = 0;
-        while (lg < 5 && (1ull << lg) < pieces) ++lg;
+        while (lg < 5 && (uint64_t(kSome) << lg) < pieces) ++lg;
         pick((pieces + (1u << lg) - 1) >> lg, std::true_type(), blocks_for(rows, kThreads >> lg), kThreads, lg);
         return;
       }
-      if (pieces > 1024 * kMost) {
+      if (pieces > 512 * kMost) {
         norm_long_kernel<T, P, VE><<<unsigned(rows), 1024, 0, stream>>>(in, x.stride, rows, uint32_t(dim), w, b,
                                                                       eps, out, y.stride, mean, rstd);
         return;
@@ -927,8 +863,9 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
         }
       }
       // Many rows: as few threads a row as hold it. Few: as many as it has pieces.
-      const uint64_t each = rows >= 148 ? std::min<uint64_t>(kMost, 4) : 1;
-      const uint64_t threads = std::min<uint64_t>(1024, ((pieces + each - 1) / each + 31) / 32 * 32);
+      const uint64_t each = rows >= 148 ? 16 / VE : 1;
+      const uint64_t threads =
+          std::max<uint64_t>(std::min<uint64_t>(1024, ((pieces + each - 1) / each + 31) / 32 * 32), 32);
       pick((pieces + threads - 1) / threads, std::false_type(), unsigned(rows), unsigned(threads), 0);
     });
   });
@@ -936,8 +873,7 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
 }
 
 size_t layer_norm_backward_workspace(uint64_t rows, uint64_t dim) {
-  const GradPlan plan(rows, dim);
-  return plan.one ? 0 : size_t(plan.blocks) * 2 * dim * 4;
+  return size_t(GradPlan(rows, dim).parts()) * 2 * dim * 4;
 }
 
 void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const float* rstd, uint64_t rows,
@@ -960,42 +896,39 @@ void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const
         constexpr int VE = decltype(width)::value;
         const size_t sums = (kThreads / 32) * 2 * (size_t(8) << plan.lg) * 4;
         if (plan.one) {
-          cudaLaunchAttribute attribute{};
-          attribute.id = cudaLaunchAttributeClusterDimension;
-          attribute.val.clusterDim = {plan.blocks, 1, 1};
-          cudaLaunchConfig_t config{};
-          config.gridDim = dim3(plan.blocks);
-          config.blockDim = dim3(kThreads);
-          config.dynamicSmemBytes = sums;
-          config.stream = stream;
-          config.attrs = &attribute;
-          config.numAttrs = 1;
-          XGBB_CUDA(cudaLaunchKernelEx(&config, norm_grad_kernel<T, P, VE, 8 / VE, true, true>, g, grad.stride, v,
-                                       x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride,
-                                       static_cast<float*>(nullptr), plan.lg, dw, db));
-        } else if (plan.fits && plan.warp) {
-          norm_grad_kernel<T, P, VE, 8 / VE, true>
+          launch_cluster(norm_grad_kernel<T, P, VE, 8 / VE, true, kThreads, true>, plan.blocks, kThreads, plan.blocks,
+                         sums, stream, g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride,
+                         static_cast<float*>(nullptr), plan.lg, dw, db);
+        } else if (plan.warp) {
+          norm_grad_kernel<T, P, VE, 8 / VE, true, kThreads>
               <<<plan.blocks, plan.threads, sums, stream>>>(g, grad.stride, v, x.stride, mean, rstd, rows,
                                                             uint32_t(dim), w, out, dx.stride, parts, plan.lg, nullptr,
                                                             nullptr);
         } else if (plan.ring && VE * sizeof(T) == 16) {
           if constexpr (VE * sizeof(T) == 16) {
-            const bool full = dim == plan.threads * 8ull;
-            if (plan.threads <= 512) {
-              constexpr int R = sizeof(T) == 2 ? 4 : 2;
-              used = 148 * (512 / plan.threads);  // no more than the plan's blocks, which hold twice as many threads
-              launch_ring(full ? norm_grad_rows_kernel<T, P, R, true> : norm_grad_rows_kernel<T, P, R, false>, used,
-                          plan.threads, size_t(2) * R * 2 * 8 * sizeof(T) * plan.threads, stream, g, grad.stride, v,
-                          x.stride, mean, rstd, uint32_t(rows), uint32_t(dim), w, out, dx.stride, parts);
-            } else {
-              constexpr int S = sizeof(T) == 2 ? 4 : 3;
-              launch_ring(full ? norm_grad_ring_kernel<T, P, S, true> : norm_grad_ring_kernel<T, P, S, false>,
-                          plan.blocks, plan.threads, size_t(S) * 2 * 8 * sizeof(T) * plan.threads, stream, g,
-                          grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts);
-            }
+            constexpr int R = sizeof(T) == 2 ? 4 : 2;
+            const auto go = [&](auto blocks) {
+              constexpr int C = decltype(blocks)::value;
+              const auto kernel = dim == plan.ring_threads * 8ull * C ? norm_grad_rows_kernel<T, P, R, C, true>
+                                                                     : norm_grad_rows_kernel<T, P, R, C, false>;
+              const size_t shared = size_t(2) * R * 2 * 8 * sizeof(T) * plan.ring_threads;
+              used = plan.ring_blocks / C;
+              if (C == 1)
+                launch_ring(kernel, plan.ring_blocks, plan.ring_threads, shared, stream, g, grad.stride, v, x.stride,
+                            mean, rstd, uint32_t(rows), uint32_t(dim), w, out, dx.stride, parts);
+              else
+                launch_cluster(kernel, plan.ring_blocks, plan.ring_threads, C, shared, stream, g, grad.stride, v,
+                               x.stride, mean, rstd, uint32_t(rows), uint32_t(dim), w, out, dx.stride, parts);
+            };
+            if (plan.ring == 1) go(std::integral_constant<int, 1>());
+            else if (plan.ring == 2) go(std::integral_constant<int, 2>());
+            else if (plan.ring == 4) go(std::integral_constant<int, 4>());
+            else go(std::integral_constant<int, 8>());
           }
         } else if (plan.fits) {
-          norm_grad_kernel<T, P, VE, 8 / VE, false><<<plan.blocks, plan.threads, 0, stream>>>(
+          const auto kernel = plan.threads <= 512 ? norm_grad_kernel<T, P, VE, 8 / VE, false, 512>
+                                                  : norm_grad_kernel<T, P, VE, 8 / VE, false, 1024>;
+          kernel<<<plan.blocks, plan.threads, 0, stream>>>(
               g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts, 0, nullptr,
               nullptr);
         } else {
