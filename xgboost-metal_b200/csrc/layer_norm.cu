@@ -47,78 +47,113 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float (*part)[N]) {
   }
 }
 
-// Sums N values a thread over groups of G lanes, or over the block.
-template <bool WARP, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], uint32_t G, float (*part)[N]) {
-  if constexpr (WARP) {
+// How a row lies in threads that hold CH pieces each. kBlock: over the block,
+// every warp its own stretch; kWarp: in a warp; kLanes: in 2^lg lanes. Pieces of a
+// thread are 32 apart (kLanes: 2^lg), so that but for kLanes their addresses
+// differ by constants: with distances that only the launch knew, rows of odd
+// length took five times the instructions (67 a value, forward).
+enum Place { kBlock, kWarp, kLanes };
+template <int PLACE, int VE, int CH>
+struct Layout {
+  uint32_t G, lane, group, first;  // lanes of a row, this one, the row's place in the block, the thread's first column
+  uint32_t dim;
+  bool whole;  // the warp's pieces all exist
+  __device__ __forceinline__ Layout(uint32_t n, int lg) : dim(n) {
+    G = PLACE == kBlock ? blockDim.x : PLACE == kWarp ? 32 : 1u << lg;
+    lane = PLACE == kBlock ? threadIdx.x : threadIdx.x & (G - 1);
+    group = PLACE == kBlock ? 0 : PLACE == kWarp ? threadIdx.x >> 5 : threadIdx.x >> lg;
+    const uint32_t begin = PLACE == kBlock ? (threadIdx.x >> 5) * (CH * 32 * VE) : 0;
+    first = begin + (PLACE == kLanes ? lane : threadIdx.x & 31) * VE;
+    whole = PLACE != kLanes && begin + CH * 32 * VE <= dim;
+  }
+  __device__ __forceinline__ uint32_t apart(int i) const { return PLACE == kLanes ? i * G * VE : i * 32 * VE; }
+  __device__ __forceinline__ bool has(int i) const { return first + apart(i) < dim; }
+};
+// Calls f(i) for the pieces that exist.
+template <int CH, class L, class F>
+__device__ __forceinline__ void each_piece(const L& at, F&& f) {
+  if (at.whole) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      for (uint32_t m = G >> 1; m; m >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], m);
+    for (int i = 0; i < CH; ++i) f(i);
   } else {
-    block_sum<N>(v, part);
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (at.has(i)) f(i);
   }
 }
 
-// Forward. A row stays in registers between its load and its store: CH pieces
-// of VE values a thread, in their own type. WARP: 2^lg lanes hold a row, else
-// the block does.
-template <class T, class P, int VE, int CH, bool WARP>
-__global__ void __launch_bounds__(WARP ? kThreads : 1024)
+// Sums N values a thread over the row's threads.
+template <int PLACE, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], uint32_t G, float (*part)[N]) {
+  if constexpr (PLACE == kBlock) {
+    block_sum<N>(v, part);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (PLACE == kWarp) {
+#pragma unroll
+        for (int m = 16; m; m >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], m);
+      } else {
+        for (uint32_t m = G >> 1; m; m >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], m);
+      }
+    }
+  }
+}
+
+// Forward. A row stays in registers between its load and its store, CH pieces of
+// VE values a thread in their own type.
+template <class T, class P, int VE, int CH, int PLACE>
+__global__ void __launch_bounds__(PLACE == kBlock ? 1024 : kThreads)
     norm_kernel(const T* __restrict__ x, int64_t x_stride, uint64_t rows, uint32_t dim, const P* __restrict__ w,
                 const P* __restrict__ b, float eps, T* __restrict__ y, int64_t y_stride, float* __restrict__ mean,
                 float* __restrict__ rstd, int lg) {
   __shared__ float part[2][32][1];
-  const uint32_t G = WARP ? 1u << lg : blockDim.x;
-  const uint32_t at = WARP ? threadIdx.x & (G - 1) : threadIdx.x;
-  const uint64_t row = WARP ? uint64_t(blockIdx.x) * (kThreads >> lg) + (threadIdx.x >> lg) : blockIdx.x;
+  const Layout<PLACE, VE, CH> at(dim, lg);
+  const uint32_t groups = PLACE == kBlock ? 1 : PLACE == kWarp ? kThreads / 32 : kThreads >> lg;
+  const uint64_t row = uint64_t(blockIdx.x) * groups + at.group;
   const bool here = row < rows;
-  const T* xr = x + int64_t(row) * x_stride;
+  const T* const xr = x + int64_t(here ? row : 0) * x_stride + at.first;  // the sums of a row that is not there go nowhere
   Pack<T, VE> v[CH];
+  each_piece<CH>(at, [&](int i) { v[i] = load<T, VE>(xr + at.apart(i)); });
   float sum[1] = {0.0f};
+  each_piece<CH>(at, [&](int i) {
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const uint32_t c = (at + i * G) * VE;
-    if (here && c < dim) v[i] = load<T, VE>(xr + c);
-  }
-#pragma unroll
-  for (int i = 0; i < CH; ++i)
-    if (here && (at + i * G) * VE < dim)
-#pragma unroll
-      for (int e = 0; e < VE; ++e) sum[0] += v[i].f(e);
-  row_sum<WARP, 1>(sum, G, part[0]);
+    for (int e = 0; e < VE; ++e) sum[0] += v[i].f(e);
+  });
+  row_sum<PLACE, 1>(sum, at.G, part[0]);
   const float m = sum[0] / float(dim);
   float square[1] = {0.0f};
+  each_piece<CH>(at, [&](int i) {
 #pragma unroll
-  for (int i = 0; i < CH; ++i)
-    if (here && (at + i * G) * VE < dim)
-#pragma unroll
-      for (int e = 0; e < VE; ++e) square[0] = fmaf(v[i].f(e) - m, v[i].f(e) - m, square[0]);
-  row_sum<WARP, 1>(square, G, part[1]);
+    for (int e = 0; e < VE; ++e) square[0] = fmaf(v[i].f(e) - m, v[i].f(e) - m, square[0]);
+  });
+  row_sum<PLACE, 1>(square, at.G, part[1]);
   const float q = inverse_sqrt(square[0] / float(dim) + eps);
   if (!here) return;
-  if (at == 0) {
+  if (at.lane == 0) {
     if (mean) mean[row] = m;
     if (rstd) rstd[row] = q;
   }
-  T* yr = y + int64_t(row) * y_stride;
+  T* const yr = y + int64_t(row) * y_stride + at.first;
+  if (w && b) {
+    each_piece<CH>(at, [&](int i) {
+      const auto f = load<P, VE>(w + at.first + at.apart(i)), g = load<P, VE>(b + at.first + at.apart(i));
+      float r[VE];
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const uint32_t c = (at + i * G) * VE;
-    if (c >= dim) continue;
-    float r[VE];
+      for (int e = 0; e < VE; ++e) r[e] = fmaf((v[i].f(e) - m) * q, f.f(e), g.f(e));
+      store<T, VE>(yr + at.apart(i), r);
+    });
+  } else {
+    each_piece<CH>(at, [&](int i) {
+      float r[VE];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) r[e] = (v[i].f(e) - m) * q;
-    if (w) {
-      const auto f = load<P, VE>(w + c);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) r[e] *= f.f(e);
-    }
-    if (b) {
-      const auto f = load<P, VE>(b + c);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) r[e] += f.f(e);
-    }
-    store<T, VE>(yr + c, r);
+      for (int e = 0; e < VE; ++e) {
+        r[e] = (v[i].f(e) - m) * q;
+        if (w) r[e] *= to_f32(w[at.first + at.apart(i) + e]);
+        if (b) r[e] += to_f32(b[at.first + at.apart(i) + e]);
+      }
+      store<T, VE>(yr + at.apart(i), r);
+    });
   }
 }
 
@@ -323,12 +358,11 @@ __global__ void __launch_bounds__(1024)
 // Backward. A thread owns CH pieces of VE columns, 8 values in all, of every
 // row that its group takes: the rows' dx from registers, and the columns' sums
 // of dy h and dy kept in registers from the first row to the last. The next
-// row's values are under way while this one's are summed (packed 16-bit values,
-// whose registers leave room). WARP: 2^lg lanes hold a row, else the block does.
-// parts[block][2][dim] gets the block's sums; ONE: the grid is one cluster, whose
-// blocks add theirs up through each other's shared memory, block 0's first.
-template <class T, class P, int VE, int CH, bool WARP, int MOST, bool ONE = false>
-__global__ void __launch_bounds__(MOST, WARP && VE * sizeof(T) == 16 ? 4 : 1)
+// row's values are under way while this one's are summed, where registers allow
+// it. parts[block][2][dim] gets the block's sums; ONE: the grid is one cluster,
+// whose blocks add theirs up through each other's shared memory, block 0's first.
+template <class T, class P, int VE, int CH, int PLACE, int MOST, bool ONE = false>
+__global__ void __launch_bounds__(MOST, PLACE != kBlock && VE * sizeof(T) == 16 ? 4 : 1)
     norm_grad_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x, int64_t x_stride,
                      const float* __restrict__ mean, const float* __restrict__ rstd, uint64_t rows, uint32_t dim,
                      const P* __restrict__ w, T* __restrict__ dx, int64_t dx_stride, float* __restrict__ parts,
@@ -336,34 +370,29 @@ __global__ void __launch_bounds__(MOST, WARP && VE * sizeof(T) == 16 ? 4 : 1)
   constexpr bool kAhead = sizeof(T) == 2 && (VE == 8 || MOST < 1024);
   constexpr int E = CH * VE;
   __shared__ float part[2][32][2];
-  const uint32_t G = WARP ? 1u << lg : blockDim.x;
-  const uint32_t at = WARP ? threadIdx.x & (G - 1) : threadIdx.x;
-  const uint32_t groups = WARP ? kThreads >> lg : 1;
+  const Layout<PLACE, VE, CH> at(dim, lg);
+  const uint32_t groups = PLACE == kBlock ? 1 : PLACE == kWarp ? kThreads / 32 : kThreads >> lg;
   const uint64_t step = uint64_t(gridDim.x) * groups;
   const float inverse = 1.0f / float(dim);
   float wv[E], dw[E] = {}, db[E] = {};
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const uint32_t c = (at + i * G) * VE;
+  for (int i = 0; i < CH; ++i)
 #pragma unroll
-    for (int e = 0; e < VE; ++e) wv[i * VE + e] = w && c + e < dim ? to_f32(w[c + e]) : 1.0f;
-  }
+    for (int e = 0; e < VE; ++e) wv[i * VE + e] = w && at.has(i) ? to_f32(w[at.first + at.apart(i) + e]) : 1.0f;
   Pack<T, VE> nv[CH], nd[CH];
   float nm = 0.0f, nq = 0.0f;
   const auto fetch = [&](uint64_t row) {
     if (row >= rows) return;
     nm = mean[row];
     nq = rstd[row];
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const uint32_t c = (at + i * G) * VE;
-      if (c < dim) {
-        nv[i] = load<T, VE>(x + int64_t(row) * x_stride + c);
-        nd[i] = load<T, VE>(grad + int64_t(row) * grad_stride + c);
-      }
-    }
+    const T* const xr = x + int64_t(row) * x_stride + at.first;
+    const T* const gr = grad + int64_t(row) * grad_stride + at.first;
+    each_piece<CH>(at, [&](int i) {
+      nv[i] = load<T, VE>(xr + at.apart(i));
+      nd[i] = load<T, VE>(gr + at.apart(i));
+    });
   };
-  uint64_t row = uint64_t(blockIdx.x) * groups + (WARP ? threadIdx.x >> lg : 0);
+  uint64_t row = uint64_t(blockIdx.x) * groups + at.group;
   const uint64_t turns = (rows - min(rows, uint64_t(blockIdx.x) * groups) + step - 1) / step;
   if (kAhead) fetch(row);
   for (uint64_t turn = 0; turn < turns; ++turn, row += step) {
@@ -375,9 +404,8 @@ __global__ void __launch_bounds__(MOST, WARP && VE * sizeof(T) == 16 ? 4 : 1)
     if (kAhead) fetch(row + step);
     const bool here = row < rows;
     float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-      if (here && (at + i * G) * VE < dim)
+    if (here)
+      each_piece<CH>(at, [&](int i) {
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           const int j = i * VE + e;
@@ -387,37 +415,37 @@ __global__ void __launch_bounds__(MOST, WARP && VE * sizeof(T) == 16 ? 4 : 1)
           dw[j] = fmaf(d[i].f(e), h, dw[j]);
           db[j] += d[i].f(e);
         }
-    row_sum<WARP, 2>(sum, G, part[turn & 1]);
-    const float a = sum[0] * inverse, bb = sum[1] * inverse;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const uint32_t c = (at + i * G) * VE;
-      if (!here || c >= dim) continue;
+      });
+    row_sum<PLACE, 2>(sum, at.G, part[turn & 1]);
+    if (!here) continue;
+    const float a = -sum[0] * inverse * q, bb = -sum[1] * inverse * q;
+    T* const dxr = dx + int64_t(row) * dx_stride + at.first;
+    each_piece<CH>(at, [&](int i) {
       float r[VE];
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         const float h = (v[i].f(e) - m) * q, g = d[i].f(e) * wv[i * VE + e];
-        r[e] = q * (g - a - h * bb);
+        r[e] = fmaf(h, bb, fmaf(g, q, a));
       }
-      store<T, VE>(dx + int64_t(row) * dx_stride + c, r);
-    }
+      store<T, VE>(dxr + at.apart(i), r);
+    });
   }
   if (!parts && !ONE) return;
   float* out = parts + uint64_t(blockIdx.x) * 2 * dim;
-  if constexpr (WARP) {
+  if constexpr (PLACE != kBlock) {
     // The groups' sums: over the warp's lanes, then over the warps in order.
     extern __shared__ float sums[];  // [warps][2][G * E]
-    for (uint32_t m = G; m < 32; m <<= 1)
+    for (uint32_t m = at.G; m < 32; m <<= 1)
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         dw[j] += __shfl_xor_sync(0xffffffffu, dw[j], m);
         db[j] += __shfl_xor_sync(0xffffffffu, db[j], m);
       }
-    const uint32_t width = G * E, warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) < G)
+    const uint32_t width = at.G * E, warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) < at.G)
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const uint32_t c = (at + (j / VE) * G) * VE + j % VE;
+        const uint32_t c = at.first + at.apart(j / VE) + j % VE;
         sums[(warp * 2) * width + c] = dw[j];
         sums[(warp * 2 + 1) * width + c] = db[j];
       }
@@ -444,16 +472,13 @@ __global__ void __launch_bounds__(MOST, WARP && VE * sizeof(T) == 16 ? 4 : 1)
       cluster.sync();  // the blocks' memory is read until here
     }
   } else {
+    each_piece<CH>(at, [&](int i) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const uint32_t c = (at + i * G) * VE;
-#pragma unroll
-      for (int e = 0; e < VE; ++e)
-        if (c + e < dim) {
-          out[c + e] = dw[i * VE + e];
-          out[dim + c + e] = db[i * VE + e];
-        }
-    }
+      for (int e = 0; e < VE; ++e) {
+        out[at.first + at.apart(i) + e] = dw[i * VE + e];
+        out[dim + at.first + at.apart(i) + e] = db[i * VE + e];
+      }
+    });
   }
 }
 
@@ -525,7 +550,7 @@ __global__ void __launch_bounds__(512, 1)
   for (uint32_t row = id * R; row < rows; row += step, turn ^= 1) {
     char* const stage = own + turn * stage_bytes;
     float q[R], val[V];
-    float2 h[R][CH][H], g[R][CH][H];
+    float2 h[R][CH][H], d[R][CH][H];
     copy_wait<1>();
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -537,17 +562,14 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
       for (int i = 0; i < CH; ++i)
         if (has(i)) {
-          float2 d[H];
           unpack16<T>(*reinterpret_cast<const uint4*>(stage + r * row_bytes + i * G * 16), h[r][i]);
-          unpack16<T>(*reinterpret_cast<const uint4*>(stage + r * row_bytes + half + i * G * 16), d);
+          unpack16<T>(*reinterpret_cast<const uint4*>(stage + r * row_bytes + half + i * G * 16), d[r][i]);
 #pragma unroll
           for (int e = 0; e < H; ++e) {
             h[r][i][e] = mul2(add2(h[r][i][e], both(-m)), both(q[r]));
-            g[r][i][e] = mul2(d[e], wv[i][e]);
-            sum_g = add2(sum_g, g[r][i][e]);
-            sum_gh = fma2(g[r][i][e], h[r][i][e], sum_gh);
-            dw[i][e] = fma2(d[e], h[r][i][e], dw[i][e]);
-            db[i][e] = add2(db[i][e], d[e]);
+            const float2 g = mul2(d[r][i][e], wv[i][e]);
+            sum_g = add2(sum_g, g);
+            sum_gh = fma2(g, h[r][i][e], sum_gh);
           }
         }
       val[2 * r] = sum_g.x + sum_g.y;
@@ -564,7 +586,21 @@ __global__ void __launch_bounds__(512, 1)
         part[turn][0][lane / L][warp] = s;
       }
     }
-    barrier();
+    if constexpr (C > 1) cluster.barrier_arrive();
+    // The columns' sums, while the sums travel.
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (row + r < rows)
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+          if (has(i))
+#pragma unroll
+            for (int e = 0; e < H; ++e) {
+              dw[i][e] = fma2(d[r][i][e], h[r][i][e], dw[i][e]);
+              db[i][e] = add2(db[i][e], d[r][i][e]);
+            }
+    if constexpr (C > 1) cluster.barrier_wait();
+    else __syncthreads();
     s = 0.0f;
 #pragma unroll
     for (int q = 0; q < C; ++q) {
@@ -586,7 +622,7 @@ __global__ void __launch_bounds__(512, 1)
       for (int i = 0; i < CH; ++i)
         if (has(i)) {
 #pragma unroll
-          for (int e = 0; e < H; ++e) h[r][i][e] = fma2(h[r][i][e], b, fma2(g[r][i][e], both(q[r]), a));
+          for (int e = 0; e < H; ++e) h[r][i][e] = fma2(h[r][i][e], b, fma2(mul2(d[r][i][e], wv[i][e]), both(q[r]), a));
           *reinterpret_cast<uint4*>(to + r * dx_stride + i * G * VE) = pack16<T>(h[r][i]);
         }
     }
@@ -791,15 +827,14 @@ struct GradPlan {
     threads = fits ? uint32_t((dim + 255) / 256 * 32) : 1024;
     blocks = fits ? uint32_t(std::min<uint64_t>(148 * (1024 / threads), (rows + 3) / 4))
                   : uint32_t(std::min<uint64_t>(296, (rows + 15) / 16));
-    for (uint32_t c = 1; c <= 8; c *= 2) {
-      if (dim > 4096 * c) continue;
-      ring_threads = uint32_t((dim + 256 * c - 1) / (256 * c) * 32);
-      // One block of 512 threads an SM; clusters of four or eight do not fit on
-      // every SM, and on 128 they do.
-      ring_blocks = c <= 2 ? 148 / c * (512 / ring_threads) * c : 128;
-      if (rows >= uint64_t(ring_blocks / c) * 16) ring = c;
-      break;
-    }
+    // One block of 512 threads an SM. (Clusters of four blocks of 256 threads, two
+    // an SM, took 284 us for 16384 x 8192 of 16 bits where clusters of two blocks of
+    // 512 take 186.) Clusters of four and eight do not fill every SM, and fit on 128.
+    ring = dim <= 4096 ? 1 : dim <= 8192 ? 2 : dim <= 16384 ? 4 : dim <= 32768 ? 8 : 0;
+    if (!ring) return;
+    ring_threads = uint32_t((dim + 256 * ring - 1) / (256 * ring) * 32);
+    ring_blocks = ring == 1 ? 148 * (512 / ring_threads) : ring == 2 ? 148 : 128;
+    if (rows < uint64_t(ring_blocks / ring) * 16) ring = 0;
   }
   uint32_t parts() const { return one ? 0 : ring ? std::max(blocks, ring_blocks / ring) : blocks; }
 };
@@ -817,32 +852,33 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
     const P *w = static_cast<const P*>(weight), *b = static_cast<const P*>(bias);
     with_norm_width<T>({x, y}, {weight, bias}, param_type, rows, dim, [&](auto width) {
       constexpr int VE = decltype(width)::value, kWide = 16 / sizeof(T);
-      constexpr int kMost = 32 / VE;                    // pieces that a thread may hold
+      constexpr int kMost = std::min(32 / VE, 16);      // pieces that a thread may hold
       constexpr int kSome = VE == 1 ? 8 : 16 / VE;      // pieces that it holds rather than leave them to more lanes
       const uint64_t pieces = (dim + VE - 1) / VE;
-      const auto go = [&](auto count, auto in_warp, unsigned blocks, unsigned threads, int lg) {
-        norm_kernel<T, P, VE, decltype(count)::value, decltype(in_warp)::value><<<blocks, threads, 0, stream>>>(
+      const auto go = [&](auto count, auto place, unsigned blocks, unsigned threads, int lg) {
+        norm_kernel<T, P, VE, decltype(count)::value, decltype(place)::value><<<blocks, threads, 0, stream>>>(
             in, x.stride, rows, uint32_t(dim), w, b, eps, out, y.stride, mean, rstd, lg);
       };
-      const auto pick = [&](uint64_t need, auto in_warp, unsigned blocks, unsigned threads, int lg) {
-        if (need <= 1) go(std::integral_constant<int, 1>(), in_warp, blocks, threads, lg);
-        else if (need <= 2) go(std::integral_constant<int, 2>(), in_warp, blocks, threads, lg);
-        else if (need <= 4) go(std::integral_constant<int, 4>(), in_warp, blocks, threads, lg);
+      const auto pick = [&](uint64_t need, auto place, unsigned blocks, unsigned threads, int lg) {
+        if (need <= 1) go(std::integral_constant<int, 1>(), place, blocks, threads, lg);
+        else if (need <= 2) go(std::integral_constant<int, 2>(), place, blocks, threads, lg);
+        else if (need <= 4) go(std::integral_constant<int, 4>(), place, blocks, threads, lg);
         else if constexpr (kMost >= 8) {
-          if (need <= 8) go(std::integral_constant<int, 8>(), in_warp, blocks, threads, lg);
+          if (need <= 8) go(std::integral_constant<int, 8>(), place, blocks, threads, lg);
           else if constexpr (kMost >= 16) {
-            if (need <= 16) go(std::integral_constant<int, 16>(), in_warp, blocks, threads, lg);
-            else go(std::integral_constant<int, kMost>(), in_warp, blocks, threads, lg);
+            go(std::integral_constant<int, 16>(), place, blocks, threads, lg);
           }
         }
       };
-      if (pieces <= 32 * kMost && rows >= 148) {
+      if (pieces <= 32 * kMost && pieces <= 512 && rows >= 148) {
         int lg = 0;
         while (lg < 5 && (uint64_t(kSome) << lg) < pieces) ++lg;
-        pick((pieces + (1u << lg) - 1) >> lg, std::true_type(), blocks_for(rows, kThreads >> lg), kThreads, lg);
+        const uint64_t need = (pieces + (1u << lg) - 1) >> lg;
+        if (lg == 5) pick(need, std::integral_constant<int, kWarp>(), blocks_for(rows, kThreads >> lg), kThreads, lg);
+        else pick(need, std::integral_constant<int, kLanes>(), blocks_for(rows, kThreads >> lg), kThreads, lg);
         return;
       }
-      if (pieces > 512 * kMost) {
+      if (dim > 16384) {
         norm_long_kernel<T, P, VE><<<unsigned(rows), 1024, 0, stream>>>(in, x.stride, rows, uint32_t(dim), w, b,
                                                                       eps, out, y.stride, mean, rstd);
         return;
@@ -866,7 +902,7 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
       const uint64_t each = rows >= 148 ? 16 / VE : 1;
       const uint64_t threads =
           std::max<uint64_t>(std::min<uint64_t>(1024, ((pieces + each - 1) / each + 31) / 32 * 32), 32);
-      pick((pieces + threads - 1) / threads, std::false_type(), unsigned(rows), unsigned(threads), 0);
+      pick((pieces + threads - 1) / threads, std::integral_constant<int, kBlock>(), unsigned(rows), unsigned(threads), 0);
     });
   });
   XGBB_CUDA(cudaGetLastError());
@@ -896,11 +932,13 @@ void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const
         constexpr int VE = decltype(width)::value;
         const size_t sums = (kThreads / 32) * 2 * (size_t(8) << plan.lg) * 4;
         if (plan.one) {
-          launch_cluster(norm_grad_kernel<T, P, VE, 8 / VE, true, kThreads, true>, plan.blocks, kThreads, plan.blocks,
+          launch_cluster(norm_grad_kernel<T, P, VE, 8 / VE, kLanes, kThreads, true>, plan.blocks, kThreads, plan.blocks,
                          sums, stream, g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride,
                          static_cast<float*>(nullptr), plan.lg, dw, db);
         } else if (plan.warp) {
-          norm_grad_kernel<T, P, VE, 8 / VE, true, kThreads>
+          const auto kernel = plan.lg == 5 ? norm_grad_kernel<T, P, VE, 8 / VE, kWarp, kThreads>
+                                           : norm_grad_kernel<T, P, VE, 8 / VE, kLanes, kThreads>;
+          kernel
               <<<plan.blocks, plan.threads, sums, stream>>>(g, grad.stride, v, x.stride, mean, rstd, rows,
                                                             uint32_t(dim), w, out, dx.stride, parts, plan.lg, nullptr,
                                                             nullptr);
@@ -926,8 +964,8 @@ void layer_norm_backward(const Mat& grad, const Mat& x, const float* mean, const
             else go(std::integral_constant<int, 8>());
           }
         } else if (plan.fits) {
-          const auto kernel = plan.threads <= 512 ? norm_grad_kernel<T, P, VE, 8 / VE, false, 512>
-                                                  : norm_grad_kernel<T, P, VE, 8 / VE, false, 1024>;
+          const auto kernel = plan.threads <= 512 ? norm_grad_kernel<T, P, VE, 8 / VE, kBlock, 512>
+                                                  : norm_grad_kernel<T, P, VE, 8 / VE, kBlock, 1024>;
           kernel<<<plan.blocks, plan.threads, 0, stream>>>(
               g, grad.stride, v, x.stride, mean, rstd, rows, uint32_t(dim), w, out, dx.stride, parts, 0, nullptr,
               nullptr);
