@@ -447,3 +447,33 @@ def test_leaf_tokens_number_the_leaves():
     # The intercept is left: both sums of 12 values and an intercept of size 1 at most are within 16 u of their size.
     size = R.bag(k, table.abs())[0].max().item() + 1.0
     assert np.abs(rest - rest[0]).max() <= 4 * 16 * R.U * size
+
+
+def test_a_head_on_leaves_learns():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "leaf_embedding.py")
+    spec = importlib.util.spec_from_file_location("leaf_embedding", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    _, first, last = example.main(rows=6000, cols=8, trees=10, depth=4, dim=16, steps=40)
+    assert abs(first - np.log(2)) < 1e-3  # a head of zeros
+    assert last < first - 0.05
+    # Its gradients are those that torch derives for the same formula in 64 bits.
+    g = _gen(14)
+    head = example.Head(90, 12, 24, torch.device(DEV))
+    tokens, labels = _tokens(g, 300, 12, 90), (torch.rand(300, generator=g) < 0.5).float().to(DEV)
+    head.v = _matrix(g, 1, 24, F32)[0]
+    margin, saved = head.forward(tokens)
+    d_margin = torch.sigmoid(margin) - labels
+    grads = head.backward(d_margin, saved)
+    leaves = [t.double().requires_grad_() for t in (head.table, head.weight, head.bias, head.v, head.c)]
+    table, weight, bias, v, c = leaves
+    h = (table[tokens.clamp(min=0).long()] * (tokens >= 0)[..., None]).sum(1) * head.scale
+    y = torch.nn.functional.layer_norm(h, (24,), weight, bias)
+    ((y @ v + c) * d_margin.double()).sum().backward()
+    for got, leaf in zip(grads, leaves):
+        want = leaf.grad
+        # Sums of up to 300 x 24 float32 terms: 2^-24 of their size for each, and their size is at most that
+        # many times the largest; held here to 1e-4 of the largest, a thousand roundings.
+        assert float((got.double() - want).abs().max()) <= 1e-4 * float(want.abs().max())

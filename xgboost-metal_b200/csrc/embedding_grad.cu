@@ -40,7 +40,7 @@ struct SharePlan {
   int lg = 0;
   uint32_t tiles, share, shares;
   SharePlan(uint64_t n, uint64_t pieces) {
-    while (lg < 5 && (1ull << lg) < pieces) ++lg;
+    lg = lanes_log2(pieces);
     tiles = blocks_for(pieces, 1u << lg);
     const uint64_t even = ((n << lg) * tiles + 148 * 1024 - 1) / (148 * 1024);
     share = uint32_t(std::min<uint64_t>(std::max<uint64_t>(8, (even + 7) / 8 * 8), 4096));

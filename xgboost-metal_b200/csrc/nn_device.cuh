@@ -147,34 +147,45 @@ __device__ __forceinline__ void load_pairs(const P* p, float2 (&f)[H]) {
   }
 }
 
-// A row's values summed up: pairs of float32 where T comes in 16 bytes.
+// An even number of values as float pairs.
+template <class T, int VE>
+__device__ __forceinline__ float2 pair_of(const Pack<T, VE>& p, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float2(p.f(2 * i), p.f(2 * i + 1));
+  } else {
+    const uint32_t w = reinterpret_cast<const uint32_t*>(&p)[i];
+    if constexpr (std::is_same_v<T, __half>) return __half22float2(reinterpret_cast<const __half2&>(w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+}
+
+// A row's values summed up, in pairs of float32 where they are even in number.
 template <class T, int VE>
 struct Sum {
-  static constexpr bool kPairs = sizeof(T) * VE == 16;
+  static constexpr bool kPairs = VE % 2 == 0;
   float2 two[kPairs ? VE / 2 : 1];
-  float one[kPairs ? 1 : VE];
+  float one;
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (float2& v : two) v = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (float& v : one) v = 0.0f;
+    one = 0.0f;
   }
   template <bool SCALED>
   __device__ __forceinline__ void add(const Pack<T, VE>& p, float f) {
     if constexpr (kPairs) {
-      float2 v[VE / 2];
-      unpack16<T>(reinterpret_cast<const uint4&>(p), v);
 #pragma unroll
-      for (int e = 0; e < VE / 2; ++e)
-        two[e] = SCALED ? fma2(make_float2(f, f), v[e], two[e]) : add2(two[e], v[e]);
+      for (int e = 0; e < VE / 2; ++e) {
+        const float2 v = pair_of<T, VE>(p, e);
+        two[e] = SCALED ? fma2(make_float2(f, f), v, two[e]) : add2(two[e], v);
+      }
     } else {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) one[e] = SCALED ? fmaf(f, p.f(e), one[e]) : one[e] + p.f(e);
+      static_assert(kPairs || VE == 1, "one value or pairs");
+      one = SCALED ? fmaf(f, p.f(0), one) : one + p.f(0);
     }
   }
   __device__ __forceinline__ void get(float (&f)[VE]) const {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) f[e] = kPairs ? (e % 2 ? two[kPairs ? e / 2 : 0].y : two[kPairs ? e / 2 : 0].x) : one[kPairs ? 0 : e];
+    for (int e = 0; e < VE; ++e) f[e] = !kPairs ? one : e % 2 ? two[e / 2].y : two[e / 2].x;
   }
 };
 
@@ -217,6 +228,17 @@ inline bool row_aligned(const void* p, int64_t stride, uint64_t rows, size_t siz
   return reinterpret_cast<uintptr_t>(p) % b == 0 && (rows <= 1 || (stride * int64_t(size)) % int64_t(b) == 0);
 }
 
+// log2 of the lanes that own a row of `pieces` or a tile of it: up to 8 lanes as
+// many as it takes, else as many of 8, 16 and 32 as leave no more lanes idle in
+// the last tile than 8 would. (33 columns in two tiles of 32 lanes took bags of
+// 100 tokens 137 us where five tiles of 8 take 104.)
+inline int lanes_log2(uint64_t pieces) {
+  int lg = 0;
+  while (lg < 3 && (1ull << lg) < pieces) ++lg;
+  while (lg >= 3 && lg < 5 && ((pieces + 7) / 8 * 8) % (2ull << lg) == 0) ++lg;
+  return lg;
+}
+
 inline unsigned blocks_for(uint64_t work, uint64_t per_block) {
   return unsigned((work + per_block - 1) / per_block);
 }
@@ -249,7 +271,7 @@ void with_param_types(int a, int b, F&& f) {
 }
 
 // Calls f with the widest VE that the two matrices' rows allow: 16 bytes of
-// T, two 16-bit values, or one value.
+// T, four or two 16-bit values, or one value.
 template <class T, class F>
 void with_width(const Mat& a, uint64_t a_rows, const Mat& b, uint64_t b_rows, uint64_t dim, F&& f) {
   const auto fits = [&](uint64_t n) {
@@ -258,6 +280,7 @@ void with_width(const Mat& a, uint64_t a_rows, const Mat& b, uint64_t b_rows, ui
   };
   constexpr int kWide = 16 / sizeof(T);
   if (fits(kWide)) f(std::integral_constant<int, kWide>());
+  else if (kWide > 4 && fits(4)) f(std::integral_constant<int, 4>());
   else if (kWide > 4 && fits(2)) f(std::integral_constant<int, kWide == 4 ? 1 : 2>());
   else f(std::integral_constant<int, 1>());
 }
