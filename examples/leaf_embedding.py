@@ -4,7 +4,7 @@ Trains a booster, numbers the leaves that each row reaches (xgboost.nn.leaf_toke
 and fits a small head on the GPU in their place: a vector for every leaf, a row's
 vectors summed (embedding), normalised (layer_norm) and projected to a margin. The
 gradients run back through layer_norm_backward and embedding_backward; PyTorch
-provides the arrays, the projection and the update.
+provides the arrays, the projection and the update (Adam).
 
     python examples/leaf_embedding.py [--rows 262144] [--trees 100] [--depth 8] [--dim 64] [--steps 60]
 """
@@ -24,13 +24,14 @@ class Head:
     """margin = layer_norm(scale * sum of the leaves' vectors) . v + c, the
     vectors in bfloat16 with a float32 copy that the updates go to."""
 
-    def __init__(self, vocab, trees, dim, device, seed=0):
+    def __init__(self, vocab, trees, dim, device, rate=0.02, seed=0):
         g = torch.Generator(device=device).manual_seed(seed)
         self.scale = trees ** -0.5
         self.master = torch.randn(vocab, dim, generator=g, device=device)
         self.table = self.master.to(torch.bfloat16)
         self.weight, self.bias = torch.ones(dim, device=device), torch.zeros(dim, device=device)
         self.v, self.c = torch.zeros(dim, device=device), torch.zeros((), device=device)
+        self.optimizer = torch.optim.Adam((self.master, self.weight, self.bias, self.v, self.c), lr=rate)
 
     def forward(self, tokens):
         h = nn.embedding(tokens, self.table, scale=self.scale, bag=True, out_dtype=torch.float32)
@@ -45,18 +46,19 @@ class Head:
         d_table = nn.embedding_backward(dh, tokens, len(self.table), scale=self.scale, bag=True)
         return d_table, d_weight, d_bias, y.t() @ d_margin, d_margin.sum()
 
-    def step(self, tokens, labels, rate):
-        """One step of gradient descent on the mean logistic loss; the loss."""
+    def step(self, tokens, labels):
+        """One step down the mean logistic loss; the loss."""
         margin, saved = self.forward(tokens)
         loss = torch.nn.functional.softplus(margin) - labels * margin
         grads = self.backward((torch.sigmoid(margin) - labels) / len(labels), saved)
         for p, g in zip((self.master, self.weight, self.bias, self.v, self.c), grads):
-            p.sub_(rate * g)
+            p.grad = g
+        self.optimizer.step()
         self.table.copy_(self.master)
         return loss.mean()
 
 
-def main(rows=262144, cols=32, trees=100, depth=8, dim=64, steps=60, rate=1.0):
+def main(rows=262144, cols=32, trees=100, depth=8, dim=64, steps=60):
     """(log loss of the booster, of the head before and after its steps), on the training rows."""
     rng = np.random.default_rng(1337)
     X = rng.normal(size=(rows, cols)).astype(np.float32)
@@ -71,7 +73,7 @@ def main(rows=262144, cols=32, trees=100, depth=8, dim=64, steps=60, rate=1.0):
     device = torch.device("cuda", 0)
     tokens, labels = torch.from_numpy(tokens).to(device), torch.from_numpy(y).to(device)
     head = Head(vocab, trees, dim, device)
-    losses = [head.step(tokens, labels, rate) for _ in range(steps)]
+    losses = [head.step(tokens, labels) for _ in range(steps)]
     first, last = float(losses[0]), float(losses[-1])
     print("booster %.4f, head %.4f -> %.4f (%d leaves, %d steps)" % (trained, first, last, vocab, steps))
     return trained, first, last

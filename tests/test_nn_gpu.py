@@ -81,7 +81,7 @@ def test_bag_gradients(shape, types):
 
 # Sorted lists of every size around the sort's tile and the shares, all one token, few tokens, or more table rows than
 # two digits of the sort reach.
-@pytest.mark.parametrize("rows,vocab,dim", [(255, 1, 8), (256, 2, 8), (257, 1, 3), (4095, 255, 8), (4096, 256, 8),
+@pytest.mark.parametrize("rows,vocab,dim", [(8192, 3000, 64), (8192, 70001, 8), (5000, 1 << 21, 2), (255, 1, 8), (256, 2, 8), (257, 1, 3), (4095, 255, 8), (4096, 256, 8),
                                             (4097, 257, 8), (20000, 1, 40), (20011, 2, 33), (50000, 65535, 4),
                                             (50000, 65536, 4), (3000, 70000, 2), (600001, 300, 8), (4200, 70000, 160),
                                             (13000, 17, 300), (24576, 1 << 20, 4), (24577, 900, 24),
@@ -91,6 +91,8 @@ def test_sorted_gradient(rows, vocab, dim):
     grad = _matrix(g, rows, dim, F32)
     tokens = _tokens(g, rows, 1, vocab).reshape(rows)
     R.close(nn.embedding_backward(grad, tokens, vocab), R.bag_grad(grad, tokens[:, None], vocab), "dtable")
+    low = _tokens(g, rows, 1, min(vocab, 7)).reshape(rows)  # tokens that lie together
+    R.close(nn.embedding_backward(grad, low, vocab), R.bag_grad(grad, low[:, None], vocab), "low tokens")
     one = torch.full((rows,), vocab - 1, dtype=torch.int64, device=DEV)
     R.close(nn.embedding_backward(grad, one, vocab), R.bag_grad(grad, one[:, None], vocab), "one token")
 

@@ -693,12 +693,14 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Few tokens, in one launch: block (x, y) owns the table's rows [x span, x span
-// + span) in a tile of columns. It picks its rows' tokens out of all n, in their
-// order, sorts them by row in shared memory, zeroes the rows that have none, and
-// sums the others: groups of 2^lg lanes take equal shares of the sorted list,
-// and what crosses shares is joined through shared memory, in the shares' order.
-// No row is written by two blocks. An entry is row << kShift | position.
+// Few tokens, in one launch: of N x M blocks, block (x, y) owns the table's rows
+// x, x + N, ... in a tile of columns (neighbours apart, since the frequent tokens
+// of many vocabularies lie together). It picks its rows' tokens out of all n, in
+// their order, sorts them by row in shared memory, zeroes the rows that have
+// none, and sums the others: groups of 2^lg lanes take equal shares of the sorted
+// list, and what crosses shares is joined through shared memory, in the shares'
+// order. No row is written by two blocks. An entry is its row's number among the
+// block's rows << kShift | position.
 constexpr int kFewThreads = 512;
 constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kShift = 13;
@@ -708,7 +710,7 @@ constexpr uint32_t kFewCounts = kFewWarps * kDigits * 4;
 
 template <class T, class O, int VE, bool SCALED>
 __global__ void __launch_bounds__(kFewThreads, 2)
-    few_kernel(const T* __restrict__ grad, int64_t grad_stride, Source src, uint32_t n, uint32_t span, Scales s,
+    few_kernel(const T* __restrict__ grad, int64_t grad_stride, Source src, uint32_t n, FastDiv blocks, Scales s,
                float scale, uint32_t dim, O* __restrict__ out, int64_t out_stride, bool accumulate, bool bulk, int lg) {
   constexpr int U = 4, kBatch = 8;
   extern __shared__ __align__(16) uint32_t space[];
@@ -719,12 +721,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   float* const head = reinterpret_cast<float*>(space);
   float* const tail = head + kFewThreads * VE;
   uint32_t* const zeros = space + max(2 * kFewThreads * VE, int(2 * kFewCounts / 4));
+  const uint32_t span = (src.vocab + blocks.d - 1) / blocks.d;  // rows of a block, at most
+  const uint32_t rows_here = (src.vocab - blockIdx.x + blocks.d - 1) / blocks.d;
   uint32_t* const present = zeros + (bulk ? kZeroBytes / 4 : 0);  // a bit a row
   uint32_t* list = present + (span + 31) / 32;
   const uint32_t turns = (n + kFewThreads - 1) / kFewThreads, per = turns * 32;
   uint32_t* other = list + kFewWarps * per;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t row0 = blockIdx.x * span, rows_here = min(span, src.vocab - row0);
 
   // Warp w looks at the tokens [w per, w per + per) and keeps its rows' there.
   for (uint32_t i = threadIdx.x; i < (span + 31) / 32; i += kFewThreads) present[i] = 0;
@@ -740,8 +743,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     else src.load_keys<kTokens32, kBatch, 32>(i0 + lane, to, key);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const uint32_t r = key[i] - row0;
-      const bool mine = r < rows_here;  // kNone - row0 is past any row
+      const uint32_t r = blocks.div(key[i]);
+      const bool mine = key[i] != kNone && key[i] - r * blocks.d == blockIdx.x;
       const uint32_t votes = __ballot_sync(0xffffffffu, mine);
       if (mine) {
         list[from + own + __popc(votes & ((1u << lane) - 1))] = r << kShift | (i0 + i * 32 + lane);
@@ -754,8 +757,9 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 
   const uint32_t G = 1u << lg, me = threadIdx.x & (G - 1), group = threadIdx.x >> lg, groups = kFewThreads >> lg;
   const uint32_t col = (blockIdx.y * G + me) * VE;
-  O* const mine_out = out + int64_t(row0) * out_stride + col;
-  // Absent rows: wide ones whole, a share of the range's rows for each column
+  const int64_t row_stride = int64_t(blocks.d) * out_stride;
+  O* const mine_out = out + int64_t(blockIdx.x) * out_stride + col;
+  // Absent rows: wide ones whole, a share of the block's rows for each column
   // tile, written behind the threads' backs while they sort and sum; narrow ones
   // by plain stores.
   if (!accumulate && bulk) {
@@ -763,13 +767,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     const uint32_t last = uint32_t(uint64_t(rows_here) * (blockIdx.y + 1) / gridDim.y);
     for (uint32_t r = uint32_t(uint64_t(rows_here) * blockIdx.y / gridDim.y) + threadIdx.x; r < last; r += kFewThreads)
       if (!(present[r >> 5] >> (r & 31) & 1)) {
-        char* row = reinterpret_cast<char*>(out + int64_t(row0 + r) * out_stride);
+        char* row = reinterpret_cast<char*>(out + int64_t(blockIdx.x) * out_stride + r * row_stride);
         for (uint32_t at = 0; at < row_bytes; at += kZeroBytes) bulk_store(row + at, zeros, min(kZeroBytes, row_bytes - at));
       }
   } else if (!accumulate && col < dim) {
     const float zero[VE] = {};
     for (uint32_t r = group; r < rows_here; r += groups)
-      if (!(present[r >> 5] >> (r & 31) & 1)) store_global<O, VE>(mine_out + int64_t(r) * out_stride, zero);
+      if (!(present[r >> 5] >> (r & 31) & 1)) store_global<O, VE>(mine_out + r * row_stride, zero);
   }
 
   // In the order of rows and, within a row, of positions.
@@ -839,7 +843,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   }
 
   const auto write = [&](int32_t local, const float(&sum)[VE]) {
-    if (col < dim) write_row<O, VE>(mine_out + int64_t(local) * out_stride, sum, scale, accumulate);
+    if (col < dim) write_row<O, VE>(mine_out + local * row_stride, sum, scale, accumulate);
   };
   const uint32_t share = max((count + groups - 1) / groups, uint32_t(U));
   const uint32_t begin = min(count, group * share), end = min(count, begin + share);
@@ -912,18 +916,18 @@ int64_t token_step(const Tokens& k) {
   return k.rows == 1 || k.stride_row == int64_t(k.per_row) * k.stride_col ? k.stride_col : 0;
 }
 
-// Shared memory of few_kernel, and its grid: rows of a block, blocks, column tiles.
+// Shared memory of few_kernel, and its grid: blocks and column tiles.
 struct FewPlan {
   int lg = 0;
-  uint32_t tiles, span, blocks;
+  uint32_t tiles, blocks;
   size_t shared;
   FewPlan(uint32_t n, uint64_t vocab, uint64_t pieces, int ve, bool bulk) {
     while (lg < 5 && (1ull << lg) < pieces) ++lg;
     tiles = blocks_for(pieces, 1u << lg);
-    // About two blocks an SM: each reads all tokens.
-    const uint64_t ranges = std::max<uint64_t>(1, 296 / tiles);
-    span = uint32_t(std::min<uint64_t>(std::max<uint64_t>((vocab + ranges - 1) / ranges, 1), 1u << 16));
-    blocks = blocks_for(vocab, span);
+    // About two blocks an SM, which all read all tokens; a row's number takes 16 bits.
+    const uint64_t want = std::max<uint64_t>(std::max<uint64_t>(1, 296 / tiles), (vocab + 65535) / 65536);
+    blocks = uint32_t(std::min(want, vocab));
+    const uint64_t span = (vocab + blocks - 1) / blocks;
     shared = std::max<size_t>(2 * kFewThreads * ve * 4, 2 * kFewCounts) + (bulk ? kZeroBytes : 0) +
              (span + 31) / 32 * 4 + size_t(2) * 4 * ((n + kFewThreads - 1) / kFewThreads * kFewThreads);
   }
@@ -1024,7 +1028,8 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
         if (plan.shared > 40 * 1024)
           XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan.shared)));
         kernel<<<dim3(plan.blocks, plan.tiles), kFewThreads, plan.shared, stream>>>(
-            g, grad.stride, src, n, plan.span, s, scale, uint32_t(dim), y, out.stride, accumulate, bulk, plan.lg);
+            g, grad.stride, src, n, FastDiv(plan.blocks), s, scale, uint32_t(dim), y, out.stride, accumulate, bulk,
+            plan.lg);
         return;
       }
       const SharePlan plan(n, pieces);
