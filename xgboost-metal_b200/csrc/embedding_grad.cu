@@ -221,7 +221,10 @@ __global__ void __launch_bounds__(kThreads)
 // 32 entries at a time, and counts its own digits. The tile is put in
 // order in shared memory and leaves it in runs of equal digits, while the next
 // tile's keys are on their way. The first pass tells how many entries are
-// present.
+// present. Bound by shared memory (77 % of its wavefronts): 26.2 M entries take
+// 195 us in the first pass and 145 in the second, after 32 and 27 us for the
+// counts. With the lanes of a digit found by ballots it took 284 and 210 us, by
+// match.any 448 and 252.
 template <int READ, int kItems>
 __global__ void __launch_bounds__(kThreads, 4)
     sort_scatter_kernel(Source src, uint32_t* __restrict__ present, uint32_t n, uint32_t per, int shift,
@@ -342,7 +345,9 @@ __device__ __forceinline__ void zero_rows_beside(const Source& src, uint32_t n, 
 // The whole sort of up to 1024 ITEMS entries in one block, which holds them in
 // registers, (key, position) with 16-bit positions and ranks, and passes them
 // through shared memory after each pass. The other blocks zero the rows that
-// have no token meanwhile.
+// have no token meanwhile: of 16411 tokens' gradient of 65536 x 2048 f32 the sort
+// takes 30 us, the zeros 80, and all 116 (166 with the zeros beside the sums),
+// where its 604 MB take 92 at the copy rate.
 template <int READ, int ITEMS>
 __global__ void __launch_bounds__(kOneThreads)
     sort_one_kernel(Source src, uint32_t n, int passes, uint32_t* __restrict__ present,
@@ -479,6 +484,10 @@ __device__ __forceinline__ void zero_absent(const uint32_t* __restrict__ keys, u
 // that came in from the share before goes to head[share], of one that goes on
 // into the next to tail[share] (a share inside one token has its sum in head).
 // The first `zero_blocks` blocks zero the rows without a token.
+// Bound by the latency of gathers from the L2 cache: 26.2 M rows of 64 bf16, 3.36
+// GB, in 355 us (9.5 TB/s). With the keys of a step read by every lane, and
+// registers for the next step's, it took 540 us at three blocks an SM and 810,
+// spilling, at four; five and six blocks spill as well (405 and 415).
 template <class T, class O, int VE, bool SCALED>
 __global__ void __launch_bounds__(kThreads, 4)
     share_sum_kernel(const T* __restrict__ grad, int64_t grad_stride, const uint32_t* __restrict__ keys,
@@ -700,7 +709,9 @@ __global__ void __launch_bounds__(kThreads)
 // none, and sums the others: groups of 2^lg lanes take equal shares of the sorted
 // list, and what crosses shares is joined through shared memory, in the shares'
 // order. No row is written by two blocks. An entry is its row's number among the
-// block's rows << kShift | position.
+// block's rows << kShift | position. Bound by latency: 4100 tokens of 96 f32 take
+// 8 us, 8000 of 32 bf16 8 to 13, where the sort's launches alone take 20; from 8193
+// tokens on, each block's look at all of them costs more than the sort.
 constexpr int kFewThreads = 512;
 constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kShift = 13;

@@ -101,7 +101,9 @@ __device__ __forceinline__ void row_sum(float (&v)[N], uint32_t G, float (*part)
 }
 
 // Forward. A row stays in registers between its load and its store, CH pieces of
-// VE values a thread in their own type.
+// VE values a thread in their own type. Bound by device memory where pieces are of
+// 16 bytes (100000 x 784 f32: 96 us, the copy rate's time) and by instructions where
+// they are single values (65536 x 1001 bf16: 76 us, 53 % of it).
 template <class T, class P, int VE, int CH, int PLACE>
 __global__ void __launch_bounds__(PLACE == kBlock ? 1024 : kThreads)
     norm_kernel(const T* __restrict__ x, int64_t x_stride, uint64_t rows, uint32_t dim, const P* __restrict__ w,
@@ -184,6 +186,10 @@ __device__ __forceinline__ float warp_sums(float (&v)[N], uint32_t lane) {
 // warp w,
 //   mean = sum s_w / n,  variance n = sum M_w + n_w (s_w / n_w - mean)^2,
 // all of whose terms are positive. FULL: every thread holds CH pieces.
+// Bound by device memory: 32768 x 8192 bf16 in 167 us, 98 % of the copy rate. What
+// bounded it before was the chain of shuffles and barriers of a row: 262 us with two
+// barriers a row, 213 with one, 188 with two rows a barrier and two blocks an SM, 167
+// with four rows and one block of 128 registers a thread.
 template <class T, class P, int CH, int R, int MOST, bool FULL>
 __global__ void __launch_bounds__(MOST)
     norm_ring_kernel(const T* __restrict__ x, int64_t x_stride, uint32_t rows, uint32_t dim,
@@ -521,7 +527,9 @@ __global__ void __launch_bounds__(MOST, PLACE != kBlock && VE * sizeof(T) == 16 
 // cluster of C of them, R rows at a time: the rows' 2 R sums are reduced together,
 // each shuffle halving how many of them a lane holds, and share their barrier;
 // in a cluster each block leaves its warps' sums with all blocks. The next R
-// rows are under way into shared memory.
+// rows are under way into shared memory. Bound by device memory: 32768 x 4096 bf16
+// in 131 us, 94 % of the copy rate (179 us a row at a time); in clusters by their
+// barriers (16384 x 8192: 180 us, 68 %; 8000 x 16384: 232 us, 52 %).
 template <class T, class P, int R, int C, bool FULL>
 __global__ void __launch_bounds__(512, 1)
     norm_grad_rows_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x,
