@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kThreads)
 // each. SPLIT: S = 2^ls such groups share a row's tokens, a contiguous span each,
 // and add their sums up in shared memory, first span first; and the blocks of a
 // cluster, where there are several, share the tokens in the same way. A group
-// reads its tokens K to a lane, a step ahead, and hands them round by shuffles,
+// reads its tokens K to a lane, a step ahead, and passes them on by shuffles,
 // eight gathers in flight; a step without a missing token is summed without a
 // look at each.
 // Bound by instructions, then by the L1 cache's lines: 262144 bags of 100 x 64

@@ -59,7 +59,7 @@ struct Layout {
       return p;
     };
     for (int i = 0; i < 2; ++i) {
-      keys[i] = take(n * 4 + 512);  // a round of 32 lanes may read past the end
+      keys[i] = take(n * 4 + 512);  // 32 lanes' four entries may lie past the end
       values[i] = take(n * 4 + 512);
     }
     hist = take(size_t(kDigits) * sort_blocks(n) * 4);
@@ -478,7 +478,7 @@ __device__ __forceinline__ void zero_absent(const uint32_t* __restrict__ keys, u
 
 // Groups of G = 2^lg lanes own VE columns a lane (blockIdx.y: the tile of
 // columns) and sum `share` sorted entries each. The lanes read four entries
-// each, a round ahead, and hand them round by shuffles; a round that lies in one
+// each, a turn ahead, and pass them on by shuffles; a turn that lies in one
 // token, as most do where tokens are frequent, is summed without a look at its
 // keys. A token that lies in one share whole goes to its row; the sum of one
 // that came in from the share before goes to head[share], of one that goes on
@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     if (from_before || goes_on) store_global<float, VE>((from_before ? head : tail) + share * dim + col, y);
     else write_row<O, VE>(out + int64_t(current) * out_stride + col, y, scale, accumulate);
   };
-  // What a round reads past the list's end is not used.
+  // What a turn reads past the list's end is not used.
   const uint4* key4 = reinterpret_cast<const uint4*>(keys + begin) + lane;
   const uint4* value4 = reinterpret_cast<const uint4*>(values + begin) + lane;
   uint4 next_key = *key4, next_value = *value4;
