@@ -407,6 +407,16 @@ def test_refusals_of_tensors():
     for call, needle in ((lambda: nn.embedding(k, w.double()), "float32"),
                          (lambda: nn.embedding(k, w.half(), out_dtype=BF16), "table's type"),
                          (lambda: nn.embedding(k, w.t()), "contiguous"),
+                         (lambda: nn.embedding(k, w[0]), "two dimensions"),
+                         (lambda: nn.embedding(k.float(), w), "int32 or int64"),
+                         (lambda: nn.embedding(k[0], w, bag=True), "at least one dimension"),
+                         (lambda: nn.embedding_backward(w, k, 9), "shape of the lookup"),
+                         (lambda: nn.embedding_backward(w[:3], k, 1 << 31), "vocab"),
+                         (lambda: nn.embedding_backward(w[:3].half(), k, 9, out_dtype=BF16), "grad's type"),
+                         (lambda: nn.embedding_scale_backward(w[:3], k, w[:, :4]), "shape of the lookup"),
+                         (lambda: nn.layer_norm_backward(w, w.half(), k, k, w[0]), "x's shape and type"),
+                         (lambda: nn.layer_norm_backward(w, w, w[0], w[0], w[0]), "one value a row"),
+                         (lambda: nn.layer_norm(w, w[0].half()), "x's type"),
                          (lambda: nn.embedding(k.cpu(), w), "device memory"),
                          (lambda: nn.embedding(k, w, token_scale=torch.zeros(2, device=DEV)), "broadcast"),
                          (lambda: nn.embedding(k, w, out=w[:3]), "out must not be"),

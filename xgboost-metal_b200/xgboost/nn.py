@@ -53,12 +53,13 @@ _LIB.XGBBLayerNormBackwardWorkspace.argtypes = _SIZES[:2] + [ctypes.c_void_p]
 
 _TYPESTR = {"<f4": _F32, "<f2": _F16, "<i4": _I32, "<i8": _I64}
 _codes, _dtypes = {}, {}  # torch's dtypes by code and back, filled when the first tensor comes
-_raw_stream = None
+_raw_stream = _empty_like = None
 
 
 def _know_torch():
-    global _raw_stream
+    global _raw_stream, _empty_like
     t = sys.modules["torch"]
+    _empty_like = t.empty_like
     _codes.update({t.float32: _F32, t.float16: _F16, t.bfloat16: _BF16, t.int32: _I32, t.int64: _I64})
     _dtypes.update({c: d for d, c in _codes.items()})
     _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or \
@@ -313,6 +314,173 @@ def _space(workspace, size, like):
     return workspace, v[0]
 
 
+# The calls below take contiguous tensors of one device a short way, which asks
+# only what such tensors can be wrong in: a small call's time is mostly Python's.
+# Where that way finds anything else it gives None (or _Long), and the long way
+# takes the call or says what is wrong.
+
+
+class _Long(Exception):
+    pass
+
+
+def _plain(a, device, dim=None):
+    """(pointer, dtype code) of a contiguous tensor on `device`, of `dim` values in
+    one dimension if given."""
+    if a.get_device() != device or not a.is_contiguous() or \
+            (dim is not None and (a.numel() != dim or a.dim() != 1)):
+        raise _Long
+    return a.data_ptr(), _codes[a.dtype]
+
+
+def _short_way(f):
+    @functools.wraps(f)
+    def call(*args):
+        try:
+            return f(*args)
+        except (_Long, AttributeError, KeyError, IndexError, ZeroDivisionError):
+            return None
+    return call
+
+
+@_short_way
+def _embedding_short(tokens, table, scale, token_scale, bag, out_dtype):
+    device = table.get_device()
+    if device < 0 or table.dim() != 2:
+        return None
+    w, code = _plain(table, device)
+    k, k_code = _plain(tokens, device)
+    shape, (vocab, dim) = tokens.shape, table.shape
+    if code not in _FLOATS or k_code not in _INTS:
+        return None
+    s = 0
+    if token_scale is not None:
+        s, s_code = _plain(token_scale, device)
+        if s_code != _F32 or token_scale.shape != shape:
+            return None
+    per_row = shape[-1] if bag else 1
+    rows = tokens.numel() // per_row
+    lead = shape[:-1] if bag else shape
+    y_code = code if out_dtype is None else _codes[out_dtype]
+    if y_code not in _FLOATS:
+        return None
+    out = table.new_empty(*lead, dim) if y_code == code else table.new_empty(*lead, dim, dtype=out_dtype)
+    _call(_LIB.XGBBEmbedding, _pack_embedding(
+        k, s, rows, per_row, per_row, 1, per_row, 1, k_code, scale, w, out.data_ptr(), _raw_stream(device), vocab, dim,
+        dim, dim, code, y_code, device))
+    return out
+
+
+@_short_way
+def _embedding_backward_short(grad, tokens, vocab, scale, token_scale, bag, out_dtype):
+    device = grad.get_device()
+    if device < 0:
+        return None
+    g, code = _plain(grad, device)
+    k, k_code = _plain(tokens, device)
+    shape = tokens.shape
+    g_shape = grad.shape
+    if code not in _FLOATS or k_code not in _INTS or g_shape[:-1] != (shape[:-1] if bag else shape):
+        return None
+    s = 0
+    if token_scale is not None:
+        s, s_code = _plain(token_scale, device)
+        if s_code != _F32 or token_scale.shape != shape:
+            return None
+    per_row, dim = shape[-1] if bag else 1, g_shape[-1]
+    rows = tokens.numel() // per_row
+    y_code = code if out_dtype is None else _codes[out_dtype]
+    if y_code not in _FLOATS:
+        return None
+    size = embedding_backward_workspace(rows, per_row, vocab, dim)
+    out = grad.new_empty(vocab, dim) if y_code == code else grad.new_empty(vocab, dim, dtype=out_dtype)
+    space = grad.new_empty(size, dtype=sys.modules["torch"].uint8) if size else None
+    _call(_LIB.XGBBEmbeddingBackward, _pack_embedding_backward(
+        k, s, rows, per_row, per_row, 1, per_row, 1, k_code, scale, g, out.data_ptr(), space.data_ptr() if size else 0,
+        _raw_stream(device), size, vocab, dim, dim, dim, code, y_code, 0, device))
+    return out
+
+
+@_short_way
+def _embedding_scale_backward_short(grad, tokens, table, scale, bag):
+    device = grad.get_device()
+    if device < 0 or table.dim() != 2:
+        return None
+    g, code = _plain(grad, device)
+    k, k_code = _plain(tokens, device)
+    w, w_code = _plain(table, device)
+    shape, g_shape, (vocab, dim) = tokens.shape, grad.shape, table.shape
+    if code not in _FLOATS or w_code not in _FLOATS or k_code not in _INTS or g_shape[-1] != dim or \
+            g_shape[:-1] != (shape[:-1] if bag else shape):
+        return None
+    per_row = shape[-1] if bag else 1
+    out = grad.new_empty(*shape, dtype=_dtypes[_F32])
+    _call(_LIB.XGBBEmbeddingScaleBackward, _pack_embedding_scale_backward(
+        k, 0, tokens.numel() // per_row, per_row, per_row, 1, 0, 0, k_code, scale, g, w, out.data_ptr(),
+        _raw_stream(device), vocab, dim, dim, dim, code, w_code, device))
+    return out
+
+
+@_short_way
+def _layer_norm_short(x, weight, bias, eps):
+    device = x.get_device()
+    if device < 0:
+        return None
+    v, code = _plain(x, device)
+    shape = x.shape
+    dim = shape[-1]
+    w = b = 0
+    param = _F32
+    if weight is not None:
+        w, param = _plain(weight, device, dim)
+    if bias is not None:
+        b, b_code = _plain(bias, device, dim)
+        if weight is not None and b_code != param:
+            return None
+        param = b_code
+    if code not in _FLOATS or (param != code and param != _F32):
+        return None
+    out = _empty_like(x)
+    if len(shape) == 2:
+        rows = shape[0]
+        mean = x.new_empty(rows, dtype=_dtypes[_F32])
+    else:
+        rows = x.numel() // dim
+        mean = x.new_empty(shape[:-1], dtype=_dtypes[_F32])
+    rstd = _empty_like(mean)
+    _call(_LIB.XGBBLayerNorm, _pack_layer_norm(
+        v, w, b, out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _raw_stream(device), rows, dim, dim, dim, code,
+        param, device, eps))
+    return out, mean, rstd
+
+
+@_short_way
+def _layer_norm_backward_short(grad, x, mean, rstd, weight, bias_grad):
+    device = x.get_device()
+    if device < 0:
+        return None
+    v, code = _plain(x, device)
+    g, g_code = _plain(grad, device)
+    m, m_code = _plain(mean, device)
+    q, q_code = _plain(rstd, device)
+    shape = x.shape
+    dim = shape[-1]
+    lead = shape[:-1]
+    w, param = _plain(weight, device, dim)
+    if code not in _FLOATS or g_code != code or grad.shape != shape or m_code != _F32 or q_code != _F32 or \
+            mean.shape != lead or rstd.shape != lead or (param != code and param != _F32):
+        return None
+    rows = shape[0] if len(shape) == 2 else x.numel() // dim
+    out, dweight = _empty_like(x), _empty_like(weight)
+    dbias = _empty_like(weight) if bias_grad else None
+    size = layer_norm_backward_workspace(rows, dim)
+    space = x.new_empty(size, dtype=sys.modules["torch"].uint8) if size else None
+    _call(_LIB.XGBBLayerNormBackward, _pack_layer_norm_backward(
+        g, v, m, q, w, out.data_ptr(), dweight.data_ptr(), dbias.data_ptr() if bias_grad else 0,
+        space.data_ptr() if size else 0, _raw_stream(device), size, rows, dim, dim, dim, dim, code, param, device))
+    return out, dweight, dbias
+
+
 def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None, out_dtype=None, stream=None):
     """scale * token_scale * table[tokens]: shape tokens.shape + (dim,), or
     with `bag` the sum over the tokens' last dimension, tokens.shape[:-1] +
@@ -327,6 +495,10 @@ def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None
         with _on(stream, (tokens, table, token_scale, out)):
             return embedding(tokens, table, scale=scale, token_scale=token_scale, bag=bag, out=out,
                              out_dtype=out_dtype)
+    if out is None:
+        got = _embedding_short(tokens, table, scale, token_scale, bag, out_dtype)
+        if got is not None:
+            return got
     k, w = _view(tokens, "tokens"), _view(table, "table")
     rows, per_row, stride_row, stride_col, lead = _token_grid(k, bag)
     vocab, dim, table_stride = _matrix(w, "table")
@@ -362,6 +534,10 @@ def embedding_backward(grad, tokens, vocab, *, scale=1.0, token_scale=None, bag=
         with _on(stream, (grad, tokens, token_scale, out, workspace)):
             return embedding_backward(grad, tokens, vocab, scale=scale, token_scale=token_scale, bag=bag, out=out,
                                       out_dtype=out_dtype, accumulate=accumulate, workspace=workspace)
+    if out is None and workspace is None and not accumulate:
+        got = _embedding_backward_short(grad, tokens, vocab, scale, token_scale, bag, out_dtype)
+        if got is not None:
+            return got
     g, k = _view(grad, "grad"), _view(tokens, "tokens")
     rows, per_row, stride_row, stride_col, lead = _token_grid(k, bag)
     _, dim, g_stride = _matrix(g, "grad")
@@ -392,6 +568,10 @@ def embedding_scale_backward(grad, tokens, table, *, scale=1.0, bag=False, out=N
     if stream is not None and hasattr(grad, "data_ptr"):
         with _on(stream, (grad, tokens, table, out)):
             return embedding_scale_backward(grad, tokens, table, scale=scale, bag=bag, out=out)
+    if out is None:
+        got = _embedding_scale_backward_short(grad, tokens, table, scale, bag)
+        if got is not None:
+            return got
     g, k, w = _view(grad, "grad"), _view(tokens, "tokens"), _view(table, "table")
     rows, per_row, stride_row, stride_col, lead = _token_grid(k, bag)
     vocab, dim, table_stride = _matrix(w, "table")
@@ -416,6 +596,10 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
     if stream is not None and hasattr(x, "data_ptr"):
         with _on(stream, (x, weight, bias, out, mean, rstd)):
             return layer_norm(x, weight, bias, eps=eps, out=out, mean=mean, rstd=rstd)
+    if out is None and mean is None and rstd is None:
+        got = _layer_norm_short(x, weight, bias, eps)
+        if got is not None:
+            return got
     v = _view(x, "x")
     rows, dim, stride = _matrix(v, "x")
     w = b = None
@@ -429,7 +613,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
         param = b_code
     lead = v[1][:-1]
     if out is None and v[5] is not None and x.is_contiguous():
-        out = sys.modules["torch"].empty_like(x)
+        out = _empty_like(x)
         y, y_stride, y_device = out.data_ptr(), dim, v[4]
     else:
         out, y, _, y_stride, y_device = _result(out, v[1], v[3], v, "out")
@@ -460,6 +644,10 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
         with _on(stream, (grad, x, mean, rstd, weight, out, dweight, dbias, workspace)):
             return layer_norm_backward(grad, x, mean, rstd, weight, bias_grad=bias_grad, out=out, dweight=dweight,
                                        dbias=dbias, workspace=workspace)
+    if weight is not None and out is None and dweight is None and dbias is None and workspace is None:
+        got = _layer_norm_backward_short(grad, x, mean, rstd, weight, bias_grad)
+        if got is not None:
+            return got
     g, v = _view(grad, "grad"), _view(x, "x")
     rows, dim, stride = _matrix(v, "x")
     _, _, g_stride = _matrix(g, "grad")
@@ -469,7 +657,7 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
     m, m_device = _row_values(mean, lead, "mean")
     q, q_device = _row_values(rstd, lead, "rstd")
     if out is None and v[5] is not None and x.is_contiguous():
-        out = sys.modules["torch"].empty_like(x)
+        out = _empty_like(x)
         dx, dx_stride, dx_device = out.data_ptr(), dim, v[4]
     else:
         out, dx, _, dx_stride, dx_device = _result(out, v[1], v[3], v, "out")
