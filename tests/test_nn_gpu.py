@@ -489,3 +489,40 @@ def test_a_head_on_leaves_learns():
         # Sums of up to 300 x 24 float32 terms: 2^-24 of their size for each, and their size is at most that
         # many times the largest; held here to 1e-4 of the largest, a thousand roundings.
         assert float((got.double() - want).abs().max()) <= 1e-4 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("rows,per_row,vocab,dim", [(9000, 1, 300, 40), (30000, 1, 70000, 8), (700, 100, 2560, 64),
+                                                    (16000, 1, 40000, 1024)])
+def test_what_a_workspace_held_does_not_matter(rows, per_row, vocab, dim):
+    """Back to back and replayed, on workspaces full of what never was an index."""
+    g = _gen(15, rows, vocab)
+    grad, tokens = _matrix(g, rows, dim, F32), _tokens(g, rows, per_row, vocab)
+    want = nn.embedding_backward(grad, tokens, vocab, bag=True)
+    R.close(want, R.bag_grad(grad, tokens, vocab))
+    space = torch.empty(nn.embedding_backward_workspace(rows, per_row, vocab, dim), dtype=torch.uint8, device=DEV)
+    out = torch.empty_like(want)
+    x, w = _matrix(g, 3000, 600, F32), torch.ones(600, device=DEV)
+    _, mean, rstd = nn.layer_norm(x, w)
+    first = nn.layer_norm_backward(x, x * 2, mean, rstd, w)
+    twice = x * 2
+    parts = torch.empty(nn.layer_norm_backward_workspace(3000, 600), dtype=torch.uint8, device=DEV)
+
+    def both():
+        space.fill_(0xff)
+        parts.fill_(0xff)
+        nn.embedding_backward(grad, tokens, vocab, bag=True, out=out, workspace=space)
+        return nn.layer_norm_backward(x, twice, mean, rstd, w, workspace=parts)
+
+    for _ in range(3):
+        again = both()
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(again, first))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = both()
+    for _ in range(3):
+        out.fill_(7.0)
+        for a in again:
+            a.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(again, first))
