@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kThreads)
 // eight gathers in flight; a step without a missing token is summed without a
 // look at each.
 // Bound by instructions, then by the L1 cache's lines: 262144 bags of 100 x 64
-// bf16 gather 3.36 GB in 270 us (12.4 TB/s, 72 % of the issue slots), where what
+// bf16 gather 3.36 GB in 269 us (12.5 TB/s, 72 % of the issue slots), where what
 // they read and write once is 175 MB. 64 registers, so that an SM holds 1024
 // threads: at 128 it took 493 us. Seven bags of 2000 x 33 f32 take 20.6 us in
 // blocks alone and 5.0 in clusters of eight.
