@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 4)
 // The rows without a token, for blocks beside a block that sorts: block b of
 // `blocks` looks through all tokens for those of its equal share of the rows and
 // zeroes the others: wide rows by copies behind the threads' backs, narrow ones
-// by plain stores. No block at all where there is nothing to zero.
+// by plain stores.
 struct Rows {
   char* data;
   int64_t stride;  // bytes

@@ -514,11 +514,14 @@ __global__ void __launch_bounds__(MOST, PLACE != kBlock && VE * sizeof(T) == 16 
     }
   } else {
     each_piece<CH>(at, [&](int i) {
+      float a[VE], b[VE];
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        out[at.first + at.apart(i) + e] = dw[i * VE + e];
-        out[dim + at.first + at.apart(i) + e] = db[i * VE + e];
+        a[e] = dw[i * VE + e];
+        b[e] = db[i * VE + e];
       }
+      store_global<float, VE>(out + at.first + at.apart(i), a);
+      store_global<float, VE>(out + dim + at.first + at.apart(i), b);
     });
   }
 }
@@ -675,14 +678,18 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const uint32_t c = (at + i * G) * VE;
-    if (c < dim)
+    float a[VE], b[VE];
 #pragma unroll
-      for (int e = 0; e < H; ++e) {
-        out[c + 2 * e] = dw[i][e].x;
-        out[c + 2 * e + 1] = dw[i][e].y;
-        out[dim + c + 2 * e] = db[i][e].x;
-        out[dim + c + 2 * e + 1] = db[i][e].y;
-      }
+    for (int e = 0; e < H; ++e) {
+      a[2 * e] = dw[i][e].x;
+      a[2 * e + 1] = dw[i][e].y;
+      b[2 * e] = db[i][e].x;
+      b[2 * e + 1] = db[i][e].y;
+    }
+    if (c < dim) {
+      store_global<float, VE>(out + c, a);
+      store_global<float, VE>(out + dim + c, b);
+    }
   }
 }
 
@@ -757,11 +764,8 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
   float* out = parts + uint64_t(blockIdx.x) * 2 * dim + c;
-#pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    out[e] = dw[e];
-    out[dim + e] = db[e];
-  }
+  store_global<float, VE>(out, dw);
+  store_global<float, VE>(out + dim, db);
 }
 
 // The parts' sums: 32 columns a block (of dw's and db's 2 dim), each warp every
@@ -866,9 +870,9 @@ struct GradPlan {
       blocks = uint32_t(std::min<uint64_t>(148 * 4, (rows + once - 1) / once));
       return;
     }
-    // Four rows a block at least: the blocks' parts are read again.
+    // A block an SM, then four rows a block at least: the blocks' parts are read again.
     threads = fits ? uint32_t((dim + 255) / 256 * 32) : 1024;
-    blocks = fits ? uint32_t(std::min<uint64_t>(148 * (1024 / threads), (rows + 3) / 4))
+    blocks = fits ? uint32_t(std::min<uint64_t>(148 * (1024 / threads), std::max((rows + 3) / 4, std::min<uint64_t>(rows, 148))))
                   : uint32_t(std::min<uint64_t>(296, (rows + 15) / 16));
     // One block of 512 threads an SM. (Clusters of four blocks of 256 threads, two
     // an SM, took 284 us for 16384 x 8192 of 16 bits where clusters of two blocks of
