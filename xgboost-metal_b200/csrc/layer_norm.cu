@@ -531,8 +531,8 @@ __global__ void __launch_bounds__(MOST, PLACE != kBlock && VE * sizeof(T) == 16 
 // each shuffle halving how many of them a lane holds, and share their barrier;
 // in a cluster each block leaves its warps' sums with all blocks. The next R
 // rows are under way into shared memory. Bound by device memory: 32768 x 4096 bf16
-// in 131 us, 94 % of the copy rate (179 us a row at a time); in clusters by their
-// barriers (16384 x 8192: 180 us, 68 %; 8000 x 16384: 232 us, 52 %).
+// in 127 us, 97 % of the copy rate (179 us a row at a time); in clusters by their
+// barriers (16384 x 8192: 176 us, 70 %; 8000 x 16384: 227 us, 53 %).
 template <class T, class P, int R, int C, bool FULL>
 __global__ void __launch_bounds__(512, 1)
     norm_grad_rows_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x,
@@ -876,7 +876,7 @@ struct GradPlan {
                   : uint32_t(std::min<uint64_t>(296, (rows + 15) / 16));
     // One block of 512 threads an SM. (Clusters of four blocks of 256 threads, two
     // an SM, took 284 us for 16384 x 8192 of 16 bits where clusters of two blocks of
-    // 512 take 186.) Clusters of four and eight do not fill every SM, and fit on 128.
+    // 512 took 186.) Clusters of four and eight do not fill every SM, and fit on 128.
     ring = dim <= 4096 ? 1 : dim <= 8192 ? 2 : dim <= 16384 ? 4 : dim <= 32768 ? 8 : 0;
     if (!ring) return;
     ring_threads = uint32_t((dim + 256 * ring - 1) / (256 * ring) * 32);
