@@ -237,8 +237,19 @@ __global__ void __launch_bounds__(kThreads, 4)
   __shared__ uint32_t keys[kTile < kWarps * kDigits ? kWarps * kDigits : kTile], values[kTile];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = threadIdx.x;
   if (READ == kSorted) n = *present;
-  uint32_t all;
-  uint32_t next = block_scan<kWarps>(totals[d], warp_sums, all) + hist[d * gridDim.x + blockIdx.x];
+  uint32_t all, before = 0, digits = 0;
+  if (totals) {
+    digits = totals[d];
+    before = hist[d * gridDim.x + blockIdx.x];
+  } else {  // few blocks, whose counts nobody has added up
+    const uint32_t* h = hist + d * gridDim.x;
+#pragma unroll 8
+    for (uint32_t b = 0; b < gridDim.x; ++b) {
+      if (b < blockIdx.x) before += h[b];
+      digits += h[b];
+    }
+  }
+  uint32_t next = block_scan<kWarps>(digits, warp_sums, all) + before;
   if (READ != kSorted && blockIdx.x == 0 && d == 0) *present = all;
   uint32_t* const masks = keys;  // [warps][digits], while the tile is ranked
   const uint32_t mine = warp * (kItems * 32) + lane;
@@ -1004,9 +1015,11 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
           constexpr int READ = decltype(read)::value;
           const int to = pass ? sorted ^ 1 : 0;
           sort_hist_kernel<READ><<<grid, kThreads, 0, stream>>>(src, present, n, per, pass * 8, u32(at.hist));
-          sort_scan_kernel<<<kDigits, kThreads, 0, stream>>>(u32(at.hist), grid, u32(at.totals));
+          // Up to 64 blocks add the counts up themselves: a launch less.
+          if (grid > 64) sort_scan_kernel<<<kDigits, kThreads, 0, stream>>>(u32(at.hist), grid, u32(at.totals));
           const auto scatter = tile == kThreads * 4 ? sort_scatter_kernel<READ, 4> : sort_scatter_kernel<READ, 16>;
-          scatter<<<grid, kThreads, 0, stream>>>(src, present, n, per, pass * 8, u32(at.hist), u32(at.totals),
+          scatter<<<grid, kThreads, 0, stream>>>(src, present, n, per, pass * 8, u32(at.hist),
+                                                 grid > 64 ? u32(at.totals) : nullptr,
                                                  u32(at.keys[to]), u32(at.values[to]));
           sorted = to;
         };
