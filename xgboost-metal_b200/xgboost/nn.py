@@ -300,18 +300,18 @@ def _row_values(a, lead, what):
 
 
 def _space(workspace, size, like):
-    """(workspace, pointer) of `size` bytes."""
+    """(workspace, pointer, device) of `size` bytes."""
     if workspace is None:
         if like[5] is None:
             raise XGBoostError("workspace must be given where the inputs are no tensors")
         workspace = like[5].new_empty(size, dtype=sys.modules["torch"].uint8)
-        return workspace, workspace.data_ptr()
+        return workspace, workspace.data_ptr(), like[4]
     v = _view(workspace, "workspace")
     n, stride = _flat(v[1], v[2], "workspace")
     width = v[5].element_size() if v[5] is not None else int(workspace.__cuda_array_interface__["typestr"][2:])
     if n * width < size or (n > 1 and stride != 1):
         raise XGBoostError("workspace must be %d contiguous bytes" % size)
-    return workspace, v[0]
+    return workspace, v[0], v[4]
 
 
 # The calls below take contiguous tensors of one device a short way, which asks
@@ -550,10 +550,10 @@ def embedding_backward(grad, tokens, vocab, *, scale=1.0, token_scale=None, bag=
     code = g[3] if out_dtype is None else _dtype_code(out_dtype)
     out, y, code, y_stride, y_device = _result(out, (vocab, dim), 0 if out is not None and out_dtype is None else code,
                                                g, "out")
-    device = _one_device(g[4], k[4], s_device, y_device)
-    space = 0
+    space, space_device = 0, -1
     if size:
-        workspace, space = _space(workspace, size, g)
+        workspace, space, space_device = _space(workspace, size, g)
+    device = _one_device(g[4], k[4], s_device, y_device, space_device)
     _call(_LIB.XGBBEmbeddingBackward, _pack_embedding_backward(
         k[0], s, rows, per_row, stride_row, stride_col, s_row, s_col, k[3], scale, g[0], y, space,
         _handle(stream, device, g), size, vocab, dim, g_stride, y_stride, g[3], code, bool(accumulate), device))
@@ -662,7 +662,7 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
     else:
         out, dx, _, dx_stride, dx_device = _result(out, v[1], v[3], v, "out")
     w = dw = db = space = size = 0
-    w_code, w_device, dw_device, db_device = _F32, -1, -1, -1
+    w_code, w_device, dw_device, db_device, space_device = _F32, -1, -1, -1, -1
     if weight is not None:
         wv = _vector(weight, dim, v[3], "weight")
         w, _, _, w_code, w_device, _ = wv
@@ -671,10 +671,10 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
             dbias, db, db_device = _flat_result(dbias, (dim,), w_code, wv, "dbias")
         size = layer_norm_backward_workspace(rows, dim)
         if size:
-            workspace, space = _space(workspace, size, v)
+            workspace, space, space_device = _space(workspace, size, v)
     elif dweight is not None or dbias is not None:
         raise XGBoostError("dweight and dbias need weight")
-    device = _one_device(v[4], g[4], m_device, q_device, w_device, dx_device, dw_device, db_device)
+    device = _one_device(v[4], g[4], m_device, q_device, w_device, dx_device, dw_device, db_device, space_device)
     _call(_LIB.XGBBLayerNormBackward, _pack_layer_norm_backward(
         g[0], v[0], m, q, w, dx, dw, db, space, _handle(stream, device, v), size, rows, dim, g_stride, stride,
         dx_stride, v[3], w_code, device))
