@@ -1,0 +1,77 @@
+"""How xgboost.nn's calls go with one another and with the arrays' producers, on
+the GPU: host threads, streams."""
+import threading
+
+import pytest
+import torch
+
+import nn_reference as R
+from xgboost import nn
+from xgboost.core import _LIB
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _refused(calls, times):
+    """How many of each call's repetitions the library refused, every call on a host thread of its own."""
+    refused, start = [0] * len(calls), threading.Barrier(len(calls))
+
+    def work(i):
+        function, args = calls[i]
+        start.wait()
+        refused[i] = sum(function(args) != 0 for _ in range(times))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return refused
+
+
+# The library's calls back to back, which leave no time between one thread's and another's: with the shared memory's
+# limit set to each launch's own, 72 to 610 of 20000 gradients of the longer list were refused in each of 4 threads.
+
+
+def test_threads_with_short_and_long_lists():
+    g = torch.Generator().manual_seed(1)
+    held, calls = [], []
+    for n, vocab in ((600, 40), (8192, 3000)) * 2:
+        grad, k = torch.randn(n, 16, generator=g).to(DEV), torch.randint(0, vocab, (n,), generator=g).to(DEV)
+        out, stream = torch.zeros(vocab, 16, device=DEV), torch.cuda.Stream(DEV)
+        held.append((grad, k, out, stream))
+        calls.append((_LIB.XGBBEmbeddingBackward, nn._pack_embedding_backward(
+            k.data_ptr(), 0, n, 1, 1, 1, 0, 0, 8, 1.0, grad.data_ptr(), out.data_ptr(), 0, stream.cuda_stream, 0, vocab,
+            16, 16, 16, 1, 1, 0, 0)))
+    torch.cuda.synchronize()
+    assert _refused(calls, 20000) == [0] * 4
+    for grad, k, out, _ in held:
+        R.close(out, R.bag_grad(grad, k[:, None], len(out)))
+
+
+def test_threads_with_rows_of_different_lengths():
+    g = torch.Generator().manual_seed(2)
+    held, forward, backward = [], [], []
+    for dim in (3080, 4096):
+        x, w, stream = torch.randn(2400, dim, generator=g).to(BF16).to(DEV), torch.ones(dim, device=DEV), \
+            torch.cuda.Stream(DEV)
+        y, dx = torch.zeros_like(x), torch.zeros_like(x)
+        _, mean, rstd = nn.layer_norm(x)
+        dw, db = torch.zeros(dim, device=DEV), torch.zeros(dim, device=DEV)
+        size = nn.layer_norm_backward_workspace(2400, dim)
+        space = torch.empty(size, dtype=torch.uint8, device=DEV)
+        held.append((x, w, stream, y, dx, mean, rstd, dw, db, space))
+        forward.append((_LIB.XGBBLayerNorm, nn._pack_layer_norm(
+            x.data_ptr(), w.data_ptr(), 0, y.data_ptr(), 0, 0, stream.cuda_stream, 2400, dim, dim, dim, 4, 1, 0, 1e-5)))
+        backward.append((_LIB.XGBBLayerNormBackward, nn._pack_layer_norm_backward(
+            x.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), dx.data_ptr(), dw.data_ptr(),
+            db.data_ptr(), space.data_ptr(), stream.cuda_stream, size, 2400, dim, dim, dim, dim, 4, 1, 0)))
+    torch.cuda.synchronize()
+    assert _refused(forward, 800) == [0] * 2 and _refused(backward, 800) == [0] * 2
+    for x, w, _, y, dx, mean, rstd, dw, db, _ in held:
+        R.close(y, R.norm(x, w)[0])
+        for got, want in zip((dx, dw, db), R.norm_grad(x, x, mean, rstd, w)):
+            R.close(got, want)

@@ -940,6 +940,9 @@ int64_t token_step(const Tokens& k) {
 
 // Shared memory of few_kernel, and its grid: blocks and column tiles.
 struct FewPlan {
+  // Of the widest pieces, all tokens and 65536 rows a block.
+  static constexpr size_t kMostShared = std::max<size_t>(2 * kFewThreads * 8 * 4, 2 * kFewCounts) + kZeroBytes +
+                                        65536 / 8 + size_t(2) * 4 * kFewTokens;
   int lg = 0;
   uint32_t tiles, blocks;
   size_t shared;
@@ -996,8 +999,7 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
           constexpr int ITEMS = decltype(items)::value;
           const auto kernel = sort_one_kernel<decltype(read)::value, ITEMS>;
           const size_t shared = size_t(kOneThreads) * ITEMS * 6 + kOneThreads / 32 * kDigits * 6;
-          if (shared > 40 * 1024)
-            XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)));
+          allow_shared(kernel, shared, shared);
           const size_t e = type_size(out.type);
           const Rows rows{static_cast<char*>(const_cast<void*>(out.data)), out.stride * int64_t(e), uint32_t(dim * e),
                           uint32_t(e), bulk_rows(out, vocab, dim)};
@@ -1049,8 +1051,7 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
       if (n <= kFewTokens) {
         const FewPlan plan(n, vocab, pieces, VE, bulk);
         const auto kernel = s.data ? few_kernel<T, O, VE, true> : few_kernel<T, O, VE, false>;
-        if (plan.shared > 40 * 1024)
-          XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan.shared)));
+        allow_shared(kernel, plan.shared, FewPlan::kMostShared);
         kernel<<<dim3(plan.blocks, plan.tiles), kFewThreads, plan.shared, stream>>>(
             g, grad.stride, src, n, FastDiv(plan.blocks), s, scale, uint32_t(dim), y, out.stride, accumulate, bulk,
             plan.lg);

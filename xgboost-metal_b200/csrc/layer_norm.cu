@@ -817,12 +817,14 @@ void with_norm_width(std::initializer_list<Mat> mats, std::initializer_list<cons
   else f(std::integral_constant<int, 1>());
 }
 
+// What a launch may ask for: the stream kernels' ring, at its largest.
+constexpr size_t kMostShared = 128 * 1024;
+
 // Launches a kernel with more shared memory than a launch has unasked.
 template <class... Params, class... Args>
 void launch_ring(void (*kernel)(Params...), unsigned blocks, unsigned threads, size_t shared, cudaStream_t stream,
                  Args... args) {
-  if (shared > 40 * 1024)
-    XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)));
+  allow_shared(kernel, shared, kMostShared);
   kernel<<<blocks, threads, shared, stream>>>(args...);
 }
 
@@ -830,8 +832,7 @@ void launch_ring(void (*kernel)(Params...), unsigned blocks, unsigned threads, s
 template <class... Params, class... Args>
 void launch_cluster(void (*kernel)(Params...), unsigned blocks, unsigned threads, unsigned cluster, size_t shared,
                     cudaStream_t stream, Args... args) {
-  if (shared > 40 * 1024)
-    XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)));
+  allow_shared(kernel, shared, kMostShared);
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeClusterDimension;
   attribute.val.clusterDim = {cluster, 1, 1};

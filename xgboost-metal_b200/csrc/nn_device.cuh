@@ -239,6 +239,17 @@ inline int lanes_log2(uint64_t pieces) {
   return lg;
 }
 
+// Lets a kernel be launched with `shared` bytes of dynamic shared memory. The
+// limit belongs to the kernel on its device and not to one launch, so every call
+// sets the same one, the `most` that any launch of the kernel asks for: another
+// host thread's launch may come between this and the caller's.
+template <class... Params>
+void allow_shared(void (*kernel)(Params...), size_t shared, size_t most) {
+  require(shared <= most, "a launch asks for more shared memory than its kernel allows");
+  if (shared > 40 * 1024)
+    XGBB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most)));
+}
+
 inline unsigned blocks_for(uint64_t work, uint64_t per_block) {
   return unsigned((work + per_block - 1) / per_block);
 }
