@@ -1,6 +1,8 @@
 """What xgboost.nn's Python layer makes of the arrays that it is given: their
 devices, streams and flags. Without a GPU: tensors are stand-ins with torch's
 methods, and what would be handed to the library is recorded instead."""
+import sys
+
 import pytest
 import torch
 
@@ -52,3 +54,21 @@ def test_a_workspace_on_another_device_is_refused():
     with pytest.raises(xgb.XGBoostError, match="different devices"):
         nn.layer_norm_backward(x, x, stats, stats, w, out=Tensor(3, 400, ptr=8192), dweight=Tensor(400),
                                dbias=Tensor(400), workspace=space)
+
+
+def test_torch_counts_as_known_only_when_all_of_it_is(monkeypatch):
+    """_codes is what other threads look at: nothing may still be missing when it is filled."""
+    codes, dtypes = {}, {}
+    for name, value in (("_codes", codes), ("_dtypes", dtypes), ("_raw_stream", None), ("_empty_like", None)):
+        monkeypatch.setattr(nn, name, value)
+    seen = []
+
+    class Torch:
+        def __getattr__(self, name):  # where another thread may come in between
+            seen.append(name)
+            assert not codes or (dtypes and nn._raw_stream and nn._empty_like), name
+            return getattr(torch, name)
+
+    monkeypatch.setitem(sys.modules, "torch", Torch())
+    nn._know_torch()
+    assert "_C" in seen and len(codes) == len(dtypes) == 5 and nn._raw_stream and nn._empty_like

@@ -60,10 +60,11 @@ def _know_torch():
     global _raw_stream, _empty_like
     t = sys.modules["torch"]
     _empty_like = t.empty_like
-    _codes.update({t.float32: _F32, t.float16: _F16, t.bfloat16: _BF16, t.int32: _I32, t.int64: _I64})
-    _dtypes.update({c: d for d, c in _codes.items()})
     _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or \
         (lambda device: t.cuda.current_stream(device).cuda_stream)
+    codes = {t.float32: _F32, t.float16: _F16, t.bfloat16: _BF16, t.int32: _I32, t.int64: _I64}
+    _dtypes.update({c: d for d, c in codes.items()})
+    _codes.update(codes)  # last: other threads take it that all is known
 
 
 def _call(function, args):
