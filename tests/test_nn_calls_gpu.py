@@ -1,5 +1,5 @@
 """How xgboost.nn's calls go with one another and with the arrays' producers, on
-the GPU: host threads, streams."""
+the GPU: host threads, streams; and the widest rows."""
 import threading
 
 import pytest
@@ -75,3 +75,19 @@ def test_threads_with_rows_of_different_lengths():
         R.close(y, R.norm(x, w)[0])
         for got, want in zip((dx, dw, db), R.norm_grad(x, x, mean, rstd, w)):
             R.close(got, want)
+
+
+# More tiles of 8 and of 16 lanes than a grid has in y, 65535.
+@pytest.mark.parametrize("dim", [524290, 1048561])
+def test_rows_of_more_tiles_than_a_grid_has(dim):
+    table = torch.arange(3 * dim, device=DEV, dtype=F32).reshape(3, dim) % 1024  # sums below are whole numbers
+    tokens = torch.tensor([[0, 2], [1, -1], [2, 2]], device=DEV)
+    want = torch.stack((table[0] + table[2], table[1], 2 * table[2]))
+    assert torch.equal(nn.embedding(tokens, table, bag=True), want)
+    assert torch.equal(nn.embedding_scale_backward(torch.ones(3, 1, device=DEV).expand(3, dim).contiguous(), tokens,
+                                                   torch.ones_like(table), bag=True),
+                       torch.tensor([[dim, dim], [dim, 0], [dim, dim]], device=DEV, dtype=F32))
+    for n in (5, 8200):  # one row's gradient for all tokens
+        k = torch.arange(n, device=DEV) % 2
+        got = nn.embedding_backward(table[:1].expand(n, dim), k, 3)
+        assert torch.equal(got, table[:1] * torch.tensor([[n - n // 2], [n // 2], [0]], device=DEV))

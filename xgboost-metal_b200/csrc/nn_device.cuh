@@ -231,11 +231,13 @@ inline bool row_aligned(const void* p, int64_t stride, uint64_t rows, size_t siz
 // log2 of the lanes that own a row of `pieces` or a tile of it: up to 8 lanes as
 // many as it takes, else as many of 8, 16 and 32 as leave no more lanes idle in
 // the last tile than 8 would. (33 columns in two tiles of 32 lanes took bags of
-// 100 tokens 137 us where five tiles of 8 take 104.)
+// 100 tokens 137 us where five tiles of 8 take 104.) And as many as leave no more
+// tiles than a grid has in y, whatever lanes are idle.
 inline int lanes_log2(uint64_t pieces) {
+  constexpr uint64_t kTiles = 65535;
   int lg = 0;
   while (lg < 3 && (1ull << lg) < pieces) ++lg;
-  while (lg >= 3 && lg < 5 && ((pieces + 7) / 8 * 8) % (2ull << lg) == 0) ++lg;
+  while (lg >= 3 && lg < 5 && (((pieces + 7) / 8 * 8) % (2ull << lg) == 0 || pieces > kTiles << lg)) ++lg;
   return lg;
 }
 
