@@ -1,6 +1,7 @@
 """What xgboost.nn's Python layer makes of the arrays that it is given: their
 devices, streams and flags. Without a GPU: tensors are stand-ins with torch's
 methods, and what would be handed to the library is recorded instead."""
+import struct
 import sys
 
 import pytest
@@ -72,3 +73,96 @@ def test_torch_counts_as_known_only_when_all_of_it_is(monkeypatch):
     monkeypatch.setitem(sys.modules, "torch", Torch())
     nn._know_torch()
     assert "_C" in seen and len(codes) == len(dtypes) == 5 and nn._raw_stream and nn._empty_like
+
+
+class Array:
+    """A device array by its interface alone; nothing reads its memory."""
+
+    def __init__(self, *shape, typestr="<f4", ptr=1 << 16, read_only=False, **more):
+        self.__cuda_array_interface__ = {"data": (ptr, read_only), "shape": shape, "typestr": typestr, "version": 3,
+                                         **more}
+
+
+@pytest.fixture
+def enqueued(monkeypatch):
+    """The library's calls in their order, (name, arguments), none of which is made. Torch's current stream is 77."""
+    calls = []
+    nn._codes or nn._know_torch()
+    monkeypatch.setattr(nn, "_call", lambda function, args: calls.append((function.__name__, args)))
+    monkeypatch.setattr(nn, "_raw_stream", lambda device: 77)
+    return calls
+
+
+FORMS = {"XGBBEmbedding": ("PPQQqqqqifPPPQQqqiii4x", 12), "XGBBEmbeddingBackward": ("PPQQqqqqifPPPPNQQqqiiii", 13),
+         "XGBBEmbeddingScaleBackward": ("PPQQqqqqifPPPPQQqqiii4x", 13), "XGBBLayerNorm": ("PPPPPPPQQqqiiif", 6),
+         "XGBBLayerNormBackward": ("PPPPPPPPPPNQQqqqiii4x", 9)}
+
+
+def _stream(call):
+    form, at = FORMS[call[0]]
+    return struct.unpack("@" + form, call[1])[at]
+
+
+def _calls(kind, at, **more):
+    """Every operator with arrays of which all are plain but number `at`, a tensor of the given kind."""
+    def make(i, *shape, typestr="<f4", dtype=torch.float32):
+        return kind(*shape, dtype=dtype) if i == at else Array(*shape, typestr=typestr, ptr=(i + 1) << 16)
+
+    def tokens(i):
+        return make(i, 3, 5, typestr="<i4", dtype=torch.int32)
+
+    yield lambda: nn.embedding(tokens(0), make(1, 4, 2), bag=True, token_scale=make(2, 3, 5), out=make(3, 3, 2), **more)
+    yield lambda: nn.embedding_backward(make(0, 3, 2), tokens(1), 4, bag=True, token_scale=make(2, 3, 5),
+                                        out=make(3, 4, 2), **more)
+    yield lambda: nn.embedding_scale_backward(make(0, 3, 2), tokens(1), make(2, 4, 2), bag=True, out=make(3, 3, 5),
+                                              **more)
+    yield lambda: nn.layer_norm(make(0, 3, 4), make(1, 4), make(2, 4), out=make(3, 3, 4), mean=make(4, 3),
+                                rstd=make(5, 3), **more)
+    yield lambda: nn.layer_norm_backward(make(0, 3, 4), make(1, 3, 4), make(2, 3), make(3, 3), make(4, 4),
+                                         out=make(5, 3, 4), dweight=make(6, 4), dbias=make(7, 4), **more)
+
+
+@pytest.mark.parametrize("at", range(8))
+def test_any_tensor_brings_torchs_current_stream(enqueued, at):
+    for call, count in zip(_calls(Tensor, at), (4, 4, 4, 6, 8)):
+        call()
+        assert _stream(enqueued[-1]) == (77 if at < count else 0)
+    for call in _calls(Tensor, None, stream=55):
+        call()
+        assert _stream(enqueued[-1]) == 55
+
+
+@pytest.mark.parametrize("at", range(8))
+def test_any_tensor_is_told_of_the_stream_that_is_given(enqueued, monkeypatch, at):
+    told = []
+
+    class Told(Tensor):
+        device = torch.device("cuda", 0)
+
+        def record_stream(self, stream):
+            told.append(stream)
+
+    class Stream:
+        device = torch.device("cuda", 0)
+        cuda_stream = 99
+
+        def __init__(self, handle, device):
+            assert handle == 99 and device == self.device
+
+    class Current:
+        def __init__(self, stream):
+            self.handle = stream.cuda_stream
+
+        def __enter__(self):
+            monkeypatch.setattr(nn, "_raw_stream", lambda device: self.handle)
+
+        def __exit__(self, *_):
+            monkeypatch.setattr(nn, "_raw_stream", lambda device: 77)
+
+    monkeypatch.setattr(torch.cuda, "ExternalStream", Stream)
+    monkeypatch.setattr(torch.cuda, "stream", Current)
+    for call, count in zip(_calls(Told, at, stream=99), (4, 4, 4, 6, 8)):
+        told.clear()
+        call()
+        assert _stream(enqueued[-1]) == 99
+        assert bool(told) == (at < count)

@@ -192,11 +192,16 @@ def _stream_handle(stream):
     return int(stream)
 
 
-def _handle(stream, device, v):
-    """The handle of the stream to use: torch's current one for tensors."""
-    if v[5] is not None:
+def _handle(stream, device):
+    """The handle of the stream to use: torch's current one where any array is a
+    tensor, as the device tells then."""
+    if device >= 0:
         return _raw_stream(device)
     return 0 if stream is None else _stream_handle(stream)
+
+
+def _tensors(*arrays):
+    return any(hasattr(a, "data_ptr") for a in arrays)
 
 
 @contextlib.contextmanager
@@ -492,7 +497,7 @@ def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None
     broadcasts to the tokens' shape. Sums are float32. The result has the
     table's type, or `out_dtype`; of the two types one is float32 or both are
     the same."""
-    if stream is not None and hasattr(table, "data_ptr"):
+    if stream is not None and _tensors(tokens, table, token_scale, out):
         with _on(stream, (tokens, table, token_scale, out)):
             return embedding(tokens, table, scale=scale, token_scale=token_scale, bag=bag, out=out,
                              out_dtype=out_dtype)
@@ -512,7 +517,7 @@ def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None
     device = _one_device(w[4], k[4], s_device, y_device)
     _call(_LIB.XGBBEmbedding, _pack_embedding(
         k[0], s, rows, per_row, stride_row, stride_col, s_row, s_col, k[3], scale, w[0], y,
-        _handle(stream, device, w), vocab, dim, table_stride, y_stride, w[3], code, device))
+        _handle(stream, device), vocab, dim, table_stride, y_stride, w[3], code, device))
     return out
 
 
@@ -531,7 +536,7 @@ def embedding_backward(grad, tokens, vocab, *, scale=1.0, token_scale=None, bag=
     gradient `grad`. Missing tokens and those past the table add nothing.
     With `accumulate` it is added to what `out` holds. It has grad's type, or
     `out_dtype`; of the two types one is float32 or both are the same."""
-    if stream is not None and hasattr(grad, "data_ptr"):
+    if stream is not None and _tensors(grad, tokens, token_scale, out, workspace):
         with _on(stream, (grad, tokens, token_scale, out, workspace)):
             return embedding_backward(grad, tokens, vocab, scale=scale, token_scale=token_scale, bag=bag, out=out,
                                       out_dtype=out_dtype, accumulate=accumulate, workspace=workspace)
@@ -557,7 +562,7 @@ def embedding_backward(grad, tokens, vocab, *, scale=1.0, token_scale=None, bag=
     device = _one_device(g[4], k[4], s_device, y_device, space_device)
     _call(_LIB.XGBBEmbeddingBackward, _pack_embedding_backward(
         k[0], s, rows, per_row, stride_row, stride_col, s_row, s_col, k[3], scale, g[0], y, space,
-        _handle(stream, device, g), size, vocab, dim, g_stride, y_stride, g[3], code, bool(accumulate), device))
+        _handle(stream, device), size, vocab, dim, g_stride, y_stride, g[3], code, bool(accumulate), device))
     return out
 
 
@@ -566,7 +571,7 @@ def embedding_scale_backward(grad, tokens, table, *, scale=1.0, bag=False, out=N
     for a missing token, NaN for one past the table. (Where token_scale was
     broadcast, its own gradient is this one's sum over the broadcast
     dimensions.)"""
-    if stream is not None and hasattr(grad, "data_ptr"):
+    if stream is not None and _tensors(grad, tokens, table, out):
         with _on(stream, (grad, tokens, table, out)):
             return embedding_scale_backward(grad, tokens, table, scale=scale, bag=bag, out=out)
     if out is None:
@@ -585,7 +590,7 @@ def embedding_scale_backward(grad, tokens, table, *, scale=1.0, bag=False, out=N
     device = _one_device(g[4], k[4], w[4], y_device)
     _call(_LIB.XGBBEmbeddingScaleBackward, _pack_embedding_scale_backward(
         k[0], 0, rows, per_row, stride_row, stride_col, 0, 0, k[3], scale, g[0], w[0], y,
-        _handle(stream, device, g), vocab, dim, g_stride, table_stride, g[3], w[3], device))
+        _handle(stream, device), vocab, dim, g_stride, table_stride, g[3], w[3], device))
     return out
 
 
@@ -594,7 +599,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
     * rstd * weight + bias in x's type, mean and rstd = 1 / sqrt(variance +
     eps) in float32, one a row. weight and bias have x's type or are float32,
     both the same."""
-    if stream is not None and hasattr(x, "data_ptr"):
+    if stream is not None and _tensors(x, weight, bias, out, mean, rstd):
         with _on(stream, (x, weight, bias, out, mean, rstd)):
             return layer_norm(x, weight, bias, eps=eps, out=out, mean=mean, rstd=rstd)
     if out is None and mean is None and rstd is None:
@@ -622,7 +627,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
     rstd, q, q_device = _flat_result(rstd, lead, _F32, v, "rstd")
     device = _one_device(v[4], w_device, b_device, y_device, m_device, q_device)
     _call(_LIB.XGBBLayerNorm, _pack_layer_norm(
-        v[0], w or 0, b or 0, y, m, q, _handle(stream, device, v), rows, dim, stride, y_stride, v[3], param, device,
+        v[0], w or 0, b or 0, y, m, q, _handle(stream, device), rows, dim, stride, y_stride, v[3], param, device,
         eps))
     return out, mean, rstd
 
@@ -641,7 +646,7 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
     """(dx, dweight, dbias) from the gradient `grad` of layer_norm's y and the
     mean and rstd that it returned. Without a weight (then y is the normalised
     x) dweight and dbias are None; without `bias_grad` dbias is None."""
-    if stream is not None and hasattr(grad, "data_ptr"):
+    if stream is not None and _tensors(grad, x, mean, rstd, weight, out, dweight, dbias, workspace):
         with _on(stream, (grad, x, mean, rstd, weight, out, dweight, dbias, workspace)):
             return layer_norm_backward(grad, x, mean, rstd, weight, bias_grad=bias_grad, out=out, dweight=dweight,
                                        dbias=dbias, workspace=workspace)
@@ -677,7 +682,7 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
         raise XGBoostError("dweight and dbias need weight")
     device = _one_device(v[4], g[4], m_device, q_device, w_device, dx_device, dw_device, db_device, space_device)
     _call(_LIB.XGBBLayerNormBackward, _pack_layer_norm_backward(
-        g[0], v[0], m, q, w, dx, dw, db, space, _handle(stream, device, v), size, rows, dim, g_stride, stride,
+        g[0], v[0], m, q, w, dx, dw, db, space, _handle(stream, device), size, rows, dim, g_stride, stride,
         dx_stride, v[3], w_code, device))
     return out, dweight, dbias
 
