@@ -166,3 +166,21 @@ def test_any_tensor_is_told_of_the_stream_that_is_given(enqueued, monkeypatch, a
         call()
         assert _stream(enqueued[-1]) == 99
         assert bool(told) == (at < count)
+
+
+def test_a_stream_of_another_device_is_refused(enqueued, monkeypatch):
+    class Stream:
+        device = torch.device("cuda", 1)
+
+    class There(Tensor):
+        device = torch.device("cuda", 0)
+
+        def record_stream(self, stream):
+            raise AssertionError("told of a stream that is not used")
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: pytest.fail("made current"))
+    for call in _calls(There, 1, stream=Stream()):
+        with pytest.raises(xgb.XGBoostError, match="another device"):
+            call()
+    assert not enqueued

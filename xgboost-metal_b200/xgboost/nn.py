@@ -219,6 +219,8 @@ def _on(stream, tensors):
     else:
         handle = _stream_handle(stream)
         s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    if s.device != device:
+        raise XGBoostError("stream is one of another device than the arrays'")
     with torch.cuda.stream(s):
         for t in tensors:
             t.record_stream(s)
