@@ -237,4 +237,11 @@ typedef struct {
 XGB_DLL int XGBBLayerNormBackwardWorkspace(bst_ulong rows, bst_ulong dim, size_t* bytes);
 XGB_DLL int XGBBLayerNormBackward(const XGBBLayerNormBackwardArgs* args);
 
+/* Work that is enqueued on `stream` from now on waits for what is on `after`
+ * now (both streams of `device`; -1: the calling thread's device; a null
+ * pointer is the default stream). Nothing is waited for here. While `stream` is
+ * being captured and `after` is not in the same capture, nothing is done: then
+ * the order is that of the graph's launch. */
+XGB_DLL int XGBBStreamWait(int32_t device, void* stream, void* after);
+
 #endif /* XGB_B200_EXTENSIONS_H_ */

@@ -103,10 +103,13 @@ def _stream(call):
     return struct.unpack("@" + form, call[1])[at]
 
 
-def _calls(kind, at, **more):
-    """Every operator with arrays of which all are plain but number `at`, a tensor of the given kind."""
+def _calls(kind, at, own={}, **more):
+    """Every operator with arrays of which all are plain but number `at`: a tensor of the given kind, or an array whose
+    interface has `own`."""
     def make(i, *shape, typestr="<f4", dtype=torch.float32):
-        return kind(*shape, dtype=dtype) if i == at else Array(*shape, typestr=typestr, ptr=(i + 1) << 16)
+        if i == at and kind is not Array:
+            return kind(*shape, dtype=dtype)
+        return Array(*shape, typestr=typestr, ptr=(i + 1) << 16, **(own if i == at else {}))
 
     def tokens(i):
         return make(i, 3, 5, typestr="<i4", dtype=torch.int32)
@@ -184,3 +187,18 @@ def test_a_stream_of_another_device_is_refused(enqueued, monkeypatch):
         with pytest.raises(xgb.XGBoostError, match="another device"):
             call()
     assert not enqueued
+
+
+@pytest.mark.parametrize("at", range(8))
+def test_the_stream_of_an_array_is_waited_for(enqueued, monkeypatch, at):
+    monkeypatch.setattr(nn._LIB, "XGBBStreamWait", lambda *args: enqueued.append(("wait", args)) or 0)
+    for call, count in zip(_calls(Array, at, dict(stream=99), stream=55), (4, 4, 4, 6, 8)):
+        enqueued.clear()
+        call()
+        assert [c[0] == "wait" for c in enqueued] == [True] * (at < count) + [False]
+        assert at >= count or enqueued[0][1] == (-1, 55, 99)
+    for same in (None, 55):
+        for call in _calls(Array, at, dict(stream=same), stream=55):
+            enqueued.clear()
+            call()
+            assert len(enqueued) == 1

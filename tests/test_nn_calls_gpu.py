@@ -91,3 +91,56 @@ def test_rows_of_more_tiles_than_a_grid_has(dim):
         k = torch.arange(n, device=DEV) % 2
         got = nn.embedding_backward(table[:1].expand(n, dim), k, 3)
         assert torch.equal(got, table[:1] * torch.tensor([[n - n // 2], [n // 2], [0]], device=DEV))
+
+
+class _Filled:
+    """A tensor by its interface alone, as one that is filled on a stream."""
+
+    def __init__(self, t, stream=None):
+        self.keep = t
+        self.__cuda_array_interface__ = {"data": (t.data_ptr(), False), "shape": tuple(t.shape), "version": 3,
+                                         "typestr": "<f4", "strides": None, "stream": stream}
+
+
+def test_arrays_that_are_filled_on_another_stream():
+    x, y, mean, rstd = (torch.zeros(s, device=DEV) for s in ((64, 96), (64, 96), 64, 64))
+    filled = torch.randn(64, 96, generator=torch.Generator().manual_seed(3)).to(DEV)
+    producer, consumer = torch.cuda.Stream(DEV), torch.cuda.Stream(DEV)
+
+    def call(stream):
+        out = [_Filled(t) for t in (y, mean, rstd)]
+        nn.layer_norm(_Filled(x, producer.cuda_stream), out=out[0], mean=out[1], rstd=out[2], stream=stream)
+
+    for stream in (0, consumer.cuda_stream, producer.cuda_stream):
+        x.zero_()
+        y.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(producer):
+            torch.cuda._sleep(50_000_000)  # 25 to 50 ms
+            x.copy_(filled)
+        call(stream)
+        torch.cuda.synchronize()
+        R.close(y, R.norm(filled)[0])
+    # In a capture: of a stream that is none of it, nothing is recorded; of one that is, the order.
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=consumer):
+        call(consumer.cuda_stream)
+    y.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    R.close(y, R.norm(filled)[0])
+    other = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other, stream=consumer):
+        producer.wait_stream(consumer)
+        with torch.cuda.stream(producer):
+            torch.cuda._sleep(50_000_000)
+            x.copy_(filled)
+        call(consumer.cuda_stream)
+        consumer.wait_stream(producer)
+    for _ in range(2):
+        x.zero_()
+        y.zero_()
+        torch.cuda.synchronize()
+        other.replay()
+        torch.cuda.synchronize()
+        R.close(y, R.norm(filled)[0])

@@ -33,6 +33,31 @@ class OnDevice {
   int back_ = -1;
 };
 
+// The default stream has two handles.
+bool is_default(cudaStream_t s) { return s == nullptr || s == cudaStreamLegacy; }
+
+// The capture that a stream is in, 0 for none. The default stream is in none,
+// and may not be asked during one.
+unsigned long long capture_of(cudaStream_t s) {
+  if (is_default(s)) return 0;
+  cudaStreamCaptureStatus status;
+  unsigned long long id = 0;
+  XGBB_CUDA(cudaStreamGetCaptureInfo(s, &status, &id));
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
+void stream_wait(cudaStream_t stream, cudaStream_t after) {
+  if (stream == after || (is_default(stream) && is_default(after))) return;
+  const unsigned long long capture = capture_of(stream);
+  if (capture && capture_of(after) != capture) return;
+  cudaEvent_t event;
+  XGBB_CUDA(cudaEventCreateWithFlags(&event, cudaEventDisableTiming));
+  cudaError_t e = cudaEventRecord(event, after);
+  if (e == cudaSuccess) e = cudaStreamWaitEvent(stream, event, 0);
+  cudaEventDestroy(event);  // freed once it is done
+  xgbb::cuda_check(e, "cudaStreamWaitEvent");
+}
+
 bool is_float(int t) { return t == nn::kF32 || t == nn::kF16 || t == nn::kBF16; }
 
 void require_pointer(const void* p, size_t align, const char* what) {
@@ -205,5 +230,12 @@ XGB_DLL int XGBBLayerNormBackward(const XGBBLayerNormBackwardArgs* args) {
     const OnDevice on(a.device);
     nn::layer_norm_backward(g, in, a.mean, a.rstd, a.rows, a.dim, a.weight, a.param_type, out, a.dweight, a.dbias,
                             a.workspace, static_cast<cudaStream_t>(a.stream));
+  });
+}
+
+XGB_DLL int XGBBStreamWait(int32_t device, void* stream, void* after) {
+  return guarded([&] {
+    const OnDevice on(device);
+    stream_wait(static_cast<cudaStream_t>(stream), static_cast<cudaStream_t>(after));
   });
 }

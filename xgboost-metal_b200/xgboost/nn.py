@@ -16,8 +16,9 @@ any stride; the values of a row are contiguous.
 
 Work is enqueued and not waited for: on `stream` where one is given (a handle,
 or an object that has one as `cuda_stream` or `ptr`), else on torch's current
-stream of the arrays' device, or the default stream for other arrays. Equal
-inputs give equal bits. These functions have no counterpart in the reference.
+stream of the arrays' device where one of them is a tensor, else on the default
+stream. It runs after what is enqueued on the streams that the arrays'
+interfaces name. Equal inputs give equal bits. These functions have no counterpart in the reference.
 """
 import contextlib
 import ctypes
@@ -50,6 +51,7 @@ for _name in ("XGBBEmbedding", "XGBBEmbeddingBackward", "XGBBEmbeddingScaleBackw
 _SIZES = [ctypes.c_uint64] * 4
 _LIB.XGBBEmbeddingBackwardWorkspace.argtypes = _SIZES + [ctypes.c_void_p]
 _LIB.XGBBLayerNormBackwardWorkspace.argtypes = _SIZES[:2] + [ctypes.c_void_p]
+_LIB.XGBBStreamWait.argtypes = [ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
 
 _TYPESTR = {"<f4": _F32, "<f2": _F16, "<i4": _I32, "<i8": _I64}
 _codes, _dtypes = {}, {}  # torch's dtypes by code and back, filled when the first tensor comes
@@ -192,12 +194,22 @@ def _stream_handle(stream):
     return int(stream)
 
 
-def _handle(stream, device):
+def _handle(stream, device, *arrays):
     """The handle of the stream to use: torch's current one where any array is a
-    tensor, as the device tells then."""
+    tensor, as the device tells then. It waits for the streams that the arrays'
+    interfaces name, where their producers may still be at work."""
     if device >= 0:
-        return _raw_stream(device)
-    return 0 if stream is None else _stream_handle(stream)
+        handle = _raw_stream(device)
+    else:
+        handle = 0 if stream is None else _stream_handle(stream)
+    waited = {None, handle}
+    for a in arrays:
+        if a is not None and not hasattr(a, "data_ptr"):
+            after = a.__cuda_array_interface__.get("stream")
+            if after not in waited:
+                waited.add(after)
+                _check_call(_LIB.XGBBStreamWait(device, handle, after))
+    return handle
 
 
 def _tensors(*arrays):
@@ -517,9 +529,10 @@ def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None
     out, y, code, y_stride, y_device = _result(out, (*lead, dim), 0 if out is not None and out_dtype is None else code,
                                                w, "out")
     device = _one_device(w[4], k[4], s_device, y_device)
+    handle = _handle(stream, device, tokens, table, token_scale, out)
     _call(_LIB.XGBBEmbedding, _pack_embedding(
         k[0], s, rows, per_row, stride_row, stride_col, s_row, s_col, k[3], scale, w[0], y,
-        _handle(stream, device), vocab, dim, table_stride, y_stride, w[3], code, device))
+        handle, vocab, dim, table_stride, y_stride, w[3], code, device))
     return out
 
 
@@ -562,9 +575,10 @@ def embedding_backward(grad, tokens, vocab, *, scale=1.0, token_scale=None, bag=
     if size:
         workspace, space, space_device = _space(workspace, size, g)
     device = _one_device(g[4], k[4], s_device, y_device, space_device)
+    handle = _handle(stream, device, grad, tokens, token_scale, out, workspace)
     _call(_LIB.XGBBEmbeddingBackward, _pack_embedding_backward(
         k[0], s, rows, per_row, stride_row, stride_col, s_row, s_col, k[3], scale, g[0], y, space,
-        _handle(stream, device), size, vocab, dim, g_stride, y_stride, g[3], code, bool(accumulate), device))
+        handle, size, vocab, dim, g_stride, y_stride, g[3], code, bool(accumulate), device))
     return out
 
 
@@ -590,9 +604,10 @@ def embedding_scale_backward(grad, tokens, table, *, scale=1.0, bag=False, out=N
         raise XGBoostError("grad must have the shape of the lookup's result")
     out, y, y_device = _flat_result(out, k[1], _F32, g, "out")
     device = _one_device(g[4], k[4], w[4], y_device)
+    handle = _handle(stream, device, grad, tokens, table, out)
     _call(_LIB.XGBBEmbeddingScaleBackward, _pack_embedding_scale_backward(
         k[0], 0, rows, per_row, stride_row, stride_col, 0, 0, k[3], scale, g[0], w[0], y,
-        _handle(stream, device), vocab, dim, g_stride, table_stride, g[3], w[3], device))
+        handle, vocab, dim, g_stride, table_stride, g[3], w[3], device))
     return out
 
 
@@ -628,8 +643,9 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
     mean, m, m_device = _flat_result(mean, lead, _F32, v, "mean")
     rstd, q, q_device = _flat_result(rstd, lead, _F32, v, "rstd")
     device = _one_device(v[4], w_device, b_device, y_device, m_device, q_device)
+    handle = _handle(stream, device, x, weight, bias, out, mean, rstd)
     _call(_LIB.XGBBLayerNorm, _pack_layer_norm(
-        v[0], w or 0, b or 0, y, m, q, _handle(stream, device), rows, dim, stride, y_stride, v[3], param, device,
+        v[0], w or 0, b or 0, y, m, q, handle, rows, dim, stride, y_stride, v[3], param, device,
         eps))
     return out, mean, rstd
 
@@ -683,8 +699,9 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
     elif dweight is not None or dbias is not None:
         raise XGBoostError("dweight and dbias need weight")
     device = _one_device(v[4], g[4], m_device, q_device, w_device, dx_device, dw_device, db_device, space_device)
+    handle = _handle(stream, device, grad, x, mean, rstd, weight, out, dweight, dbias, workspace)
     _call(_LIB.XGBBLayerNormBackward, _pack_layer_norm_backward(
-        g[0], v[0], m, q, w, dx, dw, db, space, _handle(stream, device), size, rows, dim, g_stride, stride,
+        g[0], v[0], m, q, w, dx, dw, db, space, handle, size, rows, dim, g_stride, stride,
         dx_stride, v[3], w_code, device))
     return out, dweight, dbias
 
