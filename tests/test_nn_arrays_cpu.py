@@ -202,3 +202,21 @@ def test_the_stream_of_an_array_is_waited_for(enqueued, monkeypatch, at):
             enqueued.clear()
             call()
             assert len(enqueued) == 1
+
+
+def test_results_are_not_written_to_read_only_arrays(enqueued):
+    firsts = (3, 3, 3, 3, 5)  # of the results, the last arrays of a call
+    for at in range(8):
+        for call, first, count in zip(_calls(Array, at, dict(read_only=True)), firsts, (4, 4, 4, 6, 8)):
+            enqueued.clear()
+            if first <= at < count:
+                with pytest.raises(xgb.XGBoostError, match="read-only"):
+                    call()
+                assert not enqueued
+            else:
+                call()
+                assert enqueued
+    n = 1 << 14
+    space = Array(nn.embedding_backward_workspace(n, 1, 4, 2), typestr="|u1", ptr=1 << 20, read_only=True)
+    with pytest.raises(xgb.XGBoostError, match="workspace is read-only"):
+        nn.embedding_backward(Array(n, 2), Array(n, typestr="<i4"), 4, out=Array(4, 2, ptr=8192), workspace=space)

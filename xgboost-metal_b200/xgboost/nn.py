@@ -74,13 +74,13 @@ def _call(function, args):
         _check_call(-1)
 
 
-def _view(a, what):
+def _view(a, what, written=False):
     """What a call needs of an array: (pointer, shape, strides in elements,
     dtype code, device ordinal or -1 for the current one, the tensor or None)."""
     try:
         ptr = a.data_ptr()
     except AttributeError:
-        return _interface_view(a, what)
+        return _interface_view(a, what, written)
     if not a.is_cuda:
         raise XGBoostError("%s must be in device memory" % what)
     if not _codes:
@@ -88,13 +88,15 @@ def _view(a, what):
     return ptr, a.shape, a.stride(), _codes.get(a.dtype, 0), a.get_device(), a
 
 
-def _interface_view(a, what):
+def _interface_view(a, what, written):
     inf = getattr(a, "__cuda_array_interface__", None)
     if inf is None:
         raise XGBoostError("%s must be a device array: a CUDA tensor, or an object with a "
                            "__cuda_array_interface__" % what)
     if inf.get("mask") is not None:
         raise XGBoostError("%s must not be masked" % what)
+    if written and inf["data"][1]:
+        raise XGBoostError("%s is read-only" % what)
     shape, size = tuple(inf["shape"]), int(inf["typestr"][2:])
     if inf.get("strides") is None:
         strides, step = [], 1
@@ -271,7 +273,7 @@ def _result(out, shape, code, like, what):
     if out is None:
         out, ptr = _new(shape, code, like, what)
         return out, ptr, code, shape[-1] if shape else 1, like[4]
-    v = _view(out, what)
+    v = _view(out, what, True)
     if tuple(v[1]) != tuple(shape):
         raise XGBoostError("%s must have the shape %s" % (what, tuple(shape)))
     if code and v[3] != code:
@@ -284,7 +286,7 @@ def _flat_result(out, shape, code, like, what):
     if out is None:
         out, ptr = _new(shape, code, like, what)
         return out, ptr, like[4]
-    v = _view(out, what)
+    v = _view(out, what, True)
     if tuple(v[1]) != tuple(shape):
         raise XGBoostError("%s must have the shape %s" % (what, tuple(shape)))
     if v[3] != code:
@@ -326,7 +328,7 @@ def _space(workspace, size, like):
             raise XGBoostError("workspace must be given where the inputs are no tensors")
         workspace = like[5].new_empty(size, dtype=sys.modules["torch"].uint8)
         return workspace, workspace.data_ptr(), like[4]
-    v = _view(workspace, "workspace")
+    v = _view(workspace, "workspace", True)
     n, stride = _flat(v[1], v[2], "workspace")
     width = v[5].element_size() if v[5] is not None else int(workspace.__cuda_array_interface__["typestr"][2:])
     if n * width < size or (n > 1 and stride != 1):
