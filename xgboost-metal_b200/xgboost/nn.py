@@ -664,8 +664,9 @@ def layer_norm_backward_workspace(rows, dim):
 def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out=None, dweight=None, dbias=None,
                         workspace=None, stream=None):
     """(dx, dweight, dbias) from the gradient `grad` of layer_norm's y and the
-    mean and rstd that it returned. Without a weight (then y is the normalised
-    x) dweight and dbias are None; without `bias_grad` dbias is None."""
+    mean and rstd that it returned. Without a weight dweight is None, and dbias
+    too where no array for it is given (float32 or of x's type); without
+    `bias_grad` dbias is None."""
     if stream is not None and _tensors(grad, x, mean, rstd, weight, out, dweight, dbias, workspace):
         with _on(stream, (grad, x, mean, rstd, weight, out, dweight, dbias, workspace)):
             return layer_norm_backward(grad, x, mean, rstd, weight, bias_grad=bias_grad, out=out, dweight=dweight,
@@ -695,11 +696,15 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, bias_grad=True, out
         dweight, dw, dw_device = _flat_result(dweight, (dim,), w_code, wv, "dweight")
         if bias_grad:
             dbias, db, db_device = _flat_result(dbias, (dim,), w_code, wv, "dbias")
+    elif dweight is not None:
+        raise XGBoostError("dweight would need weight")
+    elif dbias is not None and bias_grad:
+        w_code = _F32 if _view(dbias, "dbias")[3] == _F32 else v[3]
+        dbias, db, db_device = _flat_result(dbias, (dim,), w_code, v, "dbias")
+    if dw or db:
         size = layer_norm_backward_workspace(rows, dim)
         if size:
             workspace, space, space_device = _space(workspace, size, v)
-    elif dweight is not None or dbias is not None:
-        raise XGBoostError("dweight and dbias need weight")
     device = _one_device(v[4], g[4], m_device, q_device, w_device, dx_device, dw_device, db_device, space_device)
     handle = _handle(stream, device, grad, x, mean, rstd, weight, out, dweight, dbias, workspace)
     _call(_LIB.XGBBLayerNormBackward, _pack_layer_norm_backward(
