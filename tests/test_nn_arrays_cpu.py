@@ -14,7 +14,7 @@ from xgboost import nn
 class Tensor:
     """A contiguous CUDA tensor by its methods; nothing reads its memory."""
 
-    is_cuda = True
+    is_cuda, requires_grad = True, False
 
     def __init__(self, *shape, dtype=torch.float32, device=0, ptr=4096):
         self.shape, self.dtype, self.ordinal, self.ptr = torch.Size(shape), dtype, device, ptr
@@ -220,3 +220,22 @@ def test_results_are_not_written_to_read_only_arrays(enqueued):
     space = Array(nn.embedding_backward_workspace(n, 1, 4, 2), typestr="|u1", ptr=1 << 20, read_only=True)
     with pytest.raises(xgb.XGBoostError, match="workspace is read-only"):
         nn.embedding_backward(Array(n, 2), Array(n, typestr="<i4"), 4, out=Array(4, 2, ptr=8192), workspace=space)
+
+
+def test_what_takes_no_part_in_automatic_differentiation(enqueued):
+    class Leaf(Tensor):
+        requires_grad = True
+
+    refused = [call for i, call in enumerate(_calls(Leaf, 1)) if i in (0, 3)]  # the table, the norm's weight
+    for call in refused:
+        with pytest.raises(xgb.XGBoostError, match="automatic differentiation"):
+            call()
+    with pytest.raises(xgb.XGBoostError, match="differentiation needs tensors"):
+        nn.embedding(Array(3, typestr="<i4"), Leaf(4, 2))
+    with pytest.raises(xgb.XGBoostError, match="differentiation needs tensors"):
+        nn.layer_norm(Leaf(3, 4), Array(4))
+    assert not enqueued
+    with torch.no_grad():
+        for call in refused:
+            call()
+    assert len(enqueued) == 2

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import nn_reference as R
+import xgboost as xgb
 from xgboost import nn
 
 pytestmark = pytest.mark.gpu
@@ -30,3 +31,79 @@ def test_bias_without_a_weight(rows, dim, a, p):
     R.close(dx, want[0], "dx")
     R.close(db, want[2], "dbias")
     assert nn.layer_norm_backward(grad, x, mean, rstd)[1:] == (None, None)
+
+
+@pytest.mark.parametrize("a,b", [(F32, F32), (BF16, F32), (F16, F16)])
+@pytest.mark.parametrize("scales", [None, (30, 12), (12,), (30, 1)])
+def test_autograd_of_bags(a, b, scales):
+    g = torch.Generator().manual_seed(5)
+    tokens = torch.randint(-1, 90, (30, 12), generator=g).to(DEV)
+    table, grad = _randn(g, 90, 20, dtype=a).requires_grad_(), _randn(g, 20, 30, dtype=b).t()  # no contiguous rows
+    s = None if scales is None else _randn(g, *scales).requires_grad_()
+    y = nn.embedding(tokens, table, scale=0.7, token_scale=s, bag=True, out_dtype=b)
+    R.close(y.detach(), R.bag(tokens, table.detach(), 0.7, None if s is None else s.detach(), b))
+    y.backward(grad)
+    R.close(table.grad, R.bag_grad(grad, tokens, 90, 0.7, None if s is None else s.detach(), a), "dtable")
+    if s is not None:
+        value, bound = R.scale_grad(grad, tokens, table.detach(), 0.7)
+        # A broadcast scale's gradient is torch's float32 sum of at most 30 of these.
+        for i in (0, 1):
+            if s.numel() < 360 and (2 - i > s.dim() or s.shape[i - 2] == 1):
+                error = 30 * R.U * (value.abs() + bound).sum(i, keepdim=True)
+                value, bound = value.sum(i, keepdim=True), bound.sum(i, keepdim=True) + error
+        R.close(s.grad, (value.reshape(s.shape), bound.reshape(s.shape)), "dscale")
+
+
+@pytest.mark.parametrize("which", ["x", "w", "b", "xwb", "xw", "xb"])
+@pytest.mark.parametrize("a,p", [(F32, F32), (BF16, F32), (F16, F16)])
+def test_autograd_of_the_norm(which, a, p):
+    g = torch.Generator().manual_seed(6)
+    x, w, b = _randn(g, 30, 70, dtype=a), _randn(g, 70, dtype=p), _randn(g, 70, dtype=p)
+    grad = _randn(g, 70, 30, dtype=a).t()
+    if which == "xb":
+        w = None
+    for name, t in (("x", x), ("w", w), ("b", b)):
+        if name in which:
+            t.requires_grad_()
+    y, mean, rstd = nn.layer_norm(x, w, b)
+    assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
+    y.backward(grad)
+    wants = R.norm_grad(grad, x.detach(), mean, rstd, None if w is None else w.detach(), p)
+    for name, t, want in zip("xwb", (x, w, b), wants):
+        if name in which:
+            R.close(t.grad, want, name)
+        else:
+            assert t is None or t.grad is None
+
+
+def test_autograd_on_another_stream_and_its_refusals():
+    g = torch.Generator().manual_seed(7)
+    tokens, table = torch.randint(0, 40, (200, 5), generator=g).to(DEV), _randn(g, 40, 16).requires_grad_()
+    w, grad = _randn(g, 16).requires_grad_(), _randn(g, 200, 16)
+
+    def run(stream=None):
+        table.grad = w.grad = None
+        y = nn.layer_norm(nn.embedding(tokens, table, bag=True, stream=stream), w, stream=stream)[0]
+        if stream is not None:
+            torch.cuda.current_stream().wait_stream(stream)
+        y.backward(grad)
+        return y.detach(), table.grad, w.grad
+
+    want, stream = run(), torch.cuda.Stream(DEV)
+    torch.cuda.synchronize()
+    got = run(stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, u) for v, u in zip(got, want))
+    with torch.no_grad():  # nothing is recorded, and results may be given
+        out = torch.empty(200, 16, device=DEV)
+        assert nn.embedding(tokens, table, bag=True, out=out) is out
+        y = nn.layer_norm(out, w)[0]
+        assert torch.equal(y, want[0]) and not y.requires_grad
+    with pytest.raises(xgb.XGBoostError, match="automatic differentiation"):
+        nn.embedding(tokens, table, bag=True, out=out)
+    with pytest.raises(xgb.XGBoostError, match="automatic differentiation"):
+        nn.layer_norm(out, w, mean=torch.empty(200, device=DEV))
+    x = torch.ones(3, 4, device=DEV, requires_grad=True)
+    dx, = torch.autograd.grad(nn.layer_norm(x)[0].sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):  # not differentiated again
+        dx.sum().backward()

@@ -8,7 +8,8 @@ each token has a learned vector:
     y, mean, rstd = xgboost.nn.layer_norm(h, weight, bias)
 
 with the gradients `embedding_backward`, `embedding_scale_backward` and
-`layer_norm_backward`. Arrays are device memory: tensors with torch's methods
+`layer_norm_backward`, which torch's autograd calls too (once: their results are
+not differentiated). Arrays are device memory: tensors with torch's methods
 (`data_ptr`, `stride`, `new_empty`), or any object with a
 `__cuda_array_interface__`, whose outputs and workspaces the caller passes in.
 Values are float32, float16 or bfloat16, tokens int32 or int64. Rows may have
@@ -159,16 +160,22 @@ def _token_grid(v, bag):
     return rows, shape[-1], stride, strides[-1], shape[:-1]
 
 
+def _expand(scale, shape):
+    """token_scale broadcast to the tokens' shape, where it can tell how."""
+    if hasattr(scale, "expand") and scale.shape != shape:
+        try:
+            return scale.expand(shape)
+        except RuntimeError as e:
+            raise XGBoostError("token_scale does not broadcast to the tokens' shape: %s" % e) from None
+    return scale
+
+
 def _scale_grid(scale, tokens, bag):
     """(pointer, row stride, column stride, device) of token_scale, broadcast to
     the tokens' shape."""
     if scale is None:
         return 0, 0, 0, -1
-    if hasattr(scale, "expand") and scale.shape != tokens[1]:
-        try:
-            scale = scale.expand(tokens[1])
-        except RuntimeError as e:
-            raise XGBoostError("token_scale does not broadcast to the tokens' shape: %s" % e) from None
+    scale = _expand(scale, tokens[1])
     ptr, shape, strides, code, device, _ = _view(scale, "token_scale")
     if tuple(shape) != tuple(tokens[1]):
         raise XGBoostError("token_scale must have the tokens' shape")
@@ -336,6 +343,80 @@ def _space(workspace, size, like):
     return workspace, v[0], v[4]
 
 
+# Automatic differentiation. The library's gradients, not torch's, run backward:
+# what they give is not differentiated again.
+
+
+def _tracked(*arrays):
+    """Whether torch records what is done with one of them."""
+    for a in arrays:
+        if getattr(a, "requires_grad", False):
+            return sys.modules["torch"].is_grad_enabled()
+    return False
+
+
+def _recorded(function, arrays, results, *rest):
+    """A call that torch records, of arrays that are all tensors, if any; `results`
+    that the caller brings would not be part of the record."""
+    if any(r is not None for r in results):
+        raise XGBoostError("results that are given take no part in automatic differentiation: "
+                           "call with torch.no_grad() or with detached inputs")
+    if not all(a is None or hasattr(a, "requires_grad") for a in arrays):
+        raise XGBoostError("automatic differentiation needs tensors: "
+                           "call with torch.no_grad() or with detached inputs")
+    return _functions()[function].apply(*arrays, *rest)
+
+
+@functools.lru_cache(maxsize=None)
+def _functions():
+    from torch.autograd import Function
+    from torch.autograd.function import once_differentiable
+
+    class Embedding(Function):
+        @staticmethod
+        def forward(ctx, tokens, table, token_scale, scale, bag, out_dtype):
+            ctx.save_for_backward(tokens, table if ctx.needs_input_grad[2] else None, token_scale)
+            ctx.rest = scale, bag, table.shape[0], table.dtype
+            return embedding(tokens, table, scale=scale, token_scale=token_scale, bag=bag, out_dtype=out_dtype)
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, grad):
+            tokens, table, token_scale = ctx.saved_tensors
+            scale, bag, vocab, dtype = ctx.rest
+            grad, d_table, d_scale = grad.contiguous(), None, None
+            if ctx.needs_input_grad[1]:
+                d_table = embedding_backward(grad, tokens, vocab, scale=scale, token_scale=token_scale, bag=bag,
+                                             out_dtype=dtype)
+            if ctx.needs_input_grad[2]:
+                d_scale = embedding_scale_backward(grad, tokens, table, scale=scale, bag=bag)
+            return None, d_table, d_scale, None, None, None
+
+    class LayerNorm(Function):
+        @staticmethod
+        def forward(ctx, x, weight, bias, eps):
+            y, mean, rstd = layer_norm(x, weight, bias, eps=eps)
+            ctx.save_for_backward(x, weight, mean, rstd)
+            ctx.bias_type = None if bias is None else bias.dtype
+            ctx.mark_non_differentiable(mean, rstd)
+            ctx.set_materialize_grads(False)
+            return y, mean, rstd
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, grad, _mean, _rstd):
+            if grad is None:
+                return None, None, None, None
+            x, weight, mean, rstd = ctx.saved_tensors
+            of_bias = ctx.needs_input_grad[2]
+            dbias = x.new_empty(x.shape[-1], dtype=ctx.bias_type) if of_bias and weight is None else None
+            dx, dweight, dbias = layer_norm_backward(grad.contiguous(), x, mean, rstd, weight, bias_grad=of_bias,
+                                                     dbias=dbias)
+            return dx, dweight, dbias, None
+
+    return {"embedding": Embedding, "layer_norm": LayerNorm}
+
+
 # The calls below take contiguous tensors of one device a short way, which asks
 # only what such tensors can be wrong in: a small call's time is mostly Python's.
 # Where that way finds anything else it gives None (or _Long), and the long way
@@ -369,6 +450,9 @@ def _short_way(f):
 def _embedding_short(tokens, table, scale, token_scale, bag, out_dtype):
     device = table.get_device()
     if device < 0 or table.dim() != 2:
+        return None
+    if (table.requires_grad or (token_scale is not None and token_scale.requires_grad)) and \
+            _tracked(table, token_scale):
         return None
     w, code = _plain(table, device)
     k, k_code = _plain(tokens, device)
@@ -448,14 +532,20 @@ def _layer_norm_short(x, weight, bias, eps):
     device = x.get_device()
     if device < 0:
         return None
+    if x.requires_grad and _tracked(x):
+        return None
     v, code = _plain(x, device)
     shape = x.shape
     dim = shape[-1]
     w = b = 0
     param = _F32
     if weight is not None:
+        if weight.requires_grad and _tracked(weight):
+            return None
         w, param = _plain(weight, device, dim)
     if bias is not None:
+        if bias.requires_grad and _tracked(bias):
+            return None
         b, b_code = _plain(bias, device, dim)
         if weight is not None and b_code != param:
             return None
@@ -512,7 +602,7 @@ def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None
     zeros); one past the table makes its row NaN. token_scale (float32)
     broadcasts to the tokens' shape. Sums are float32. The result has the
     table's type, or `out_dtype`; of the two types one is float32 or both are
-    the same."""
+    the same. Torch's autograd gets the gradients of table and token_scale."""
     if stream is not None and _tensors(tokens, table, token_scale, out):
         with _on(stream, (tokens, table, token_scale, out)):
             return embedding(tokens, table, scale=scale, token_scale=token_scale, bag=bag, out=out,
@@ -521,6 +611,9 @@ def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None
         got = _embedding_short(tokens, table, scale, token_scale, bag, out_dtype)
         if got is not None:
             return got
+    if _tracked(table, token_scale):
+        return _recorded("embedding", (tokens, table, _expand(token_scale, _view(tokens, "tokens")[1])), (out,), scale,
+                         bag, out_dtype)
     k, w = _view(tokens, "tokens"), _view(table, "table")
     rows, per_row, stride_row, stride_col, lead = _token_grid(k, bag)
     vocab, dim, table_stride = _matrix(w, "table")
@@ -617,7 +710,8 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
     """(y, mean, rstd) of a layer norm over x's last dimension: y = (x - mean)
     * rstd * weight + bias in x's type, mean and rstd = 1 / sqrt(variance +
     eps) in float32, one a row. weight and bias have x's type or are float32,
-    both the same."""
+    both the same. Torch's autograd gets y's gradients with respect to x, weight
+    and bias; mean and rstd have none."""
     if stream is not None and _tensors(x, weight, bias, out, mean, rstd):
         with _on(stream, (x, weight, bias, out, mean, rstd)):
             return layer_norm(x, weight, bias, eps=eps, out=out, mean=mean, rstd=rstd)
@@ -625,6 +719,8 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
         got = _layer_norm_short(x, weight, bias, eps)
         if got is not None:
             return got
+    if _tracked(x, weight, bias):
+        return _recorded("layer_norm", (x, weight, bias), (out, mean, rstd), eps)
     v = _view(x, "x")
     rows, dim, stride = _matrix(v, "x")
     w = b = None
