@@ -1,5 +1,6 @@
 """Forms of xgboost.nn's operators that the grids of test_nn_gpu.py leave out,
 against the same 64-bit forms and bounds."""
+import numpy as np
 import pytest
 import torch
 
@@ -107,3 +108,19 @@ def test_autograd_on_another_stream_and_its_refusals():
     dx, = torch.autograd.grad(nn.layer_norm(x)[0].sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):  # not differentiated again
         dx.sum().backward()
+
+
+def test_the_modules_first_example_runs():
+    rng = np.random.default_rng(8)
+    X = rng.normal(size=(300, 4)).astype(np.float32)
+    d = xgb.DMatrix(X, label=X[:, 0])
+    g = torch.Generator().manual_seed(8)
+    names = {"xgboost": xgb, "torch": torch, "dmatrix": d, "table": _randn(g, 5 * 8, 16), "weight": _randn(g, 16),
+             "bias": _randn(g, 16),
+             "booster": xgb.train({"tree_method": "hist", "device": "cuda", "max_depth": 3}, d, 5)}
+    lines = [line.strip() for line in nn.__doc__.splitlines() if line.startswith("    ")]
+    assert len(lines) >= 3
+    exec("\n".join(lines), names)
+    assert names["vocab"] <= 5 * 8
+    R.close(names["h"], R.bag(names["tokens"], names["table"]))
+    R.close(names["y"], R.norm(names["h"], names["weight"], names["bias"])[0])

@@ -3,8 +3,9 @@
 Every leaf of every tree is a token, a row's leaves are its bag of tokens, and
 each token has a learned vector:
 
-    tokens, vocab = xgboost.nn.leaf_tokens(booster, dmatrix)   # int32 [rows, trees]
-    h = xgboost.nn.embedding(tokens, table, bag=True)          # [rows, dim]
+    tokens, vocab = xgboost.nn.leaf_tokens(booster, dmatrix)   # int32 [rows, trees], on the host
+    tokens = torch.from_numpy(tokens).cuda()
+    h = xgboost.nn.embedding(tokens, table, bag=True)          # [rows, dim] of a table [vocab, dim]
     y, mean, rstd = xgboost.nn.layer_norm(h, weight, bias)
 
 with the gradients `embedding_backward`, `embedding_scale_backward` and
