@@ -124,3 +124,20 @@ def test_the_modules_first_example_runs():
     assert names["vocab"] <= 5 * 8
     R.close(names["h"], R.bag(names["tokens"], names["table"]))
     R.close(names["y"], R.norm(names["h"], names["weight"], names["bias"])[0])
+
+
+@pytest.mark.parametrize("scales", [(4, 5), (5,), (6, 1, 5), (6, 4, 1), (1,), (4, 1)])
+@pytest.mark.parametrize("bag", [False, True])
+def test_scales_that_broadcast_over_leading_dimensions(scales, bag):
+    g = torch.Generator().manual_seed(9)
+    tokens, table = torch.randint(-1, 30, (6, 4, 5), generator=g).to(DEV), _randn(g, 30, 8)
+    s, per_row = _randn(g, *scales), 5 if bag else 1
+    rows = 120 // per_row
+    k, f = tokens.reshape(rows, per_row), s.expand(6, 4, 5).reshape(rows, per_row)
+    y = nn.embedding(tokens, table, bag=bag, token_scale=s)
+    R.close(y.reshape(rows, 8), R.bag(k, table, 1.0, f))
+    grad = _randn(g, *y.shape)
+    R.close(nn.embedding_backward(grad, tokens, 30, bag=bag, token_scale=s),
+            R.bag_grad(grad.reshape(rows, 8), k, 30, 1.0, f))
+    leaf = s.clone().requires_grad_()
+    assert torch.equal(nn.embedding(tokens, table, bag=bag, token_scale=leaf).detach(), y)

@@ -161,22 +161,27 @@ def _token_grid(v, bag):
     return rows, shape[-1], stride, strides[-1], shape[:-1]
 
 
-def _expand(scale, shape):
-    """token_scale broadcast to the tokens' shape, where it can tell how."""
-    if hasattr(scale, "expand") and scale.shape != shape:
+def _expand(scale, shape, bag):
+    """token_scale broadcast to the tokens' shape, where it can tell how; as a copy
+    where one stride cannot walk it. The caller holds it until the call is made."""
+    if hasattr(scale, "expand"):
         try:
-            return scale.expand(shape)
+            if scale.shape != shape:
+                scale = scale.expand(shape)
+            lead = len(shape) - bool(bag)
+            _flat(scale.shape[:lead], scale.stride()[:lead], "token_scale")
         except RuntimeError as e:
             raise XGBoostError("token_scale does not broadcast to the tokens' shape: %s" % e) from None
+        except XGBoostError:
+            scale = scale.contiguous()
     return scale
 
 
 def _scale_grid(scale, tokens, bag):
-    """(pointer, row stride, column stride, device) of token_scale, broadcast to
-    the tokens' shape."""
+    """(pointer, row stride, column stride, device) of token_scale in the tokens'
+    shape."""
     if scale is None:
         return 0, 0, 0, -1
-    scale = _expand(scale, tokens[1])
     ptr, shape, strides, code, device, _ = _view(scale, "token_scale")
     if tuple(shape) != tuple(tokens[1]):
         raise XGBoostError("token_scale must have the tokens' shape")
@@ -613,13 +618,14 @@ def embedding(tokens, table, *, scale=1.0, token_scale=None, bag=False, out=None
         if got is not None:
             return got
     if _tracked(table, token_scale):
-        return _recorded("embedding", (tokens, table, _expand(token_scale, _view(tokens, "tokens")[1])), (out,), scale,
-                         bag, out_dtype)
+        return _recorded("embedding", (tokens, table, _expand(token_scale, _view(tokens, "tokens")[1], bag)), (out,),
+                         scale, bag, out_dtype)
     k, w = _view(tokens, "tokens"), _view(table, "table")
     rows, per_row, stride_row, stride_col, lead = _token_grid(k, bag)
     vocab, dim, table_stride = _matrix(w, "table")
     if len(w[1]) != 2:
         raise XGBoostError("table must have two dimensions")
+    token_scale = _expand(token_scale, k[1], bag)
     s, s_row, s_col, s_device = _scale_grid(token_scale, k, bag)
     code = w[3] if out_dtype is None else _dtype_code(out_dtype)
     out, y, code, y_stride, y_device = _result(out, (*lead, dim), 0 if out is not None and out_dtype is None else code,
@@ -662,6 +668,7 @@ def embedding_backward(grad, tokens, vocab, *, scale=1.0, token_scale=None, bag=
         raise XGBoostError("grad must have the shape of the lookup's result")
     if accumulate and out is None:
         raise XGBoostError("accumulate needs out")
+    token_scale = _expand(token_scale, k[1], bag)
     s, s_row, s_col, s_device = _scale_grid(token_scale, k, bag)
     size = embedding_backward_workspace(rows, per_row, vocab, dim)
     code = g[3] if out_dtype is None else _dtype_code(out_dtype)
