@@ -4,6 +4,7 @@ methods, and what would be handed to the library is recorded instead."""
 import struct
 import sys
 
+import numpy as np
 import pytest
 import torch
 
@@ -239,3 +240,23 @@ def test_what_takes_no_part_in_automatic_differentiation(enqueued):
         for call in refused:
             call()
     assert len(enqueued) == 2
+
+
+def test_out_dtype_is_looked_at_where_out_is_given(enqueued, monkeypatch):
+    def calls(**more):
+        yield lambda: nn.embedding(Array(3, typestr="<i4"), Array(4, 2), out=Array(3, 2, ptr=8192), **more)
+        yield lambda: nn.embedding_backward(Array(3, 2), Array(3, typestr="<i4"), 4, out=Array(4, 2, ptr=8192), **more)
+
+    monkeypatch.setattr(nn, "_codes", {})  # as before the first tensor
+    for dtype in (torch.float64, torch.int32, np.float64, "int8", object()):
+        for call in calls(out_dtype=dtype):
+            with pytest.raises(xgb.XGBoostError, match="out_dtype must be"):
+                call()
+    for call in calls(out_dtype=torch.float16):
+        with pytest.raises(xgb.XGBoostError, match="another type"):
+            call()
+    assert not enqueued
+    for dtype in (torch.float32, np.float32, "float32"):
+        for call in calls(out_dtype=dtype):
+            call()
+    assert len(enqueued) == 6

@@ -255,12 +255,16 @@ def _on(stream, tensors):
 
 
 def _dtype_code(dtype):
-    if dtype in _codes:
-        return _codes[dtype]
+    """The code of a given out_dtype, one of a float type."""
+    if not _codes and "torch" in sys.modules:
+        _know_torch()
     try:
-        return _TYPESTR.get(np.dtype(dtype).str, 0)
+        code = _codes[dtype] if dtype in _codes else _TYPESTR.get(np.dtype(dtype).str, 0)
     except TypeError:
-        return 0
+        code = 0
+    if code not in _FLOATS:
+        raise XGBoostError("out_dtype must be float32, float16 or bfloat16")
+    return code
 
 
 def _new(shape, code, like, what):
