@@ -737,12 +737,12 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   constexpr int U = 4, kBatch = 8;
   extern __shared__ __align__(16) uint32_t space[];
   __shared__ uint32_t warp_sums[kFewWarps];
-  // While sorting, counts and masks; then sums that came in and sums that go on, [threads][VE] each.
+  // While sorting, counts and masks; then the sums that came in from the group before, [threads][VE].
   uint32_t* const counts = space;
   uint32_t* const masks = space + kFewCounts / 4;
   float* const head = reinterpret_cast<float*>(space);
-  float* const tail = head + kFewThreads * VE;
-  uint32_t* const zeros = space + max(2 * kFewThreads * VE, int(2 * kFewCounts / 4));
+  static_assert(kFewThreads * VE * 4 <= 2 * kFewCounts, "head in the place of counts and masks");
+  uint32_t* const zeros = space + 2 * kFewCounts / 4;
   const uint32_t span = (src.vocab + blocks.d - 1) / blocks.d;  // rows of a block, at most
   const uint32_t rows_here = (src.vocab - blockIdx.x + blocks.d - 1) / blocks.d;
   uint32_t* const present = zeros + (bulk ? kZeroBytes / 4 : 0);  // a bit a row
@@ -908,11 +908,10 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const bool goes_on = current >= 0 && current == after;
   if (current >= 0) {
     if (from_before) store<float, VE>(head + threadIdx.x * VE, sum);
-    else if (goes_on) store<float, VE>(tail + threadIdx.x * VE, sum);
-    else write(current, sum);
+    else if (!goes_on) write(current, sum);
   }
   __syncthreads();
-  // The group in whose share a row began joins it.
+  // The group in whose share a row began joins it, from what it holds of it.
   if (goes_on && !from_before) {
     uint32_t lo = end, hi = count;  // the first entry of a later row
     while (lo < hi) {
@@ -940,21 +939,20 @@ int64_t token_step(const Tokens& k) {
 
 // Shared memory of few_kernel, and its grid: blocks and column tiles.
 struct FewPlan {
-  // Of the widest pieces, all tokens and 65536 rows a block.
-  static constexpr size_t kMostShared = std::max<size_t>(2 * kFewThreads * 8 * 4, 2 * kFewCounts) + kZeroBytes +
-                                        65536 / 8 + size_t(2) * 4 * kFewTokens;
+  // Of the most tokens and 65536 rows a block.
+  static constexpr size_t kMostShared = 2 * kFewCounts + kZeroBytes + 65536 / 8 + size_t(2) * 4 * kFewTokens;
   int lg = 0;
   uint32_t tiles, blocks;
   size_t shared;
-  FewPlan(uint32_t n, uint64_t vocab, uint64_t pieces, int ve, bool bulk) {
+  FewPlan(uint32_t n, uint64_t vocab, uint64_t pieces, bool bulk) {
     while (lg < 5 && (1ull << lg) < pieces) ++lg;
     tiles = blocks_for(pieces, 1u << lg);
     // About two blocks an SM, which all read all tokens; a row's number takes 16 bits.
     const uint64_t want = std::max<uint64_t>(std::max<uint64_t>(1, 296 / tiles), (vocab + 65535) / 65536);
     blocks = uint32_t(std::min(want, vocab));
     const uint64_t span = (vocab + blocks - 1) / blocks;
-    shared = std::max<size_t>(2 * kFewThreads * ve * 4, 2 * kFewCounts) + (bulk ? kZeroBytes : 0) +
-             (span + 31) / 32 * 4 + size_t(2) * 4 * ((n + kFewThreads - 1) / kFewThreads * kFewThreads);
+    shared = 2 * kFewCounts + (bulk ? kZeroBytes : 0) + (span + 31) / 32 * 4 +
+             size_t(2) * 4 * ((n + kFewThreads - 1) / kFewThreads * kFewThreads);
   }
 };
 
@@ -1049,7 +1047,7 @@ void embedding_backward(const Mat& grad, const Tokens& k, uint64_t vocab, uint64
       }
       const bool bulk = !accumulate && bulk_rows(out, vocab, dim);
       if (n <= kFewTokens) {
-        const FewPlan plan(n, vocab, pieces, VE, bulk);
+        const FewPlan plan(n, vocab, pieces, bulk);
         const auto kernel = s.data ? few_kernel<T, O, VE, true> : few_kernel<T, O, VE, false>;
         allow_shared(kernel, plan.shared, FewPlan::kMostShared);
         kernel<<<dim3(plan.blocks, plan.tiles), kFewThreads, plan.shared, stream>>>(
