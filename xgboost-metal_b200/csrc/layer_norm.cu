@@ -801,7 +801,8 @@ bool param_aligned(const void* p, size_t size, uint64_t n) {
   return reinterpret_cast<uintptr_t>(p) % std::min<size_t>(32, n * size) == 0;
 }
 
-// Calls f with the widest VE that every matrix and vector allows.
+// Calls f with the widest VE that every matrix and vector allows: 16 bytes of T,
+// a pair of 16-bit values, or one value.
 template <class T, class F>
 void with_norm_width(std::initializer_list<Mat> mats, std::initializer_list<const void*> vectors, int param_type,
                      uint64_t rows, uint64_t dim, F&& f) {
@@ -812,9 +813,11 @@ void with_norm_width(std::initializer_list<Mat> mats, std::initializer_list<cons
     return ok;
   };
   constexpr int kWide = 16 / sizeof(T);
-  if (fits(kWide)) f(std::integral_constant<int, kWide>());
-  else if (kWide > 4 && fits(2)) f(std::integral_constant<int, kWide == 4 ? 1 : 2>());
-  else f(std::integral_constant<int, 1>());
+  if (fits(kWide)) return f(std::integral_constant<int, kWide>());
+  if constexpr (kWide > 4) {
+    if (fits(2)) return f(std::integral_constant<int, 2>());
+  }
+  f(std::integral_constant<int, 1>());
 }
 
 // What a launch may ask for: the stream kernels' ring, at its largest.

@@ -264,7 +264,6 @@ void with_type(int type, F&& f) {
   else f(static_cast<__nv_bfloat16*>(nullptr));
 }
 // The same for a pair (a, b): equal, or one of them float.
-inline bool pairs_up(int a, int b) { return a == b || a == kF32 || b == kF32; }
 template <class F>
 void with_types(int a, int b, F&& f) {
   with_type(a, [&](auto* pa) {
@@ -292,10 +291,12 @@ void with_width(const Mat& a, uint64_t a_rows, const Mat& b, uint64_t b_rows, ui
            row_aligned(b.data, b.stride, b_rows, type_size(b.type), n);
   };
   constexpr int kWide = 16 / sizeof(T);
-  if (fits(kWide)) f(std::integral_constant<int, kWide>());
-  else if (kWide > 4 && fits(4)) f(std::integral_constant<int, 4>());
-  else if (kWide > 4 && fits(2)) f(std::integral_constant<int, kWide == 4 ? 1 : 2>());
-  else f(std::integral_constant<int, 1>());
+  if (fits(kWide)) return f(std::integral_constant<int, kWide>());
+  if constexpr (kWide > 4) {
+    if (fits(4)) return f(std::integral_constant<int, 4>());
+    if (fits(2)) return f(std::integral_constant<int, 2>());
+  }
+  f(std::integral_constant<int, 1>());
 }
 
 }  // namespace xgbb::nn
