@@ -1,7 +1,10 @@
 """What xgboost.nn's Python layer makes of the arrays that it is given: their
 devices, streams and flags. Without a GPU: tensors are stand-ins with torch's
 methods, and what would be handed to the library is recorded instead."""
+import os
+import re
 import struct
+import subprocess
 import sys
 
 import numpy as np
@@ -260,3 +263,40 @@ def test_out_dtype_is_looked_at_where_out_is_given(enqueued, monkeypatch):
         for call in calls(out_dtype=dtype):
             call()
     assert len(enqueued) == 6
+
+
+STRUCTS = {"XGBBEmbeddingArgs": nn._pack_embedding, "XGBBEmbeddingBackwardArgs": nn._pack_embedding_backward,
+           "XGBBEmbeddingScaleBackwardArgs": nn._pack_embedding_scale_backward, "XGBBLayerNormArgs": nn._pack_layer_norm,
+           "XGBBLayerNormBackwardArgs": nn._pack_layer_norm_backward}
+
+
+def _fields(header, name):
+    body = re.search(r"typedef struct \{([^}]*)\} %s;" % name, header).group(1)
+    for names in re.findall(r"[\s*](\w+(?:, \w+)*);", body):
+        yield from names.split(", ")
+
+
+def test_every_argument_lies_where_the_header_has_it(tmp_path):
+    """Each field of each structure packed with a value of its own, and read back by a C program by its name."""
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    with open(os.path.join(include, "xgb_b200.h")) as f:
+        header = f.read()
+    inner, lines, want = ["tokens." + f for f in _fields(header, "XGBBTokens")], [], []
+    for at, (name, pack) in enumerate(STRUCTS.items()):
+        fields = [f for field in _fields(header, name) for f in (inner if field == "tokens" else [field])]
+        values = [100 + i for i in range(len(fields))]
+        data = tmp_path / name
+        data.write_bytes(pack(*values))
+        want += values
+        lines.append('{ %s a; FILE* f = fopen("%s", "rb"); if (fread(&a, 1, sizeof a + 1, f) != sizeof a) return %d;' %
+                     (name, data, at + 1))
+        lines += ['printf("%%.0f ", (double)%sa.%s);' % ("" if f in ("tokens.scale", "eps") else "(uint64_t)", f)
+                  for f in fields]
+        lines.append("fclose(f); }")
+    source = tmp_path / "read.c"
+    source.write_text("#include <stdio.h>\n#include <string.h>\n#include \"xgb_b200.h\"\nint main(void) {\n%s\nreturn 0; }" %
+                      "\n".join(lines))
+    program = str(tmp_path / "read")
+    subprocess.run(["gcc", "-I", include, str(source), "-o", program], check=True)
+    got = subprocess.run([program], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(v) for v in got] == want

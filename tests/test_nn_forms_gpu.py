@@ -141,3 +141,77 @@ def test_scales_that_broadcast_over_leading_dimensions(scales, bag):
             R.bag_grad(grad.reshape(rows, 8), k, 30, 1.0, f))
     leaf = s.clone().requires_grad_()
     assert torch.equal(nn.embedding(tokens, table, bag=bag, token_scale=leaf).detach(), y)
+
+
+def _norm_case(g, rows, dim, a, p, has, pad):
+    x, grad = (_randn(g, rows, dim + pad, dtype=a)[:, :dim] for _ in range(2))
+    w, b = _randn(g, dim, dtype=p) if "w" in has else None, _randn(g, dim, dtype=p) if "b" in has else None
+    y = torch.full((rows, dim + pad), 7.0, dtype=a, device=DEV)
+    dx = y.clone()
+    got, mean, rstd = nn.layer_norm(x, w, b, out=y[:, :dim])
+    for value, want, what in zip((got, mean, rstd), R.norm(x, w, b), ("y", "mean", "rstd")):
+        R.close(value, want, what)
+    db = torch.full((dim,), 7.0, dtype=p, device=DEV) if b is not None else None
+    got, dw, db = nn.layer_norm_backward(grad, x, mean, rstd, w, out=dx[:, :dim], dbias=db, bias_grad=b is not None)
+    want = R.norm_grad(grad, x, mean, rstd, w, p)
+    R.close(got, want[0], "dx")
+    assert (dw is None) == (w is None) and (db is None) == (b is None)
+    if w is not None:
+        R.close(dw, want[1], "dweight")
+    if b is not None:
+        R.close(db, want[2], "dbias")
+    assert (y[:, dim:] == 7).all() and (dx[:, dim:] == 7).all()  # what lies between the rows stays
+
+
+# The forms of many rows: a warp's lanes, a warp; streams of a block, of whole and of partly filled ones, of 32 threads
+# and of 1024; clusters of two, four and eight; parts of a block where there are few.
+@pytest.mark.parametrize("has", ["wb", "w", "b", ""])
+@pytest.mark.parametrize("rows,dim,a,p,pad", [
+    (2401, 64, BF16, F32, 8), (2403, 512, F32, F32, 4), (2402, 1024, F16, F16, 8), (9473, 1000, BF16, BF16, 8),
+    (2369, 4096, BF16, F32, 8), (2371, 3080, F32, F32, 4), (1190, 8192, BF16, F32, 8), (600, 16000, F16, F32, 16),
+    (260, 32768, BF16, BF16, 8), (2400, 777, BF16, F32, 3), (40, 1024, BF16, F32, 8)])
+def test_many_padded_rows_with_and_without_weight_and_bias(rows, dim, a, p, pad, has):
+    _norm_case(torch.Generator().manual_seed(rows + dim), rows, dim, a, p, has, pad)
+
+
+@pytest.mark.parametrize("has", ["b", ""])
+@pytest.mark.parametrize("rows,dim,a", [(5, 64, F32), (3, 1001, F16), (2, 16385, BF16), (1, 40001, F32)])
+def test_few_rows_without_a_weight(rows, dim, a, has):
+    _norm_case(torch.Generator().manual_seed(rows + dim), rows, dim, a, a, has, 0)
+
+
+# One block sorts and the others zero absent rows: 12 or 24 entries a thread, rows of plain stores of 4 and 2 bytes and
+# of whole copies, tokens of both types, with and without scales.
+@pytest.mark.parametrize("n,per_row,vocab,dim,a,b,index,scaled", [
+    (9000, 1, 1100003, 33, F32, F32, torch.int32, False), (20000, 4, 1920001, 35, BF16, BF16, torch.int64, True),
+    (12288, 3, 33001, 1028, F16, F32, torch.int64, True), (12289, 1, 140003, 256, F32, F32, torch.int64, False)])
+def test_gradient_sorted_beside_the_zeros(n, per_row, vocab, dim, a, b, index, scaled):
+    assert vocab * dim * b.itemsize >= 128 << 20
+    g = torch.Generator().manual_seed(n)
+    rows = n // per_row
+    tokens = torch.randint(-vocab // 8, vocab, (rows, per_row), generator=g)
+    tokens[: rows // 3] %= 5
+    tokens, grad = tokens.to(index).to(DEV), _randn(g, rows, dim, dtype=a)
+    s = _randn(g, rows, per_row) if scaled else None
+    out = torch.full((vocab, dim), 7.0, dtype=b, device=DEV)
+    nn.embedding_backward(grad, tokens, vocab, bag=True, scale=0.3, token_scale=s, out=out)
+    # The rows that have tokens, by their order, and all others zero.
+    present, k = torch.unique(tokens[tokens >= 0].cpu(), return_inverse=True)
+    dense = torch.full((rows, per_row), -1, dtype=torch.int64)
+    dense[tokens.cpu() >= 0] = k
+    R.close(out[present.to(DEV)], R.bag_grad(grad, dense, len(present), 0.3, s, b))
+    out[present.to(DEV)] = 0
+    assert not out.any()
+
+
+@pytest.mark.parametrize("n,vocab,dim", [(300, 50, 40), (9000, 70000, 40), (30000, 300, 40), (9000, 1100003, 33),
+                                         (9000, 40000, 1024)])
+def test_gradient_of_tokens_of_which_none_is_there(n, vocab, dim):
+    grad = torch.full((n, dim), float("nan"), device=DEV)
+    for nothing in (-1, vocab):
+        tokens = torch.full((n,), nothing, dtype=torch.int32, device=DEV)
+        out = torch.full((vocab, dim), 7.0, device=DEV)
+        assert not nn.embedding_backward(grad, tokens, vocab, out=out).any()
+        out.fill_(3.0)
+        nn.embedding_backward(grad, tokens, vocab, out=out, accumulate=True)
+        assert (out == 3).all()
