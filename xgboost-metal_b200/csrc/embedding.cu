@@ -295,8 +295,10 @@ void embedding(const Tokens& k, const Mat& table, uint64_t vocab, uint64_t dim, 
       // of the block, down to 8 tokens a group.
       int ls = 0;
       while (lg + ls < 8 && k.rows * tiles << (lg + ls) < 148 * 1024 && k.per_row >> (ls + 1) >= 8) ++ls;
-      // And over clusters, where a group still has over 16 and eight blocks an SM
-      // hold them all. (100000 bags of 50 x 8 in clusters: 216 us for 33.)
+      // And over clusters, where a group still has over 16 and the clusters' blocks
+      // are eight an SM at most, two to four turns of what an SM holds of them.
+      // (7 bags of 2000 x 33: 20.6 us without, 5.0 in clusters; 100000 bags of 50 x 8
+      // in clusters: 216 us for 33.)
       const uint64_t blocks = blocks_for(k.rows, kThreads >> (lg + ls));
       const unsigned cluster = ls && k.per_row >> ls > 16 && blocks * tiles * 8 <= 148 * 8 ? 8 : 1;
       const dim3 grid(unsigned(blocks * cluster), tiles);

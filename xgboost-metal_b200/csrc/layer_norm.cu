@@ -863,7 +863,9 @@ struct GradPlan {
     if (warp) {
       while ((8ull << lg) < dim) ++lg;
       threads = kThreads;
-      // Up to eight turns of eight blocks: one cluster, and one launch.
+      // Up to eight turns of eight blocks: one cluster, one launch and no workspace.
+      // 512 x 64 f32, two turns: 4.5 us for 4.8 in parts; 2048 x 64, eight: 9.0 for
+      // 5.0, but a call from Python takes 11.5 us for 15.6.
       const uint64_t once = kThreads >> lg;
       if (rows <= once * 64) {
         one = true;
@@ -885,6 +887,9 @@ struct GradPlan {
     if (!ring) return;
     ring_threads = uint32_t((dim + 256 * ring - 1) / (256 * ring) * 32);
     ring_blocks = ring == 1 ? 148 * (512 / ring_threads) : ring == 2 ? 148 : 128;
+    // The stream from 16 rows a block or cluster on. A row a block at a time takes
+    // 24.8 us for 14.7 at 2368 x 4096 bf16, where it begins, and 10.2 for 8.8 at 592;
+    // 9.6 for 8.4 at 2368 x 1024, 6.7 for 7.4 at 592.
     if (rows < uint64_t(ring_blocks / ring) * 16) ring = 0;
   }
   uint32_t parts() const { return one ? 0 : ring ? std::max(blocks, ring_blocks / ring) : blocks; }
@@ -921,6 +926,9 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
           }
         }
       };
+      // Rows of up to 512 pieces in lanes of a warp, where there is one for each SM.
+      // Fewer go faster in a block each: 74 x 255 f32 take 2.3 us for 3.3, and 2368 x 255
+      // 3.5 for 3.5, 37888 x 255 22.3 for 14.9.
       if (pieces <= 32 * kMost && pieces <= 512 && rows >= 148) {
         int lg = 0;
         while (lg < 5 && (uint64_t(kSome) << lg) < pieces) ++lg;
@@ -944,6 +952,9 @@ void layer_norm(const Mat& x, uint64_t rows, uint64_t dim, const void* weight, c
                       148 * (MOST / threads), threads, size_t(2) * R * CH * threads * 16, stream, in, x.stride,
                       uint32_t(rows), uint32_t(dim), w, b, eps, out, y.stride, mean, rstd);
         };
+        // The stream from 16 rows an SM on: 2368 x 4096 bf16 in 7.4 us for 12.2 with a
+        // block a row, 592 rows 4.5 for 4.4. (float32: 32768 x 8192 in 362 for 358, 4096
+        // columns 186 for 155.)
         if (rows >= 148 * 16 && param_aligned(weight, 32, 1) && param_aligned(bias, 32, 1)) {
           if (threads <= 512) return ring(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
           if (threads <= 1024) return ring(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
