@@ -144,3 +144,18 @@ def test_arrays_that_are_filled_on_another_stream():
         other.replay()
         torch.cuda.synchronize()
         R.close(y, R.norm(filled)[0])
+
+
+def test_a_refused_call_leaves_nothing_to_the_next():
+    x, y = torch.randn(3, 8, device=DEV), torch.empty(3, 8, device=DEV)
+
+    def call(device):
+        return _LIB.XGBBLayerNorm(nn._pack_layer_norm(x.data_ptr(), 0, 0, y.data_ptr(), 0, 0, 0, 3, 8, 8, 8, 1, 1, device,
+                                                      1e-5))
+
+    torch.cuda.synchronize()
+    for _ in range(2):
+        assert call(99) == -1 and "device" in _LIB.XGBGetLastError().decode()
+        assert call(0) == 0, _LIB.XGBGetLastError().decode()
+    torch.cuda.synchronize()
+    R.close(y, R.norm(x)[0])

@@ -26,8 +26,12 @@ inline void require(bool ok, const char* message) {
   if (!ok) throw Error(message);
 }
 
+// The error is told here: it does not stay the thread's last one, which the next
+// call would find behind its own launches.
 inline void cuda_check(cudaError_t e, const char* what) {
-  if (e != cudaSuccess) throw Error(std::string(what) + ": " + cudaGetErrorString(e));
+  if (e == cudaSuccess) return;
+  cudaGetLastError();
+  throw Error(std::string(what) + ": " + cudaGetErrorString(e));
 }
 #define XGBB_CUDA(call) ::xgbb::cuda_check((call), #call)
 
