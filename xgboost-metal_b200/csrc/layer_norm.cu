@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(MOST, PLACE != kBlock && VE * sizeof(T) == 16 
 // in a cluster each block leaves its warps' sums with all blocks. The next R
 // rows are under way into shared memory. Bound by device memory: 32768 x 4096 bf16
 // in 127 us, 97 % of the copy rate (179 us a row at a time); in clusters by their
-// barriers (16384 x 8192: 176 us, 70 %; 8000 x 16384: 227 us, 53 %).
+// barriers (16384 x 8192: 164 us, 75 %; 8000 x 16384: 221 us, 54 %).
 template <class T, class P, int R, int C, bool FULL>
 __global__ void __launch_bounds__(512, 1)
     norm_grad_rows_kernel(const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ x,
