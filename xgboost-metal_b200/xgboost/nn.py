@@ -20,7 +20,8 @@ Work is enqueued and not waited for: on `stream` where one is given (a handle,
 or an object that has one as `cuda_stream` or `ptr`), else on torch's current
 stream of the arrays' device where one of them is a tensor, else on the default
 stream. It runs after what is enqueued on the streams that the arrays'
-interfaces name. Equal inputs give equal bits. These functions have no counterpart in the reference.
+interfaces name. Equal inputs give equal bits. These functions have no
+counterpart in the reference.
 """
 import contextlib
 import ctypes
@@ -755,8 +756,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, mean=None, rstd
     device = _one_device(v[4], w_device, b_device, y_device, m_device, q_device)
     handle = _handle(stream, device, x, weight, bias, out, mean, rstd)
     _call(_LIB.XGBBLayerNorm, _pack_layer_norm(
-        v[0], w or 0, b or 0, y, m, q, handle, rows, dim, stride, y_stride, v[3], param, device,
-        eps))
+        v[0], w or 0, b or 0, y, m, q, handle, rows, dim, stride, y_stride, v[3], param, device, eps))
     return out, mean, rstd
 
 
